@@ -282,6 +282,36 @@ int mk_qkv_rope_paged_update_quant(const void* qkv, const float* cos_t, const fl
                                    int64_t num_pages, int64_t cos_rows, int64_t group_size,
                                    int bits, int dtype, void* stream);
 
+/* Rotary positions of x [B,S,H,D] (values; its last dimension dense, the others
+ * at the given strides in values) into a dense y -- ops/rope_ops.py:61-75 for
+ * layout 0 (pairs (2i, 2i+1)) with rotary_dim == D; layout 1 has the pairs
+ * (i, i + rotary_dim/2).  Values past rotary_dim are copied.  cos/sin
+ * [cos_rows, rotary_dim/2].  Row (b, s) stands at position_offset + s
+ * (positions NULL), positions[b] + s (per_token 0; negative: the sequence is
+ * padding) or positions[b*S + s] (per_token 1).  A row whose position is
+ * negative or outside the tables gives zeros. */
+int mk_apply_rope(const void* x, const float* cos_t, const float* sin_t, const int32_t* positions, void* y, int64_t B,
+                  int64_t S, int64_t H, int64_t D, int64_t stride_b, int64_t stride_s, int64_t stride_h,
+                  int64_t rotary_dim, int64_t position_offset, int per_token, int64_t cos_rows, int layout, int dtype,
+                  void* stream);
+
+/* RMSNorm of each q and k head (q_weight, k_weight [D] in weight_dtype; both
+ * NULL: no norm), rotary positions as mk_apply_rope, and the paged write of k
+ * and v, for the rows of a packed qkv [T, (Hq+2*Hkv)*D] at row_stride values;
+ * no counterpart in the reference (ops/gqa_ops.py:493-547 has the part without
+ * norms, interleaved).  q_out [T,Hq,D].  sequences NULL: T == B, token t is
+ * block_table row t's, and the later of two tokens of one slot wins.
+ * Otherwise token t is of row sequences[t], and two tokens of one slot race.
+ * A token with a negative position, one outside the tables or a sequence
+ * outside [0, B) gives zeros in q_out and writes nothing; one without a page
+ * writes nothing. */
+int mk_qk_norm_rope_paged_update(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight,
+                                 float eps, const float* cos_t, const float* sin_t, const int32_t* positions,
+                                 const int32_t* sequences, const int32_t* block_table, void* K_pages, void* V_pages,
+                                 void* q_out, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                 int64_t rotary_dim, int64_t page_size, int64_t max_blocks, int64_t num_pages,
+                                 int64_t cos_rows, int layout, int weight_dtype, int dtype, void* stream);
+
 /* quantize_kv_pages -- ops/paged_quantized_kv_ops.py:194-292 for one of K or V:
  * src [rows, D] (rows = num_pages*P*Hkv) -> codes [rows, D] (q8) or
  * [rows, ceil(D/2)] (q4) and fp16 scales [rows, ceil(D/g)], with the

@@ -74,6 +74,8 @@ SIGNATURES: dict[str, list] = {
     "mk_paged_kv_update": [_P, _P, _P, _P, _P, _P] + [_I64] * 6 + [_I, _P],
     "mk_qkv_rope_paged_update": [_P] * 8 + [_I64] * 8 + [_I, _P],
     "mk_qkv_rope_paged_update_quant": [_P] * 10 + [_I64] * 9 + [_I, _I, _P],
+    "mk_apply_rope": [_P] * 5 + [_I64] * 9 + [_I, _I64, _I, _I, _P],
+    "mk_qk_norm_rope_paged_update": [_P, _I64, _P, _P, _F] + [_P] * 8 + [_I64] * 10 + [_I] * 3 + [_P],
     "mk_quantize_kv": [_P, _P, _P, _I64, _I64, _I64, _I, _I, _P],
     "mk_dequantize_kv": [_P, _P, _P, _I64, _I64, _I64, _I, _P],
     "mk_paged_attention_workspace_bytes": [_I64] * 6,

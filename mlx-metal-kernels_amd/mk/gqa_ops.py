@@ -20,8 +20,8 @@ import math
 import torch
 
 from . import _contig, _lib
-from ._common import ACT_DTYPES
-from .kv_cache_ops import normalize_positions, reference_kv_cache_update
+from ._common import ACT_DTYPES, ci_safe_mode_enabled
+from .kv_cache_ops import host_checks_enabled, normalize_positions, reference_kv_cache_update
 from .paged_kv_ops import (
     _gather_pages,
     _hip_paged_attention,
@@ -30,7 +30,8 @@ from .paged_kv_ops import (
     paged_kv_cache_update,
     reference_paged_kv_cache_update,
 )
-from .rope_ops import reference_apply_rope
+from .norm_ops import _NORM_DTYPES
+from .rope_ops import _layout_code, _rotary_dim, _rotate, _tables, reference_apply_rope
 
 
 def validate_gqa_heads(num_attention_heads: int, num_key_value_heads: int) -> None:
@@ -268,6 +269,176 @@ def paged_gqa_decode_block_from_qkv(qkv, K_pages, V_pages, block_table, cos, sin
         scale = 1.0 / math.sqrt(D)
     out = _hip_paged_attention(q_out[:, 0], K_pages, V_pages, bt, pos + 1 if lengths is None else lengths, scale)
     return out.unsqueeze(1).to(qkv.dtype), K_pages, V_pages
+
+
+# ----------------------------------------------------------------- head norms, rotation, page write
+
+
+def _qk_norm_rope_prep(qkv, K_pages, V_pages, block_table, cos, sin, position, Hq, Hkv, D, q_weight, k_weight,
+                       sequences, layout, rotary_dim):
+    """Shared checks -> (qkv [T, (Hq+2Hkv)*D], positions int32 [T], sequences int32 [T] or None)."""
+    validate_gqa_heads(Hq, Hkv)
+    _layout_code(layout)
+    rd = _rotary_dim(rotary_dim, D)
+    if D % 2 != 0:
+        raise ValueError(f"RoPE requires even D, got D={D}")
+    N = (Hq + 2 * Hkv) * D
+    if qkv.ndim == 4 and tuple(qkv.shape[1:]) == (1, Hq + 2 * Hkv, D):
+        x = qkv.reshape(qkv.shape[0], N)
+    elif qkv.ndim == 3 and tuple(qkv.shape[1:]) == (1, N):
+        x = qkv[:, 0]
+    elif qkv.ndim == 2 and qkv.shape[1] == N:
+        x = qkv
+    else:
+        raise ValueError(f"qkv must have shape [T,{N}], [T,1,{N}] or [T,1,{Hq + 2 * Hkv},{D}], got {tuple(qkv.shape)}")
+    if K_pages.shape != V_pages.shape or K_pages.ndim != 4 or K_pages.shape[2] != Hkv or K_pages.shape[3] != D:
+        raise ValueError(f"K_pages/V_pages must be [NUM_PAGES,PAGE_SIZE,{Hkv},{D}], got {tuple(K_pages.shape)}, "
+                         f"{tuple(V_pages.shape)}")
+    if K_pages.dtype not in ACT_DTYPES or V_pages.dtype != K_pages.dtype:
+        raise TypeError(f"K_pages/V_pages must share a float16/bfloat16 dtype, got {K_pages.dtype}, {V_pages.dtype}")
+    if qkv.dtype != K_pages.dtype:
+        raise TypeError(f"qkv must carry the pages' dtype {K_pages.dtype}, got {qkv.dtype}")
+    if block_table.ndim != 2:
+        raise ValueError(f"block_table must be 2-D [B,MAX_BLOCKS], got {tuple(block_table.shape)}")
+    if cos.ndim != 2 or cos.shape != sin.shape or cos.shape[1] != rd // 2:
+        raise ValueError(f"cos and sin must be [rows,{rd // 2}], got {tuple(cos.shape)}, {tuple(sin.shape)}")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("give q_weight and k_weight, or neither")
+    if q_weight is not None:
+        if tuple(q_weight.shape) != (D,) or tuple(k_weight.shape) != (D,):
+            raise ValueError(f"q_weight and k_weight must have shape {(D,)}, got {tuple(q_weight.shape)}, "
+                             f"{tuple(k_weight.shape)}")
+        if q_weight.dtype not in _NORM_DTYPES or q_weight.dtype != k_weight.dtype:
+            raise TypeError("q_weight and k_weight must share a float16, bfloat16, or float32 dtype, got "
+                            f"{q_weight.dtype}, {k_weight.dtype}")
+    T, B = x.shape[0], block_table.shape[0]
+    dev = block_table.device
+    rows = min(cos.shape[0], block_table.shape[1] * K_pages.shape[1])
+    if isinstance(position, int):
+        position = torch.full((T,), position, dtype=torch.int32, device=dev)
+    elif not isinstance(position, torch.Tensor):
+        position = torch.as_tensor(position, dtype=torch.int32)
+    if position.dtype not in (torch.int32, torch.int64) or tuple(position.shape) != (T,):
+        raise ValueError(f"position must be an int or int32 [T]={(T,)}, got {position.dtype} {tuple(position.shape)}")
+    if sequences is None:
+        if T != B:
+            raise ValueError(f"qkv has {T} rows and block_table {B}: without sequences they are one to one")
+    else:
+        if not isinstance(sequences, torch.Tensor):
+            sequences = torch.as_tensor(sequences, dtype=torch.int32)
+        if sequences.dtype not in (torch.int32, torch.int64) or tuple(sequences.shape) != (T,):
+            raise ValueError(f"sequences must be int32 [T]={(T,)}, got {sequences.dtype} {tuple(sequences.shape)}")
+    if T and host_checks_enabled(position):
+        lo, hi = int(position.min()), int(position.max())
+        if lo < -1 or hi >= rows:
+            raise ValueError(f"position must be in [-1, {rows}), got {lo} to {hi}")
+        if sequences is not None:
+            s, p = sequences.cpu().long(), position.cpu().long()
+            if int(s.min()) < 0 or int(s.max()) >= B:
+                raise ValueError(f"sequences must be in [0, {B}), got {int(s.min())} to {int(s.max())}")
+            slots = _slots(p, s, block_table.cpu().long(), K_pages.shape[0], K_pages.shape[1])
+            slots = slots[slots >= 0]
+            if slots.unique().numel() != slots.numel():
+                raise ValueError("two tokens of one call have the same cache slot")
+    return x, _i32(position, dev), None if sequences is None else _i32(sequences, dev)
+
+
+def _slots(p, s, bt, num_pages, P):
+    """Cache row page * P + offset of tokens at positions p of sequences s; -1 for none (host or device, int64)."""
+    ok = (p >= 0) & (p < bt.shape[1] * P) & (s >= 0) & (s < bt.shape[0])
+    p, s = torch.where(ok, p, 0), torch.where(ok, s, 0)
+    page = bt[s, p // P]
+    return torch.where(ok & (page >= 0) & (page < num_pages), page * P + p % P, -1)
+
+
+def reference_paged_qk_norm_rope_update(qkv, K_pages, V_pages, block_table, cos, sin, position, *,
+                                        num_attention_heads, num_key_value_heads, head_dim, q_weight=None,
+                                        k_weight=None, sequences=None, eps: float = 1e-6,
+                                        layout: str = "interleaved", rotary_dim=None):
+    """``paged_qk_norm_rope_update`` with tensor ops, on copies of the pages."""
+    Hq, Hkv, D = num_attention_heads, num_key_value_heads, head_dim
+    x, pos, seq = _qk_norm_rope_prep(qkv, K_pages, V_pages, block_table, cos, sin, position, Hq, Hkv, D, q_weight,
+                                     k_weight, sequences, layout, rotary_dim)
+    T = x.shape[0]
+    x = x.reshape(T, Hq + 2 * Hkv, D)
+    p = pos.long()
+    s = torch.arange(T, device=p.device) if seq is None else seq.long()
+    live = (p >= 0) & (p < cos.shape[0]) & (s >= 0) & (s < block_table.shape[0])
+    at = torch.where(live, p, 0)
+    c, sn = cos.to(p.device)[at].float()[:, None], sin.to(p.device)[at].float()[:, None]
+    q, k = x[:, :Hq].float(), x[:, Hq:Hq + Hkv].float()
+    if q_weight is not None:
+        q = q * torch.rsqrt((q * q).mean(-1, keepdim=True) + float(eps)) * q_weight.float()
+        k = k * torch.rsqrt((k * k).mean(-1, keepdim=True) + float(eps)) * k_weight.float()
+    q = torch.where(live[:, None, None], _rotate(q, c, sn, layout), 0.0).to(x.dtype)
+    k = _rotate(k, c, sn, layout).to(x.dtype)
+    NP, P = K_pages.shape[:2]
+    slots = torch.where(live, _slots(p, s, block_table.long(), NP, P), -1)
+    K, V = K_pages.clone(), V_pages.clone()
+    for t, slot in enumerate(slots.tolist()):  # a later token of the same slot wins
+        if slot >= 0:
+            K[slot // P, slot % P] = k[t]
+            V[slot // P, slot % P] = x[t, Hq + Hkv:]
+    return q[:, None], K, V
+
+
+def paged_qk_norm_rope_update(qkv, K_pages, V_pages, block_table, cos, sin, position, *, num_attention_heads,
+                              num_key_value_heads, head_dim, q_weight=None, k_weight=None, sequences=None,
+                              eps: float = 1e-6, layout: str = "interleaved", rotary_dim=None, backend: str = "auto"):
+    """What stands between a packed qkv projection and the attention, in one
+    launch: RMSNorm of every q and k head (``q_weight``, ``k_weight`` [D]; None:
+    no norm), rotary positions in either layout over the first ``rotary_dim``
+    values (``mk.rope_ops``), and the write of k and v into the pages, in place.
+    Norm and rotation are fp32 with one rounding at the end.
+
+    qkv [T, (Hq+2Hkv)*D] (also [T,1,...] as the decode blocks take it; rows may
+    be strided) in the pages' dtype; cos, sin fp32 [rows, rotary_dim/2];
+    position int or int32 [T].  Without ``sequences`` row t is the new token of
+    block_table's row t, and the later of two rows of one slot wins.  With
+    ``sequences`` int32 [T] the rows are the tokens of prompts, in any order:
+    row t is of block_table row sequences[t], and no two rows may have the same
+    slot.  Position -1 marks an empty row: its q is zero and nothing is written.
+
+    Returns (q [T,1,Hq,D], K_pages, V_pages).  Positions, sequences and slots
+    are checked on the host unless that is off (``host_checks_enabled``); then
+    rows outside of the tables are treated as empty, page ids outside of the
+    pages are not written, and of two tokens of one slot given with
+    ``sequences`` some values of each may stay.  A contiguous cache goes
+    through ``mk._contig`` as in ``gqa_decode_block_from_qkv``.  The pages are
+    written in place, so an input that records a gradient is refused."""
+    backend_name = backend.lower()
+    if backend_name not in ("auto", "reference", "metal"):
+        raise ValueError("backend must be one of 'reference', 'metal', 'auto'")
+    if ci_safe_mode_enabled() or backend_name == "reference":
+        return reference_paged_qk_norm_rope_update(
+            qkv, K_pages, V_pages, block_table, cos, sin, position, num_attention_heads=num_attention_heads,
+            num_key_value_heads=num_key_value_heads, head_dim=head_dim, q_weight=q_weight, k_weight=k_weight,
+            sequences=sequences, eps=eps, layout=layout, rotary_dim=rotary_dim)
+    Hq, Hkv, D = num_attention_heads, num_key_value_heads, head_dim
+    x, pos, seq = _qk_norm_rope_prep(qkv, K_pages, V_pages, block_table, cos, sin, position, Hq, Hkv, D, q_weight,
+                                     k_weight, sequences, layout, rotary_dim)
+    if not (K_pages.is_contiguous() and V_pages.is_contiguous()):
+        raise ValueError("K_pages and V_pages must be contiguous for the in-place update")
+    if torch.is_grad_enabled() and (x.requires_grad or (q_weight is not None and (q_weight.requires_grad
+                                                                                  or k_weight.requires_grad))):
+        raise RuntimeError("paged_qk_norm_rope_update records no gradient; call it under torch.no_grad()")
+    dev = _lib.require_device(x, K_pages, V_pages, block_table, q_weight, k_weight)
+    T, B = x.shape[0], block_table.shape[0]
+    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    q_out = torch.empty((T, 1, Hq, D), dtype=x.dtype, device=dev)
+    if T == 0:
+        return q_out, K_pages, V_pages
+    if q_weight is not None:
+        q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+    c, s, bt = _tables(cos, dev), _tables(sin, dev), _i32(block_table, dev)
+    _lib.launch("mk_qk_norm_rope_paged_update", dev, x.data_ptr(), x.stride(0), _lib.ptr(q_weight),
+                _lib.ptr(k_weight), float(eps), c.data_ptr(), s.data_ptr(), pos.data_ptr(), _lib.ptr(seq),
+                bt.data_ptr(), K_pages.data_ptr(), V_pages.data_ptr(), q_out.data_ptr(), T, B, Hq, Hkv, D,
+                D if rotary_dim is None else rotary_dim, K_pages.shape[1], bt.shape[1], K_pages.shape[0], c.shape[0],
+                _layout_code(layout), _lib.DT_F32 if q_weight is None else _lib.dtype_code(q_weight.dtype),
+                _lib.dtype_code(x.dtype))
+    return q_out, K_pages, V_pages
 
 
 def reference_gqa_decode_block_from_qkv(qkv, K_cache, V_cache, cos, sin, position, *, num_attention_heads,
