@@ -312,6 +312,47 @@ int mk_qk_norm_rope_paged_update(const void* qkv, int64_t row_stride, const void
                                  int64_t rotary_dim, int64_t page_size, int64_t max_blocks, int64_t num_pages,
                                  int64_t cos_rows, int layout, int weight_dtype, int dtype, void* stream);
 
+/* Pages of a cache copied, forked and compacted; no counterparts in the
+ * reference (its tables are fixed, ops/paged_kv_ops.py:99-115).  tensors and
+ * page_bytes are host arrays of num_tensors device addresses of page arrays
+ * ([num_pages, ...] dense) and bytes a page; pages of all of them move
+ * together.  page_bytes and addresses that are multiples of 16 take 16-byte
+ * accesses.
+ *
+ * mk_copy_kv_pages: page src[i] onto dst[i] (device int32), i < n; entries
+ * outside [0, num_pages) are skipped.  No page may be the destination of two
+ * pairs, or the source of one and the destination of another. */
+int mk_copy_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors, const int32_t* src,
+                     const int32_t* dst, int64_t n, int64_t num_pages, void* stream);
+
+/* Row r of the new table continues row parents[r] of block_table
+ * [B, max_blocks] (outside [0, B): an empty row) with the pages that its
+ * lengths[parent] positions lie in; ref_counts [num_pages] (references to each
+ * page, others than the table's included; a page of count 0 is free) lose the
+ * old table's references and gain the new one's.  With reserve > 0 every row
+ * gets the pages for so many more positions, and its own copy of a partly
+ * filled last page that somebody else holds too (of rows that share it the
+ * longest, then the first, keeps it if nobody else does): free pages by
+ * ascending id to rows in order.  ready[r] = 0 where the row's pages do not
+ * suffice or the table has no room: such a row gets none of them, shares its
+ * last page and must not be appended to.  Pages that only dropped rows held
+ * are free, and may be given away by the same call.  n <= 4096 rows; workspace int32, at least 2 n +
+ * min(num_pages, n (1 + ceil(reserve / page_size))). */
+int mk_fork_kv_sequences(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors,
+                         const int32_t* block_table, const int32_t* lengths, const int32_t* ref_counts,
+                         const int32_t* parents, int32_t* new_table, int32_t* new_lengths, int32_t* new_ref_counts,
+                         uint8_t* ready, int32_t* workspace, int64_t workspace_ints, int64_t B, int64_t n,
+                         int64_t max_blocks, int64_t page_size, int64_t num_pages, int64_t reserve, void* stream);
+
+/* Live pages (ref_counts > 0) to ids [0, counts[0]): of the live ones past it
+ * the i-th moves onto the i-th free one below.  page_map [num_pages] = where a
+ * page is now, -1 for a free one; new_table [entries] = block_table through
+ * it.  counts [2]: live and moved pages.  workspace: num_pages int32. */
+int mk_compact_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors,
+                        const int32_t* block_table, const int32_t* ref_counts, int32_t* new_table,
+                        int32_t* new_ref_counts, int32_t* page_map, int32_t* counts, int32_t* workspace,
+                        int64_t workspace_ints, int64_t entries, int64_t num_pages, void* stream);
+
 /* quantize_kv_pages -- ops/paged_quantized_kv_ops.py:194-292 for one of K or V:
  * src [rows, D] (rows = num_pages*P*Hkv) -> codes [rows, D] (q8) or
  * [rows, ceil(D/2)] (q4) and fp16 scales [rows, ceil(D/g)], with the

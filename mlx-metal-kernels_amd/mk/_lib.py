@@ -76,6 +76,9 @@ SIGNATURES: dict[str, list] = {
     "mk_qkv_rope_paged_update_quant": [_P] * 10 + [_I64] * 9 + [_I, _I, _P],
     "mk_apply_rope": [_P] * 5 + [_I64] * 9 + [_I, _I64, _I, _I, _P],
     "mk_qk_norm_rope_paged_update": [_P, _I64, _P, _P, _F] + [_P] * 8 + [_I64] * 10 + [_I] * 3 + [_P],
+    "mk_copy_kv_pages": [_P, _P, _I64, _P, _P, _I64, _I64, _P],
+    "mk_fork_kv_sequences": [_P, _P, _I64] + [_P] * 9 + [_I64] * 7 + [_P],
+    "mk_compact_kv_pages": [_P, _P, _I64] + [_P] * 7 + [_I64] * 3 + [_P],
     "mk_quantize_kv": [_P, _P, _P, _I64, _I64, _I64, _I, _I, _P],
     "mk_dequantize_kv": [_P, _P, _P, _I64, _I64, _I64, _I, _P],
     "mk_paged_attention_workspace_bytes": [_I64] * 6,

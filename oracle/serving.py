@@ -99,7 +99,7 @@ def fork(table, lengths, refs, parents, P, reserve, num_pages):
             need = int(copy) + int(-(-(L[b] + reserve) // P) - nb[b])
             got = free[used:used + need]
             used += need
-            if used > len(free):
+            if need and used > len(free):
                 ready[b] = False
                 continue
             for p in got:
