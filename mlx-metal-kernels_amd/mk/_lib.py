@@ -79,6 +79,8 @@ SIGNATURES: dict[str, list] = {
     "mk_copy_kv_pages": [_P, _P, _I64, _P, _P, _I64, _I64, _P],
     "mk_fork_kv_sequences": [_P, _P, _I64] + [_P] * 9 + [_I64] * 7 + [_P],
     "mk_compact_kv_pages": [_P, _P, _I64] + [_P] * 7 + [_I64] * 3 + [_P],
+    "mk_lora_workspace_bytes": [_I64] * 5,
+    "mk_lora_add": [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64] + [_I64] * 5 + [_I, _P, _SZ, _P],
     "mk_quantize_kv": [_P, _P, _P, _I64, _I64, _I64, _I, _I, _P],
     "mk_dequantize_kv": [_P, _P, _P, _I64, _I64, _I64, _I, _P],
     "mk_paged_attention_workspace_bytes": [_I64] * 6,
@@ -88,7 +90,8 @@ SIGNATURES: dict[str, list] = {
     "mk_paged_verify_attention": [_P] * 6 + [_I64] * 8 + [_F, _I, _P, _SZ, _P],
     "mk_paged_quantized_verify_attention": [_P] * 8 + [_I64] * 9 + [_I, _F, _I, _P, _SZ, _P],
 }
-_RESTYPES = {"mk_paged_attention_workspace_bytes": _SZ, "mk_matvec_workspace_bytes": _SZ}
+_RESTYPES = {"mk_paged_attention_workspace_bytes": _SZ, "mk_matvec_workspace_bytes": _SZ,
+             "mk_lora_workspace_bytes": _SZ}
 
 _lock = threading.Lock()
 _lib = None

@@ -1,0 +1,157 @@
+"""Low-rank adapters of many requests beside a shared projection: row m of a
+batch adds s_i B_i (A_i x[m]) for its own adapter i to what the shared weight
+gave.  The reference has no counterpart.
+
+Adapters lie stacked: ``lora_a`` [ADAPTERS, R, K] and ``lora_b`` [ADAPTERS, N,
+R] in the activations' dtype (an adapter of lower rank is filled up with
+zeros), ``scales`` fp32 [ADAPTERS] (None: 1).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._common import ACT_DTYPES, as_dense, ci_safe_mode_enabled, values_only
+from .kv_cache_ops import host_checks_enabled
+from .mlp_block_ops import quantized_linear
+
+MAX_RANK = 128
+
+
+def _validate(x, base, lora_a, lora_b, adapter_ids, scales, out):
+    """(M, N, K, R, adapters, ids [M])"""
+    if x.ndim < 1 or x.ndim != base.ndim or x.shape[:-1] != base.shape[:-1]:
+        raise ValueError(f"x and base must be [...,K] and [...,N] of the same rows, got {tuple(x.shape)}, "
+                         f"{tuple(base.shape)}")
+    if lora_a.ndim != 3 or lora_b.ndim != 3:
+        raise ValueError(f"lora_a and lora_b must be [ADAPTERS,R,K] and [ADAPTERS,N,R], got {tuple(lora_a.shape)}, "
+                         f"{tuple(lora_b.shape)}")
+    K, N = x.shape[-1], base.shape[-1]
+    adapters, R, _ = lora_a.shape
+    if lora_a.shape[2] != K or tuple(lora_b.shape) != (adapters, N, R):
+        raise ValueError(f"lora_a and lora_b must be [ADAPTERS,R,{K}] and [ADAPTERS,{N},R], got {tuple(lora_a.shape)}, "
+                         f"{tuple(lora_b.shape)}")
+    if K < 1 or not 1 <= R <= MAX_RANK:
+        raise ValueError(f"K must be positive and R in [1, {MAX_RANK}], got K={K}, R={R}")
+    if x.dtype not in ACT_DTYPES:
+        raise TypeError(f"x dtype must be float16 or bfloat16, got {x.dtype}")
+    for name, t in (("base", base), ("lora_a", lora_a), ("lora_b", lora_b)):
+        if t.dtype != x.dtype:
+            raise TypeError(f"{name} must carry x's dtype {x.dtype}, got {t.dtype}")
+    if scales is not None and tuple(scales.shape) != (adapters,):
+        raise ValueError(f"scales must have shape {(adapters,)}, got {tuple(scales.shape)}")
+    if out is not None and (out.shape != base.shape or out.dtype != base.dtype or out.device != base.device):
+        raise ValueError(f"out must match base {tuple(base.shape)} {base.dtype} on {base.device}, got "
+                         f"{tuple(out.shape)} {out.dtype} on {out.device}")
+    rows = x.shape[:-1]
+    M = 1
+    for n in rows:
+        M *= n
+    if not isinstance(adapter_ids, torch.Tensor):
+        adapter_ids = torch.as_tensor(adapter_ids, dtype=torch.int32)
+    if adapter_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"adapter_ids must be int32 or int64, got {adapter_ids.dtype}")
+    if adapter_ids.shape == rows or tuple(adapter_ids.shape) == (M,):
+        ids = adapter_ids.reshape(M)
+    elif len(rows) == 2 and tuple(adapter_ids.shape) == (rows[0],):
+        ids = adapter_ids[:, None].expand(rows).reshape(M)
+    else:
+        raise ValueError(f"adapter_ids must have shape {tuple(rows)}, {(M,)} or one a sequence, got "
+                         f"{tuple(adapter_ids.shape)}")
+    if M and host_checks_enabled(ids):
+        lo, hi = int(ids.min()), int(ids.max())
+        if lo < -1 or hi >= adapters:
+            raise ValueError(f"adapter_ids must be in [-1, {adapters}), got {lo} to {hi}")
+    return M, N, K, R, adapters, ids.to(device=x.device, dtype=torch.int32).contiguous()
+
+
+def reference_lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None):
+    """``lora_add`` with tensor ops, an adapter at a time."""
+    M, N, K, R, adapters, ids = _validate(x, base, lora_a, lora_b, adapter_ids, scales, None)
+    x2, out = x.reshape(M, K).float(), base.reshape(M, N).float()
+    for i in range(adapters):
+        d = (x2 @ lora_a[i].float().t()) @ lora_b[i].float().t()
+        if scales is not None:
+            d = d * scales[i].float()
+        out = torch.where((ids == i)[:, None], out + d, out)
+    return out.to(base.dtype).reshape(base.shape)
+
+
+def _rows(t, width):
+    """(t as rows of ``width`` dense values at one stride, that stride); None where it is not."""
+    if t.ndim == 2 and t.stride(1) == 1 and t.stride(0) >= width:
+        return t, t.stride(0)
+    if t.is_contiguous():
+        return t, width
+    return None, 0
+
+
+def _apart(a, b):
+    """Whether the memory that two tensors span does not overlap."""
+    def span(t):
+        n = sum((s - 1) * k for s, k in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (n + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a1 <= b0 or b1 <= a0
+
+
+def lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None, out=None, backend: str = "auto"):
+    """base + s_i B_i (A_i x) for each row's adapter i = adapter_ids[row]: x
+    [...,K], base [...,N] of the same rows (fp16 / bf16), ``adapter_ids`` int32
+    of the rows' shape, flat, or one for each sequence of [B,S,...] rows; -1 is
+    a row without an adapter.  Both products are summed in fp32 and the result
+    is rounded once.  ``out``: a tensor to write, ``base`` itself among them
+    (the rows may be strided; no other overlap).
+
+    ids are checked on the host unless that is off (``host_checks_enabled``);
+    then one outside [0, ADAPTERS) is a row without an adapter.  Backend
+    "reference", and inputs that need more than their values (a gradient, a
+    function transform, tracing), take the tensor ops."""
+    backend_name = backend.lower()
+    if backend_name not in ("auto", "reference", "metal"):
+        raise ValueError("backend must be one of 'reference', 'metal', 'auto'")
+    tensors = (x, base, lora_a, lora_b) if scales is None else (x, base, lora_a, lora_b, scales)
+    if ci_safe_mode_enabled() or backend_name == "reference" or not values_only(*tensors):
+        y = reference_lora_add(x, base, lora_a, lora_b, adapter_ids, scales=scales)
+        return y if out is None else out.copy_(y)
+    M, N, K, R, adapters, ids = _validate(x, base, lora_a, lora_b, adapter_ids, scales, out)
+    dev = _lib.require_device(x, base, lora_a, lora_b, scales)
+    x2, x_stride = _rows(x, K)
+    if x2 is None:
+        x2, x_stride = x.contiguous(), K
+    b2, base_stride = _rows(base, N)
+    if b2 is None:
+        b2, base_stride = base.contiguous(), N
+    target = out
+    if out is None:
+        target, out_stride = torch.empty(base.shape, dtype=base.dtype, device=dev), N
+    else:
+        same = out.data_ptr() == base.data_ptr() and out.stride() == base.stride()
+        if not (same or _apart(out, base)) or not _apart(out, x):
+            raise ValueError("out may be base itself, and share no memory with it or x otherwise")
+        target, out_stride = _rows(out, N)
+        if target is None:
+            target, out_stride = torch.empty(base.shape, dtype=base.dtype, device=dev), N
+    if M and N:
+        a, b = lora_a.contiguous(), lora_b.contiguous()
+        scales = as_dense(scales, torch.float32)
+        size = _lib.load().mk_lora_workspace_bytes(M, N, K, R, adapters)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        _lib.launch("mk_lora_add", dev, x2.data_ptr(), x_stride, b2.data_ptr(), base_stride, a.data_ptr() or None,
+                    b.data_ptr() or None, ids.data_ptr(), _lib.ptr(scales), target.data_ptr(), out_stride, M, N, K, R,
+                    adapters, _lib.dtype_code(x.dtype), ws.data_ptr() or None, size)
+    if out is not None and target is not out:
+        out.copy_(target)
+        return out
+    return target
+
+
+def quantized_lora_linear(x, w, scales, zeros, lora_a, lora_b, adapter_ids, *, lora_scales=None, bits=4, group_size=32,
+                          backend: str = "auto"):
+    """``quantized_linear`` with every row's adapter added to its result, in place:
+    the shared product in the activation dtype, then ``lora_add``."""
+    y = quantized_linear(x, w, scales, zeros, bits=bits, group_size=group_size, backend=backend)
+    reference = backend.lower() == "reference"
+    return lora_add(x, y, lora_a, lora_b, adapter_ids, scales=lora_scales, out=None if reference else y,
+                    backend="reference" if reference else "auto")

@@ -1,0 +1,159 @@
+"""mk_lora_add against the 64-bit oracle: ranks, widths and row counts at tile
+edges, mixed and sorted adapters, strides, values that are not numbers."""
+
+import pytest
+import torch
+
+import mk.lora_ops as lo
+from mk.mlp_block_ops import quantized_linear
+from tests._data import quant_weight, to_dev
+from tests.test_host_lora import check_lora, lora_case
+
+import numpy as np
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float16, torch.bfloat16]
+
+# (M, N, K, R, adapters)
+SHAPES = [(1, 64, 64, 16, 1), (1, 6144, 4096, 16, 4), (2, 1, 1, 1, 1), (3, 100, 72, 8, 2), (16, 64, 32, 16, 3),
+          (17, 65, 33, 17, 2), (5, 40, 30, 4, 3), (33, 130, 264, 32, 9), (20, 48, 520, 33, 20), (64, 256, 96, 64, 4),
+          (7, 200, 1000, 128, 2), (65, 72, 2056, 48, 1), (130, 1024, 136, 100, 5), (300, 96, 512, 16, 2),
+          (31, 8, 4100, 2, 3), (48, 4096, 8, 127, 2), (70, 328, 1504, 64, 7)]
+
+
+def on(dev, *tensors):
+    return [None if t is None else t.to(dev) for t in tensors]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_lora_add(dev, shape, dtype):
+    case = lora_case(sum(shape), *shape, dtype)
+    x, base, a, b, ids, s = on(dev, *case)
+    before = base.clone()
+    check_lora(lo.lora_add(x, base, a, b, ids, scales=s), *case)
+    assert torch.equal(base, before)
+    check_lora(lo.lora_add(x, base, a, b, ids), *case[:5], None)
+    order = torch.argsort(case[4], stable=True)  # prompts one after another
+    sorted_case = (case[0], case[1], *case[2:4], case[4][order], case[5])
+    check_lora(lo.lora_add(x, base, a, b, sorted_case[4].to(dev), scales=s), *sorted_case)
+    assert lo.lora_add(x, base, a, b, ids, scales=s, out=base) is base  # in place
+    check_lora(base, *case)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_and_alignment(dev, dtype):
+    """Rows of wider tensors, bases off a 16-byte boundary, 3-D rows, an adapter of every sequence."""
+    M, N, K, R, NA = 24, 80, 136, 16, 3
+    case = lora_case(7, M, N, K, R, NA, dtype)
+    x, base, a, b, ids, s = on(dev, *case)
+
+    def rows(t, pad, off):
+        wide = torch.zeros(t.shape[0], t.shape[1] + pad, dtype=dtype, device=dev)
+        view = wide[:, off:off + t.shape[1]]
+        view.copy_(t)
+        return view
+
+    for pad, off in ((8, 8), (8, 0), (3, 1), (16, 2)):
+        out = rows(torch.zeros_like(base), pad, off)
+        check_lora(lo.lora_add(rows(x, pad, off), rows(base, pad, off), a, b, ids, scales=s, out=out), *case)
+        same = rows(base, pad, off)
+        check_lora(lo.lora_add(rows(x, 0, 0), same, a, b, ids, scales=s, out=same), *case)
+    for t in (1, 3):  # adapters off a boundary
+        flat_a, flat_b = (torch.empty(v.numel() + t, dtype=dtype, device=dev)[t:].view(v.shape) for v in (a, b))
+        flat_a.copy_(a), flat_b.copy_(b)
+        check_lora(lo.lora_add(x, base, flat_a, flat_b, ids, scales=s), *case)
+    check_lora(lo.lora_add(x, base, a.transpose(1, 2).contiguous().transpose(1, 2), b, ids, scales=s), *case)
+    x3, base3 = x.reshape(6, 4, K), base.reshape(6, 4, N)
+    per = torch.tensor([2, 0, -1, 1, 1, 0], dtype=torch.int32)
+    got = lo.lora_add(x3, base3, a, b, per, scales=s)
+    check_lora(got.reshape(M, N), *case[:4], per.repeat_interleave(4), case[5])
+    turned = x3.transpose(0, 1).contiguous().transpose(0, 1)  # rows not at one stride
+    assert torch.equal(lo.lora_add(turned, base3.transpose(0, 1).contiguous().transpose(0, 1), a, b, per, scales=s), got)
+    out = torch.zeros_like(base3).transpose(0, 1).contiguous().transpose(0, 1)
+    assert lo.lora_add(x3, base3, a, b, per, scales=s, out=out) is out and torch.equal(out, got)
+    assert lo.lora_add(x[:0], base[:0], a, b, ids[:0]).shape == (0, N)
+    assert torch.equal(lo.lora_add(x, base, a[:0], b[:0], ids * 0 - 1), base)
+
+
+def test_overlaps_refused(dev):
+    x, base, a, b, ids, s = on(dev, *lora_case(8, 4, 16, 16, 4, 2, torch.float16))
+    both = torch.zeros(4, 40, dtype=torch.float16, device=dev)
+    for out, kw in ((x, {}), (both[:, 1:17], {"base": both[:, 0:16]}), (both[:, :16], {"x": both[:, 8:24]})):
+        with pytest.raises(ValueError, match="share no memory"):
+            lo.lora_add(**{**dict(x=x, base=base, lora_a=a, lora_b=b, adapter_ids=ids, out=out), **kw})
+    with pytest.raises(ValueError):
+        lo.lora_add(x, base, a, b, ids, out=base[:3])
+    with pytest.raises(ValueError):
+        lo.lora_add(x, base, a, b, ids.clone().fill_(2))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [20, 100])
+def test_values_stay_in_their_rows(dev, dtype, M, monkeypatch):
+    """A row or an adapter of infinities and NaNs changes no row that has neither; ids outside of the adapters add
+    nothing where the host does not look; large values of fp16 stay finite in between."""
+    monkeypatch.setenv("MK_SKIP_DEVICE_RANGE_CHECKS", "1")
+    x, base, a, b, ids, s = lora_case(9, M, 72, 160, 16, 5, dtype)
+    ids[3], ids[9], ids[10] = 5, 2 ** 31 - 1, -2 ** 31
+    clean = lo.lora_add(*on(dev, x, base, a, b, ids), scales=s.to(dev))
+    check_lora(clean, x, base, a, b, ids, s)
+    ids[5], ids[6] = 0, 1
+    clean = lo.lora_add(*on(dev, x, base, a, b, ids), scales=s.to(dev)).cpu()
+    x[5, 7], x[6, 3] = float("nan"), float("inf")
+    a[4, 1, 2], b[3, 5, 1] = float("inf"), float("nan")
+    got = lo.lora_add(*on(dev, x, base, a, b, ids), scales=s.to(dev)).cpu()
+    rows = torch.ones(M, dtype=torch.bool)
+    rows[5] = rows[6] = False
+    rows[(ids == 4) | (ids == 3)] = False
+    assert torch.equal(got[rows], clean[rows])
+    assert got[5].isnan().all() and not got[6].isfinite().any()
+    assert got[ids == 3][:, 5].isnan().all() and torch.equal(got[ids == 3][:, :5], clean[ids == 3][:, :5])
+    # A x past fp16 (2^18), small B: the result is finite and right
+    x, base, a, b, ids, s = lora_case(10, M, 40, 64, 8, 2, dtype, none=0.0)
+    x, a, b = torch.full_like(x, 64.0), torch.full_like(a, 64.0), b * 2.0 ** -14
+    a[:, 1::2] *= 2.0 ** -24  # and ranks that are small beside them
+    check_lora(lo.lora_add(*on(dev, x, base, a, b, ids), scales=s.to(dev)), x, base, a, b, ids, s)
+
+
+def test_quantized_lora_linear(dev):
+    """The shared projection and its adapters: what the two calls give."""
+    rng = np.random.default_rng(0)
+    K, N, g = 256, 192, 64
+    for bits in (4, 8):
+        _, w, sc, z = quant_weight(rng, N, K, g, bits)
+        w, sc, z = to_dev(w, dev), to_dev(sc, dev, torch.float16), to_dev(z, dev, torch.float16)
+        x, _, a, b, ids, s = on(dev, *lora_case(bits, 9, N, K, 16, 3, torch.float16))
+        x = x[:, None]
+        y = quantized_linear(x, w, sc, z, bits=bits, group_size=g)
+        got = lo.quantized_lora_linear(x, w, sc, z, a, b, ids, lora_scales=s, bits=bits, group_size=g)
+        assert got.shape == (9, 1, N) and torch.equal(got, lo.lora_add(x, y, a, b, ids, scales=s))
+        check_lora(got[:, 0], x[:, 0], y[:, 0], a, b, ids, s)
+
+
+def test_stream_and_graph(dev):
+    """On a side stream, and two captured calls on one: every replay against the eager calls, with eager work between."""
+    cases = [lora_case(20 + i, 12, 96, 256, 16, 3, torch.bfloat16) for i in range(2)]
+    given = [on(dev, *c) for c in cases]
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        warm = lo.lora_add(*given[0][:5], scales=given[0][5])
+    side.synchronize()
+    check_lora(warm, *cases[0])
+    graphs, outs = [], []
+    for c in given:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            outs.append(lo.lora_add(*c[:5], scales=c[5]))
+    for i in range(4):
+        for c in given:
+            c[0].copy_(torch.randn(c[0].shape, device=dev))
+            c[4].copy_(torch.randint(-1, 3, c[4].shape, device=dev))
+        eager = [lo.lora_add(*c[:5], scales=c[5]) for c in given]
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, outs)), i

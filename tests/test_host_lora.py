@@ -1,0 +1,102 @@
+"""Low-rank adapters on the host: the tensor-op path against the 64-bit oracle
+and against differences, and what is refused."""
+
+import numpy as np
+import pytest
+import torch
+
+import mk.lora_ops as lo
+from oracle import serving as sv
+
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}  # half a step of each type
+# A x is kept as the sum of two values of the type where it goes through the matrix cores
+TWO = {torch.float16: 2.0 ** -21, torch.bfloat16: 2.0 ** -16}
+
+
+def lora_case(seed, M, N, K, R, NA, dtype, none=0.2, scales=True):
+    g = torch.Generator().manual_seed(seed)
+    x, base = torch.randn(M, K, generator=g).to(dtype), torch.randn(M, N, generator=g).to(dtype)
+    a = (torch.randn(NA, R, K, generator=g) / K ** 0.5).to(dtype)
+    b = (torch.randn(NA, N, R, generator=g) / R ** 0.5).to(dtype)
+    ids = torch.randint(0, NA, (M,), generator=g, dtype=torch.int32)
+    ids[torch.rand(M, generator=g) < none] = -1
+    return x, base, a, b, ids, 0.5 + torch.rand(NA, generator=g) if scales else None
+
+
+def check_lora(got, x, base, a, b, ids, scales):
+    """One rounding of the result, and K + R + 4 fp32 roundings and those of A x of what it is a sum of; over all
+    values their root mean square is that of one rounding, with a sixteenth for the sums."""
+    f = lambda t: None if t is None else t.double().cpu().numpy()  # noqa: E731
+    want, size = sv.lora(f(x), f(base), f(a), f(b), ids.tolist(), f(scales))
+    dtype, K, R = x.dtype, x.shape[-1], a.shape[1]
+    err = np.abs(got.double().cpu().numpy() - want)
+    lim = U[dtype] * np.abs(want) + size * ((K + R + 4) * 2.0 ** -24 + TWO[dtype]) * 1.01 + 2.0 ** -25
+    assert (err <= lim).all(), (int((err > lim).sum()), float(err.max()))
+    if err.size:
+        assert np.sqrt((err ** 2).mean()) <= U[dtype] * np.sqrt((want ** 2).mean()) * 1.0625 + 2.0 ** -25
+    none = ~((ids >= 0) & (ids < len(a))).cpu()
+    assert torch.equal(got.cpu()[none], base.cpu()[none])
+
+
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("shape", [(5, 12, 20, 4, 3), (1, 1, 1, 1, 1), (9, 33, 17, 8, 2)])
+def test_reference_lora(shape, dtype):
+    case = lora_case(sum(shape), *shape, dtype)
+    check_lora(lo.lora_add(*case[:5], scales=case[5], backend="reference"), *case)
+    check_lora(lo.lora_add(*case[:5], backend="reference"), *case[:5], None)
+
+
+def test_ids_of_sequences_and_rows():
+    x, base, a, b, ids, s = lora_case(3, 6, 8, 16, 4, 3, torch.float16)
+    x3, base3 = x.reshape(2, 3, 16), base.reshape(2, 3, 8)
+    flat = lo.lora_add(x, base, a, b, ids, scales=s, backend="reference")
+    for form in (ids, ids.reshape(2, 3), ids.long(), ids.tolist()):
+        assert torch.equal(lo.lora_add(x3, base3, a, b, form, scales=s, backend="reference").reshape(6, 8), flat)
+    per = lo.lora_add(x3, base3, a, b, [2, -1], scales=s, backend="reference")
+    assert torch.equal(per.reshape(6, 8), lo.lora_add(x, base, a, b, [2] * 3 + [-1] * 3, scales=s, backend="reference"))
+    out = torch.empty_like(base)
+    assert lo.lora_add(x, base, a, b, ids, scales=s, out=out, backend="reference") is out and torch.equal(out, flat)
+    assert torch.equal(lo.lora_add(x, base, a[:0], b[:0], [-1] * 6, backend="reference"), base)
+    assert lo.lora_add(x[:0], base[:0], a, b, [], backend="reference").shape == (0, 8)
+
+
+def test_gradients_against_formula_and_differences():
+    """What needs a gradient takes the tensor ops, on any backend; the gradients against their formulas and against
+    differences of the result (which is linear in x, so that they are exact but for its roundings)."""
+    x, base, a, b, ids, s = lora_case(4, 5, 6, 7, 3, 2, torch.float16)
+    leaves = [t.clone().requires_grad_() for t in (x, base, a, b)]
+    g = torch.randn(5, 6).half()
+    lo.lora_add(*leaves, ids, scales=s).backward(g)
+    for i in range(2):
+        rows = ids == i
+        gi, xi = g[rows].double(), x[rows].double()
+        da = s[i].double() * (b[i].double().t() @ gi.t()) @ xi
+        db = s[i].double() * gi.t() @ (xi @ a[i].double().t())
+        for got, want in ((leaves[2].grad[i], da), (leaves[3].grad[i], db)):
+            assert (got.double() - want).abs().max() <= 4 * 2.0 ** -11 * (want.abs().max() + 1)
+    assert torch.equal(leaves[1].grad, g) and (leaves[0].grad[ids < 0] == 0).all()
+    step = torch.randn(5, 7).half()
+    y0, y1 = (lo.lora_add(x + k * step, base, a, b, ids, scales=s, backend="reference").double() for k in (0, 1))
+    moved = ((x + step).double() - x.double())  # what the sum's own rounding leaves of the step
+    slope = (leaves[0].grad.double() * moved).sum()
+    size = (leaves[0].grad.double().abs() * moved.abs()).sum() + (g.double().abs() * (y0.abs() + y1.abs())).sum()
+    assert abs(((y1 - y0) * g.double()).sum() - slope) <= 4 * 2.0 ** -11 * size
+
+
+def test_refusals():
+    x, base, a, b, ids, s = lora_case(5, 4, 6, 8, 2, 3, torch.float16)
+    ok = dict(x=x, base=base, lora_a=a, lora_b=b, adapter_ids=ids, scales=s, backend="reference")
+    lo.lora_add(**ok)
+    for kw in (dict(x=x[:, :7]), dict(base=base[:3]), dict(base=base[None]), dict(lora_a=a[0]), dict(lora_b=b[:2]),
+               dict(lora_b=b[:, :5]), dict(lora_a=a[:, :1]), dict(adapter_ids=ids[:3]), dict(adapter_ids=[0, 1, 2, 3]),
+               dict(adapter_ids=[0, 1, 2, -2]), dict(scales=s[:2]), dict(backend="triton"),
+               dict(lora_a=a[:, :0], lora_b=b[:, :, :0]), dict(x=x[:, :0], lora_a=a[:, :, :0]),
+               dict(lora_a=torch.zeros(1, 129, 8).half(), lora_b=torch.zeros(1, 6, 129).half())):
+        with pytest.raises(ValueError):
+            lo.lora_add(**{**ok, **kw})
+    for kw in (dict(x=x.float(), base=base.float(), lora_a=a.float(), lora_b=b.float()), dict(base=base.bfloat16()),
+               dict(lora_a=a.bfloat16()), dict(adapter_ids=ids.float())):
+        with pytest.raises(TypeError):
+            lo.lora_add(**{**ok, **kw})
+    with pytest.raises(ValueError, match="ROCm device"):
+        lo.lora_add(**{**ok, "backend": "auto"})
