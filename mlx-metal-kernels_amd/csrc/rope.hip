@@ -177,6 +177,24 @@ __device__ __forceinline__ float norm_weight(const void* w, int wdt, int i) {
   return reinterpret_cast<const float*>(w)[i];
 }
 
+// norm weights of a unit's two chunks, 16-byte loads
+__device__ __forceinline__ void norm_weights16(const void* w, int wdt, int c0, int c1, float (&v)[16]) {
+  if (wdt == MK_DT_F32) {
+    const float* p = reinterpret_cast<const float*>(w);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x4 a = ldg128(p + 8 * (h ? c1 : c0)), b = ldg128(p + 8 * (h ? c1 : c0) + 4);
+      __builtin_memcpy(v + 8 * h, &a, 16);
+      __builtin_memcpy(v + 8 * h + 4, &b, 16);
+    }
+    return;
+  }
+  const u32x4 a = ldg128(reinterpret_cast<const uint16_t*>(w) + 8 * c0);
+  const u32x4 b = ldg128(reinterpret_cast<const uint16_t*>(w) + 8 * c1);
+  if (wdt == MK_DT_F16) unpack16<f16>(a, b, v);
+  else unpack16<bf16>(a, b, v);
+}
+
 // cache row (page * page_size + offset) of token t, -1 where it has none
 __device__ __forceinline__ int64_t token_slot(const int32_t* pos, const int32_t* seq, const int32_t* bt,
                                               const QkDims& d, int t) {
@@ -240,9 +258,10 @@ __global__ __launch_bounds__(128) void qk_norm_rope_vec_kernel(
       for (int o = 0; o < lgl; ++o) ss += __shfl_xor(ss, 1 << o, MK_WAVE);
       const float inv = rsqrtf(ss / (float)d.D + d.eps);
       if (has) {
+        float wv[16];
+        norm_weights16(w, d.wdt, c0, c1, wv);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          v[e] = v[e] * inv * norm_weight(w, d.wdt, 8 * (e < 8 ? c0 : c1) + (e & 7));
+        for (int e = 0; e < 16; ++e) v[e] = v[e] * inv * wv[e];
       }
     }
     if (has && u < ru) {
@@ -382,7 +401,8 @@ int mk_qk_norm_rope_paged_update(const void* qkv, int64_t row_stride, const void
   // a head's units on at most one wave's lanes
   const bool vec = D % 16 == 0 && D <= 16 * MK_WAVE && rotary_dim % 16 == 0 && row_stride % 8 == 0 &&
                    mk_aligned(qkv, 16) && mk_aligned(q_out, 16) && mk_aligned(K_pages, 16) &&
-                   mk_aligned(V_pages, 16) && mk_aligned(cos_t, 16) && mk_aligned(sin_t, 16);
+                   mk_aligned(V_pages, 16) && mk_aligned(cos_t, 16) && mk_aligned(sin_t, 16) &&
+                   mk_aligned(q_weight, 16) && mk_aligned(k_weight, 16);
   int lgl = 0;
   while (vec && (16 << lgl) < D) ++lgl;
   const int64_t gy = vec ? ((heads << lgl) + 127) / 128 : (heads + 3) / 4;

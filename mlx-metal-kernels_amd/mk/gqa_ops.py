@@ -283,42 +283,43 @@ def _qk_norm_rope_prep(qkv, K_pages, V_pages, block_table, cos, sin, position, H
     if D % 2 != 0:
         raise ValueError(f"RoPE requires even D, got D={D}")
     N = (Hq + 2 * Hkv) * D
-    if qkv.ndim == 4 and tuple(qkv.shape[1:]) == (1, Hq + 2 * Hkv, D):
-        x = qkv.reshape(qkv.shape[0], N)
-    elif qkv.ndim == 3 and tuple(qkv.shape[1:]) == (1, N):
-        x = qkv[:, 0]
-    elif qkv.ndim == 2 and qkv.shape[1] == N:
+    shape, pages, table, rope = qkv.shape, K_pages.shape, block_table.shape, cos.shape
+    T = shape[0] if len(shape) else 0
+    if shape == (T, N):
         x = qkv
+    elif shape == (T, 1, N) or shape == (T, 1, Hq + 2 * Hkv, D):
+        x = qkv.reshape(T, N)
     else:
         raise ValueError(f"qkv must have shape [T,{N}], [T,1,{N}] or [T,1,{Hq + 2 * Hkv},{D}], got {tuple(qkv.shape)}")
-    if K_pages.shape != V_pages.shape or K_pages.ndim != 4 or K_pages.shape[2] != Hkv or K_pages.shape[3] != D:
+    if len(pages) != 4 or pages != V_pages.shape or pages[2] != Hkv or pages[3] != D:
         raise ValueError(f"K_pages/V_pages must be [NUM_PAGES,PAGE_SIZE,{Hkv},{D}], got {tuple(K_pages.shape)}, "
                          f"{tuple(V_pages.shape)}")
-    if K_pages.dtype not in ACT_DTYPES or V_pages.dtype != K_pages.dtype:
+    dtype = K_pages.dtype
+    if dtype not in ACT_DTYPES or V_pages.dtype != dtype:
         raise TypeError(f"K_pages/V_pages must share a float16/bfloat16 dtype, got {K_pages.dtype}, {V_pages.dtype}")
-    if qkv.dtype != K_pages.dtype:
+    if qkv.dtype != dtype:
         raise TypeError(f"qkv must carry the pages' dtype {K_pages.dtype}, got {qkv.dtype}")
-    if block_table.ndim != 2:
+    if len(table) != 2:
         raise ValueError(f"block_table must be 2-D [B,MAX_BLOCKS], got {tuple(block_table.shape)}")
-    if cos.ndim != 2 or cos.shape != sin.shape or cos.shape[1] != rd // 2:
+    if len(rope) != 2 or rope != sin.shape or rope[1] != rd // 2:
         raise ValueError(f"cos and sin must be [rows,{rd // 2}], got {tuple(cos.shape)}, {tuple(sin.shape)}")
     if (q_weight is None) != (k_weight is None):
         raise ValueError("give q_weight and k_weight, or neither")
     if q_weight is not None:
-        if tuple(q_weight.shape) != (D,) or tuple(k_weight.shape) != (D,):
+        if q_weight.shape != (D,) or k_weight.shape != (D,):
             raise ValueError(f"q_weight and k_weight must have shape {(D,)}, got {tuple(q_weight.shape)}, "
                              f"{tuple(k_weight.shape)}")
         if q_weight.dtype not in _NORM_DTYPES or q_weight.dtype != k_weight.dtype:
             raise TypeError("q_weight and k_weight must share a float16, bfloat16, or float32 dtype, got "
                             f"{q_weight.dtype}, {k_weight.dtype}")
-    T, B = x.shape[0], block_table.shape[0]
+    B = table[0]
     dev = block_table.device
-    rows = min(cos.shape[0], block_table.shape[1] * K_pages.shape[1])
+    rows = min(rope[0], table[1] * pages[1])
     if isinstance(position, int):
         position = torch.full((T,), position, dtype=torch.int32, device=dev)
     elif not isinstance(position, torch.Tensor):
         position = torch.as_tensor(position, dtype=torch.int32)
-    if position.dtype not in (torch.int32, torch.int64) or tuple(position.shape) != (T,):
+    if position.dtype not in (torch.int32, torch.int64) or position.shape != (T,):
         raise ValueError(f"position must be an int or int32 [T]={(T,)}, got {position.dtype} {tuple(position.shape)}")
     if sequences is None:
         if T != B:
@@ -326,7 +327,7 @@ def _qk_norm_rope_prep(qkv, K_pages, V_pages, block_table, cos, sin, position, H
     else:
         if not isinstance(sequences, torch.Tensor):
             sequences = torch.as_tensor(sequences, dtype=torch.int32)
-        if sequences.dtype not in (torch.int32, torch.int64) or tuple(sequences.shape) != (T,):
+        if sequences.dtype not in (torch.int32, torch.int64) or sequences.shape != (T,):
             raise ValueError(f"sequences must be int32 [T]={(T,)}, got {sequences.dtype} {tuple(sequences.shape)}")
     if T and host_checks_enabled(position):
         lo, hi = int(position.min()), int(position.max())
@@ -409,7 +410,7 @@ def paged_qk_norm_rope_update(qkv, K_pages, V_pages, block_table, cos, sin, posi
     backend_name = backend.lower()
     if backend_name not in ("auto", "reference", "metal"):
         raise ValueError("backend must be one of 'reference', 'metal', 'auto'")
-    if ci_safe_mode_enabled() or backend_name == "reference":
+    if backend_name == "reference" or ci_safe_mode_enabled():
         return reference_paged_qk_norm_rope_update(
             qkv, K_pages, V_pages, block_table, cos, sin, position, num_attention_heads=num_attention_heads,
             num_key_value_heads=num_key_value_heads, head_dim=head_dim, q_weight=q_weight, k_weight=k_weight,
@@ -423,21 +424,24 @@ def paged_qk_norm_rope_update(qkv, K_pages, V_pages, block_table, cos, sin, posi
                                                                                   or k_weight.requires_grad))):
         raise RuntimeError("paged_qk_norm_rope_update records no gradient; call it under torch.no_grad()")
     dev = _lib.require_device(x, K_pages, V_pages, block_table, q_weight, k_weight)
-    T, B = x.shape[0], block_table.shape[0]
-    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
+    T, N = x.shape
+    B, blocks = block_table.shape
+    row, dense = x.stride()
+    if dense != 1 or row < N:
         x = x.contiguous()
+        row = N
     q_out = torch.empty((T, 1, Hq, D), dtype=x.dtype, device=dev)
     if T == 0:
         return q_out, K_pages, V_pages
     if q_weight is not None:
         q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
     c, s, bt = _tables(cos, dev), _tables(sin, dev), _i32(block_table, dev)
-    _lib.launch("mk_qk_norm_rope_paged_update", dev, x.data_ptr(), x.stride(0), _lib.ptr(q_weight),
-                _lib.ptr(k_weight), float(eps), c.data_ptr(), s.data_ptr(), pos.data_ptr(), _lib.ptr(seq),
-                bt.data_ptr(), K_pages.data_ptr(), V_pages.data_ptr(), q_out.data_ptr(), T, B, Hq, Hkv, D,
-                D if rotary_dim is None else rotary_dim, K_pages.shape[1], bt.shape[1], K_pages.shape[0], c.shape[0],
-                _layout_code(layout), _lib.DT_F32 if q_weight is None else _lib.dtype_code(q_weight.dtype),
-                _lib.dtype_code(x.dtype))
+    num_pages, P, _, _ = K_pages.shape
+    _lib.launch("mk_qk_norm_rope_paged_update", dev, x.data_ptr(), row, _lib.ptr(q_weight), _lib.ptr(k_weight),
+                float(eps), c.data_ptr(), s.data_ptr(), pos.data_ptr(), _lib.ptr(seq), bt.data_ptr(),
+                K_pages.data_ptr(), V_pages.data_ptr(), q_out.data_ptr(), T, B, Hq, Hkv, D, rotary_dim or D, P, blocks,
+                num_pages, c.shape[0], _layout_code(layout),
+                _lib.DT_F32 if q_weight is None else _lib.dtype_code(q_weight.dtype), _lib.dtype_code(x.dtype))
     return q_out, K_pages, V_pages
 
 

@@ -17,7 +17,8 @@ equal inputs give equal tables.
 
 from __future__ import annotations
 
-import ctypes
+from array import array
+from operator import attrgetter
 
 import torch
 
@@ -27,6 +28,7 @@ from .kv_cache_ops import host_checks_enabled
 from .paged_kv_ops import _i32
 
 MAX_ROWS = 4096  # rows of a forked table
+_SHAPE, _NBYTES = attrgetter("shape"), attrgetter("nbytes")
 
 
 def _backend(backend: str) -> bool:
@@ -40,29 +42,28 @@ def _backend(backend: str) -> bool:
 def _check_pages(pages, num_pages, device):
     """Dense arrays of ``num_pages`` pages (None: those of the first), of one page size, on one device."""
     size = None
-    for t in pages:
-        if t.dim() < 2:
-            raise ValueError(f"page arrays must be [NUM_PAGES,PAGE_SIZE,...], got {tuple(t.shape)}")
-        n, p = t.shape[0], t.shape[1]
+    # the shapes that there are, once each: a cache of many layers has one or two
+    for shape in set(map(_SHAPE, pages)):
+        if len(shape) < 2:
+            raise ValueError(f"page arrays must be [NUM_PAGES,PAGE_SIZE,...], got {tuple(shape)}")
         if num_pages is None:
-            num_pages = n
+            num_pages = shape[0]
         if size is None:
-            size = p
-        if n != num_pages or p != size:
-            raise ValueError(f"page arrays must share NUM_PAGES={num_pages} and PAGE_SIZE={size}, got {tuple(t.shape)}")
-        if not t.is_contiguous():
-            raise ValueError("page arrays must be contiguous for the in-place move")
-        if t.device != device:
-            raise ValueError(f"tensors are on different devices: {device} and {t.device}")
+            size = shape[1]
+        if shape[0] != num_pages or shape[1] != size:
+            raise ValueError(f"page arrays must share NUM_PAGES={num_pages} and PAGE_SIZE={size}, got {tuple(shape)}")
+    if not all(map(torch.Tensor.is_contiguous, pages)):
+        raise ValueError("page arrays must be contiguous for the in-place move")
+    for d in set(map(torch.Tensor.get_device, pages)):  # -1: the host
+        if d != (-1 if device.type == "cpu" else device.index):
+            raise ValueError(f"tensors are on different devices: {device} and others")
     return num_pages, size
 
 
-def _addresses(pages):
-    """(addresses, bytes a page, their number) as the library takes them."""
-    k = len(pages)
-    at = (ctypes.c_void_p * k)(*[t.data_ptr() for t in pages])
-    size = (ctypes.c_int64 * k)(*[t.nbytes // t.shape[0] if t.shape[0] else 0 for t in pages])
-    return at, size, k
+def _addresses(pages, num_pages):
+    """Host arrays of the addresses and of the bytes a page, as the library takes them."""
+    return (array("Q", map(torch.Tensor.data_ptr, pages)),
+            array("q", [n // num_pages for n in map(_NBYTES, pages)]))
 
 
 def _ids(t, device, name):
@@ -116,10 +117,10 @@ def copy_kv_pages(pages, src, dst, *, backend: str = "auto"):
                     t[b] = t[a]
         return pages
     _lib.require_device(pages[0])
-    if n:
+    if n and num_pages:
         src, dst = src.contiguous(), dst.contiguous()
-        at, size, k = _addresses(pages)
-        _lib.launch("mk_copy_kv_pages", dev, at, size, k, src.data_ptr(), dst.data_ptr(), n, num_pages)
+        at, size = _addresses(pages, num_pages)
+        _lib.launch("mk_copy_kv_pages", dev, at.buffer_info()[0], size.buffer_info()[0], len(pages), src.data_ptr(), dst.data_ptr(), n, num_pages)
     return pages
 
 
@@ -210,9 +211,9 @@ def fork_kv_sequences(pages, block_table, lengths, ref_counts, parents, *, reser
     ready = torch.empty(n, dtype=torch.bool, device=dev)
     ints = 2 * n + min(num_pages, n * (1 + -(-reserve // size))) if reserve else 0
     buf = torch.empty(n + ints, dtype=torch.int32, device=dev)  # the new lengths, then the workspace
-    at, sizes, k = _addresses(pages)
+    at, sizes = _addresses(pages, num_pages)
     base = buf.data_ptr()
-    _lib.launch("mk_fork_kv_sequences", dev, at, sizes, k, table.data_ptr() or None, lengths.data_ptr() or None,
+    _lib.launch("mk_fork_kv_sequences", dev, at.buffer_info()[0], sizes.buffer_info()[0], len(pages), table.data_ptr() or None, lengths.data_ptr() or None,
                 refs.data_ptr(), parents.data_ptr() or None, new_table.data_ptr() or None, base or None,
                 new_refs.data_ptr(), ready.data_ptr() or None, base + 4 * n if ints else None, ints, B, n, blocks,
                 size, num_pages, reserve)
@@ -302,9 +303,9 @@ def compact_kv_pages(pages, block_table, ref_counts, *, backend: str = "auto"):
     new_table = torch.empty_like(table)
     new_refs, page_map = torch.empty_like(refs), torch.empty_like(refs)
     buf = torch.empty(2 + num_pages, dtype=torch.int32, device=dev)  # live and moved pages, then the workspace
-    at, sizes, k = _addresses(pages)
+    at, sizes = _addresses(pages, num_pages)
     base = buf.data_ptr()
-    _lib.launch("mk_compact_kv_pages", dev, at, sizes, k, table.data_ptr() or None, refs.data_ptr(),
+    _lib.launch("mk_compact_kv_pages", dev, at.buffer_info()[0], sizes.buffer_info()[0], len(pages), table.data_ptr() or None, refs.data_ptr(),
                 new_table.data_ptr() or None, new_refs.data_ptr(), page_map.data_ptr(), base, base + 8, num_pages,
                 table.numel(), num_pages)
     return new_table, new_refs, page_map, buf[:1]

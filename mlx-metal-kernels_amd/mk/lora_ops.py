@@ -9,6 +9,8 @@ zeros), ``scales`` fp32 [ADAPTERS] (None: 1).
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -21,41 +23,45 @@ MAX_RANK = 128
 
 def _validate(x, base, lora_a, lora_b, adapter_ids, scales, out):
     """(M, N, K, R, adapters, ids [M])"""
-    if x.ndim < 1 or x.ndim != base.ndim or x.shape[:-1] != base.shape[:-1]:
+    *rows, K = x.shape or (0,)
+    *same, N = base.shape or (0,)
+    if rows != same or not x.shape or not base.shape:
         raise ValueError(f"x and base must be [...,K] and [...,N] of the same rows, got {tuple(x.shape)}, "
                          f"{tuple(base.shape)}")
-    if lora_a.ndim != 3 or lora_b.ndim != 3:
+    a_shape = lora_a.shape
+    if len(a_shape) != 3 or lora_b.ndim != 3:
         raise ValueError(f"lora_a and lora_b must be [ADAPTERS,R,K] and [ADAPTERS,N,R], got {tuple(lora_a.shape)}, "
                          f"{tuple(lora_b.shape)}")
-    K, N = x.shape[-1], base.shape[-1]
-    adapters, R, _ = lora_a.shape
-    if lora_a.shape[2] != K or tuple(lora_b.shape) != (adapters, N, R):
+    adapters, R, _ = a_shape
+    if a_shape[2] != K or lora_b.shape != (adapters, N, R):
         raise ValueError(f"lora_a and lora_b must be [ADAPTERS,R,{K}] and [ADAPTERS,{N},R], got {tuple(lora_a.shape)}, "
                          f"{tuple(lora_b.shape)}")
     if K < 1 or not 1 <= R <= MAX_RANK:
         raise ValueError(f"K must be positive and R in [1, {MAX_RANK}], got K={K}, R={R}")
-    if x.dtype not in ACT_DTYPES:
+    dtype = x.dtype
+    if dtype not in ACT_DTYPES:
         raise TypeError(f"x dtype must be float16 or bfloat16, got {x.dtype}")
-    for name, t in (("base", base), ("lora_a", lora_a), ("lora_b", lora_b)):
-        if t.dtype != x.dtype:
-            raise TypeError(f"{name} must carry x's dtype {x.dtype}, got {t.dtype}")
-    if scales is not None and tuple(scales.shape) != (adapters,):
+    if base.dtype != dtype or lora_a.dtype != dtype or lora_b.dtype != dtype:
+        raise TypeError(f"base, lora_a and lora_b must carry x's dtype {dtype}, got {base.dtype}, {lora_a.dtype}, "
+                        f"{lora_b.dtype}")
+    if scales is not None and scales.shape != (adapters,):
         raise ValueError(f"scales must have shape {(adapters,)}, got {tuple(scales.shape)}")
     if out is not None and (out.shape != base.shape or out.dtype != base.dtype or out.device != base.device):
         raise ValueError(f"out must match base {tuple(base.shape)} {base.dtype} on {base.device}, got "
                          f"{tuple(out.shape)} {out.dtype} on {out.device}")
-    rows = x.shape[:-1]
-    M = 1
-    for n in rows:
-        M *= n
+    M = math.prod(rows)
     if not isinstance(adapter_ids, torch.Tensor):
         adapter_ids = torch.as_tensor(adapter_ids, dtype=torch.int32)
     if adapter_ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"adapter_ids must be int32 or int64, got {adapter_ids.dtype}")
-    if adapter_ids.shape == rows or tuple(adapter_ids.shape) == (M,):
-        ids = adapter_ids.reshape(M)
-    elif len(rows) == 2 and tuple(adapter_ids.shape) == (rows[0],):
-        ids = adapter_ids[:, None].expand(rows).reshape(M)
+    shape = adapter_ids.shape
+    ids = adapter_ids
+    if shape == (M,):
+        pass
+    elif shape == tuple(rows):
+        ids = ids.reshape(M)
+    elif len(rows) == 2 and shape == (rows[0],):
+        ids = ids[:, None].expand(rows).reshape(M)
     else:
         raise ValueError(f"adapter_ids must have shape {tuple(rows)}, {(M,)} or one a sequence, got "
                          f"{tuple(adapter_ids.shape)}")
@@ -63,7 +69,9 @@ def _validate(x, base, lora_a, lora_b, adapter_ids, scales, out):
         lo, hi = int(ids.min()), int(ids.max())
         if lo < -1 or hi >= adapters:
             raise ValueError(f"adapter_ids must be in [-1, {adapters}), got {lo} to {hi}")
-    return M, N, K, R, adapters, ids.to(device=x.device, dtype=torch.int32).contiguous()
+    if ids.dtype != torch.int32 or ids.device != x.device:
+        ids = ids.to(device=x.device, dtype=torch.int32)
+    return M, N, K, R, adapters, ids.contiguous()
 
 
 def reference_lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None):
@@ -80,10 +88,10 @@ def reference_lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None):
 
 def _rows(t, width):
     """(t as rows of ``width`` dense values at one stride, that stride); None where it is not."""
-    if t.ndim == 2 and t.stride(1) == 1 and t.stride(0) >= width:
-        return t, t.stride(0)
     if t.is_contiguous():
         return t, width
+    if t.ndim == 2 and t.stride(1) == 1 and t.stride(0) >= width:
+        return t, t.stride(0)
     return None, 0
 
 
@@ -112,7 +120,7 @@ def lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None, out=None, bac
     if backend_name not in ("auto", "reference", "metal"):
         raise ValueError("backend must be one of 'reference', 'metal', 'auto'")
     tensors = (x, base, lora_a, lora_b) if scales is None else (x, base, lora_a, lora_b, scales)
-    if ci_safe_mode_enabled() or backend_name == "reference" or not values_only(*tensors):
+    if backend_name == "reference" or ci_safe_mode_enabled() or not values_only(*tensors):
         y = reference_lora_add(x, base, lora_a, lora_b, adapter_ids, scales=scales)
         return y if out is None else out.copy_(y)
     M, N, K, R, adapters, ids = _validate(x, base, lora_a, lora_b, adapter_ids, scales, out)

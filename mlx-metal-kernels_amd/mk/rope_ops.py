@@ -53,30 +53,31 @@ def _rotate(x, c, s, layout: str):
 def _validate_inputs(x, cos, sin, position_offset: int, rotary_dim=None, *, any_rows: bool = False):
     """ops/rope_ops.py:25-58.  ``any_rows``: the rows needed are the
     positions' matter, not the offset's."""
-    if x.ndim != 4:
+    shape, table = x.shape, cos.shape
+    if len(shape) != 4:
         raise ValueError(f"x must be 4-D [B,S,H,D], got {tuple(x.shape)}")
-    if cos.ndim != 2 or sin.ndim != 2:
-        raise ValueError(f"cos and sin must be 2-D [S_total, D/2], got {tuple(cos.shape)}, {tuple(sin.shape)}")
-    if cos.shape != sin.shape:
+    if table != sin.shape or len(table) != 2:
+        if cos.ndim != 2 or sin.ndim != 2:
+            raise ValueError(f"cos and sin must be 2-D [S_total, D/2], got {tuple(cos.shape)}, {tuple(sin.shape)}")
         raise ValueError(f"cos and sin must have identical shapes, got {tuple(cos.shape)}, {tuple(sin.shape)}")
-    B, S, H, D = x.shape
+    B, S, H, D = shape
     if D % 2 != 0 and rotary_dim is None:
         raise ValueError(f"RoPE requires even D, got D={D}")
     if rotary_dim is not None:
         rd = _rotary_dim(rotary_dim, D)
-        if cos.shape[1] != rd // 2:
-            raise ValueError(f"cos/sin last dim must be rotary_dim/2={rd // 2}, got {cos.shape[1]}")
-    elif cos.shape[1] != D // 2:
-        raise ValueError(f"cos/sin last dim must be D/2={D // 2}, got {cos.shape[1]}")
+        if table[1] != rd // 2:
+            raise ValueError(f"cos/sin last dim must be rotary_dim/2={rd // 2}, got {table[1]}")
+    elif table[1] != D // 2:
+        raise ValueError(f"cos/sin last dim must be D/2={D // 2}, got {table[1]}")
     if position_offset < 0:
         raise ValueError("position_offset must be non-negative")
-    if not any_rows and position_offset + S > cos.shape[0]:
+    if not any_rows and position_offset + S > table[0]:
         raise ValueError(
-            f"position_offset + S must fit in cos/sin rows, got offset={position_offset}, S={S}, rows={cos.shape[0]}"
+            f"position_offset + S must fit in cos/sin rows, got offset={position_offset}, S={S}, rows={table[0]}"
         )
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"x dtype must be float16 or bfloat16, got {x.dtype}")
-    return B, S, H, D, cos.shape[0]
+    return B, S, H, D, table[0]
 
 
 def _validate_positions(positions, B: int, S: int, rows: int, device):
@@ -85,14 +86,17 @@ def _validate_positions(positions, B: int, S: int, rows: int, device):
     the table's rows where the host may read it."""
     if not isinstance(positions, torch.Tensor):
         positions = torch.as_tensor(positions, dtype=torch.int32)
-    if positions.dtype not in (torch.int32, torch.int64):
+    dtype, shape = positions.dtype, positions.shape
+    if dtype != torch.int32 and dtype != torch.int64:
         raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-    if tuple(positions.shape) not in ((B,), (B, S)):
+    if shape != (B,) and shape != (B, S):
         raise ValueError(f"positions must have shape [B]={(B,)} or [B,S]={(B, S)}, got {tuple(positions.shape)}")
     if positions.numel() and host_checks_enabled(positions):
         lo, hi = int(positions.min()), int(positions.max()) + (S if positions.ndim == 1 else 1)
         if lo < -1 or hi > rows:
             raise ValueError(f"positions must be in [-1, {rows}) with S={S}, got {lo} to {hi - 1}")
+    if dtype == torch.int32 and positions.device == device:
+        return positions.contiguous()
     return positions.to(device=device, dtype=torch.int32).contiguous()
 
 
@@ -150,21 +154,25 @@ def apply_rope(x, cos, sin, position_offset: int = 0, *, positions=None, layout:
     backend_name = backend.lower()
     if backend_name not in ("auto", "reference", "metal"):
         raise ValueError("backend must be one of 'reference', 'metal', 'auto'")
-    if ci_safe_mode_enabled() or backend_name == "reference" or not values_only(x, cos, sin):
+    if backend_name == "reference" or ci_safe_mode_enabled() or not values_only(x, cos, sin):
         return reference_apply_rope(x, cos, sin, position_offset, positions=positions, layout=layout,
                                     rotary_dim=rotary_dim)
     B, S, H, D, rows = _validate_inputs(x, cos, sin, position_offset, rotary_dim, any_rows=positions is not None)
     dev = _lib.require_device(x)
-    pos = None if positions is None else _validate_positions(positions, B, S, rows, dev)
+    pos, per_token = None, 0
+    if positions is not None:
+        pos = _validate_positions(positions, B, S, rows, dev)
+        per_token = pos.ndim - 1
     c, s = _tables(cos, dev), _tables(sin, dev)
-    if x.stride(3) != 1 and D != 1:
+    sb, ss, sh, sd = x.stride()
+    if sd != 1 and D != 1:
         x = x.contiguous()
+        sb, ss, sh, sd = x.stride()
     y = torch.empty((B, S, H, D), dtype=x.dtype, device=dev)
-    if y.numel() == 0:
+    if B == 0 or S == 0 or H == 0:
         return y
     _lib.launch("mk_apply_rope", dev, x.data_ptr(), c.data_ptr(), s.data_ptr(), _lib.ptr(pos), y.data_ptr(), B, S, H, D,
-                x.stride(0), x.stride(1), x.stride(2), D if rotary_dim is None else rotary_dim, position_offset,
-                pos is not None and pos.ndim == 2, rows, code, _lib.dtype_code(x.dtype))
+                sb, ss, sh, rotary_dim or D, position_offset, per_token, rows, code, _lib.dtype_code(x.dtype))
     return y
 
 
