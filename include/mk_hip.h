@@ -220,7 +220,7 @@ int mk_q8_rmsnorm_qkv_rope_paged(const void* x, const void* norm_w, float eps, c
  * for i = adapter_ids[m], base[m] where i is outside [0, adapters).  x [M,K],
  * base and out [M,N] at strides in values (out may be base); a [adapters,R,K],
  * b [adapters,N,R], all in dtype (fp16 / bf16); scales fp32 [adapters] (NULL:
- * 1); 1 <= R <= 128.  Sums in fp32, one rounding.  The workspace (16-byte
+ * 1); 1 <= R <= 128, 1 <= adapters <= 4096.  Sums in fp32, one rounding.  The workspace (16-byte
  * aligned, any content) has mk_lora_workspace_bytes(M, N, K, R, adapters)
  * bytes; calls that may run concurrently need distinct ones. */
 size_t mk_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t adapters);

@@ -2,16 +2,16 @@
 //
 //   out[m] = base[m] + s_i B_i (A_i x[m]),  i = ids[m]   (i outside [0, adapters): out[m] = base[m])
 //
-// No counterpart in the reference.  Two launches: the first sums t = A_i x[m]
-// in fp32 (per slice of K, in the workspace), the second joins the slices,
-// multiplies by B_i and adds base, with one rounding.
+// No counterpart in the reference.  The rows of one adapter, up to 64 of them,
+// are a group.  One launch sums t = A_i x[m] of a group's rows in fp32 (in
+// slices of K, kept in the workspace), the next joins the slices, multiplies
+// by B_i and adds base, with one rounding.  Up to 64 rows a wave finds its
+// group by itself; beyond, a launch before them lists the groups.  So every
+// adapter's matrices are read once for 64 rows, whatever the rows' order.
 //
-// Both run on 16x16x32 matrix instructions over tiles of 16 rows, without any
-// sorting of rows: for each adapter that a tile's rows name, the products of
-// all 16 rows with it are formed and the rows that name it keep theirs, so a
-// row's values touch no other row (an infinity or NaN stays where it is).
-// Prompts, whose rows name one adapter a tile, do no product twice; a decode
-// batch is bound by reading its adapters, whatever their order.
+// Both products run on 16x16x32 matrix instructions with the rows as columns:
+// a row's values touch no other row (an infinity or NaN stays where it is),
+// and which rows share a group changes no result.
 //
 // The second product's operand t is 32 bits: it goes in as the sum of two
 // values of the storage type (relative 2^-16 for bf16, 2^-21 for fp16), in fp16
@@ -52,246 +52,374 @@ __device__ __forceinline__ typename Frag<T>::v8 load_frag(const T* p, int64_t at
   return v;
 }
 
-// The adapters of a tile's 16 rows (lane & 15), each once and in the order of
-// the rows: next() gives the number `skip` further on, -1 behind the last.
-// Uniform over the wave.
-struct TileAdapters {
-  uint64_t rest;
-  int id;
-  __device__ __forceinline__ TileAdapters(int my) : rest(__ballot(my >= 0) & 0xffffull), id(my) {}
-  __device__ __forceinline__ int next(int skip) {
-    int a = -1;
-    for (int k = 0; k <= skip; ++k) {
-      if (rest == 0) return -1;
-      a = __builtin_amdgcn_readlane(id, __builtin_ctzll(rest));
-      rest &= ~__ballot(id == a);
-    }
-    return a;
-  }
+// ---------------------------------------------------------------------------
+// groups: up to 64 rows of one adapter
+// ---------------------------------------------------------------------------
+
+constexpr int kGroupRows = 64;
+constexpr int kMaxAdapters = 4096;
+
+struct Groups {
+  const int32_t* ids;
+  const int32_t* rows;      // [groups, 64], -1 behind a group's rows; NULL: up to 64 rows in all
+  const int32_t* adapters;  // [groups + 1]: the adapter of each (-1: none), in front of them their number
+  int64_t M;
+  int count;  // of adapters
 };
 
-__device__ __forceinline__ int row_adapter(const int32_t* ids, int64_t m, int64_t M, int adapters) {
-  const int i = m < M ? ids[m] : -1;
-  return i < adapters ? i : -1;
+// Group g: its adapter (-1: rows without one), its rows (row i in lane i, -1
+// behind them), their number (0: there is no such group).  Uniform but `row`.
+__device__ __forceinline__ int find_group(const Groups& gs, int g, int* adapter, int* row) {
+  const int lane = threadIdx.x & 63;
+  if (gs.rows) {
+    if (g >= gs.adapters[0]) return 0;
+    *adapter = gs.adapters[1 + g];
+    *row = gs.rows[(int64_t)g * kGroupRows + lane];
+    return __builtin_popcountll(__ballot(*row >= 0));
+  }
+  int id = lane < gs.M ? gs.ids[lane] : -1;
+  if (id < 0 || id >= gs.count) id = -1;
+  uint64_t rest = __ballot(lane < gs.M), have = 0;
+  for (int k = 0; k <= g; ++k) {
+    if (rest == 0) return 0;
+    *adapter = __builtin_amdgcn_readlane(id, __builtin_ctzll(rest));
+    have = __ballot(id == *adapter) & rest;
+    rest &= ~have;
+  }
+  // lane i of the group's rows sends its number to lane i; the others to lanes behind them
+  const int n = __builtin_popcountll(have);
+  const uint64_t below = (1ull << lane) - 1;
+  const bool in = (have >> lane) & 1;
+  const int to = in ? __builtin_popcountll(have & below) : n + __builtin_popcountll(~have & below);
+  *row = __builtin_amdgcn_ds_permute(4 * to, in ? lane : -1);
+  return n;
+}
+
+// The groups of more than 64 rows, by one workgroup.  Rows of an adapter take
+// places in the order in which the threads get there: which rows share a group
+// changes no result.
+__global__ __launch_bounds__(1024) void lora_group_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ rows,
+                                                          int32_t* __restrict__ adapters, int64_t M, int count) {
+  __shared__ int number[kMaxAdapters + 1];  // rows of each adapter; `count`: of none
+  __shared__ int first[kMaxAdapters + 1];   // its first group
+  __shared__ int sums[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i <= count; i += 1024) number[i] = 0;
+  __syncthreads();
+  // a row's place: one addition for the rows of a wave that share the first's adapter
+  auto take = [&](int bin, bool live) {
+    const uint64_t all = __ballot(live);
+    if (all == 0) return 0;
+    const int head = __builtin_ctzll(all);
+    const int lead = __builtin_amdgcn_readlane(bin, head);
+    const uint64_t same = __ballot(live && bin == lead);
+    int at = 0;
+    if (lane == head) at = atomicAdd(&number[lead], (int)__builtin_popcountll(same));
+    at = __builtin_amdgcn_readlane(at, head) + (int)__builtin_popcountll(same & ((1ull << lane) - 1));
+    if (live && bin != lead) at = atomicAdd(&number[bin], 1);
+    return at;
+  };
+  auto bin_of = [&](int64_t m) {
+    const int i = ids[m];
+    return i < 0 || i >= count ? count : i;
+  };
+  for (int64_t m0 = 0; m0 < M; m0 += 1024) {
+    const int64_t m = m0 + tid;
+    take(m < M ? bin_of(m) : 0, m < M);
+  }
+  __syncthreads();
+  // groups of each adapter, their sum up to it; a thread has a run of adapters
+  const int per = (count + 1 + 1023) / 1024, lo = tid * per, hi = min(lo + per, count + 1);
+  int mine = 0;
+  for (int i = lo; i < hi; ++i) mine += (number[i] + kGroupRows - 1) / kGroupRows;
+  int s = mine;
+#pragma unroll
+  for (int o = 1; o < MK_WAVE; o <<= 1) {
+    const int up = __shfl_up(s, o, MK_WAVE);
+    if (lane >= o) s += up;
+  }
+  if (lane == 63) sums[wave] = s;
+  __syncthreads();
+  int before = s - mine, total = 0;
+  for (int w = 0; w < 16; ++w) {
+    if (w < wave) before += sums[w];
+    total += sums[w];
+  }
+  if (tid == 0) adapters[0] = total;
+  for (int i = lo; i < hi; ++i) {
+    first[i] = before;
+    const int n = number[i], groups = (n + kGroupRows - 1) / kGroupRows;
+    for (int g = 0; g < groups; ++g) adapters[1 + before + g] = i < count ? i : -1;
+    for (int r = n; r < groups * kGroupRows; ++r) rows[(int64_t)before * kGroupRows + r] = -1;
+    before += groups;
+    number[i] = 0;
+  }
+  __syncthreads();
+  for (int64_t m0 = 0; m0 < M; m0 += 1024) {
+    const int64_t m = m0 + tid;
+    const int bin = m < M ? bin_of(m) : 0;
+    const int at = take(bin, m < M);
+    if (m < M) rows[(int64_t)first[bin] * kGroupRows + at] = (int32_t)m;
+  }
 }
 
 // ---------------------------------------------------------------------------
-// t = A x: a workgroup of 8 waves has a tile of rows, a slice of K, and every
-// gridDim.z-th adapter of the tile; its waves take turns of 32 values of K and
-// are summed through LDS.  The product is A (ranks down) times x (rows
-// across): a lane ends with 4 ranks of one row.
+// t = A x: a workgroup of 8 waves has a group and a slice of K; its waves take
+// turns of 32 values of K and are summed through LDS.  The product is A (ranks
+// down) times x (rows across): a lane ends with 4 ranks of a row.
 // ---------------------------------------------------------------------------
 
 constexpr int kShrinkWaves = 8;
 
-template <typename T, int RT, bool VEC>
-__global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(
-    const T* __restrict__ x, int64_t x_stride, const T* __restrict__ a, const int32_t* __restrict__ ids,
-    float* __restrict__ t, int64_t M, int64_t K, int R, int adapters, int64_t k_slice) {
-  constexpr int UN = VEC ? (RT >= 4 ? 2 : 4) : 1;  // turns whose loads are in flight together
-  __shared__ f32x4 part[kShrinkWaves][RT][64];
+template <typename T, int RT, int MT, bool VEC>
+__device__ __forceinline__ void shrink_group(const T* x, int64_t x_stride, const T* ai, float* t, int64_t K, int R,
+                                             int64_t k0, int64_t k1, int rowlist, f32x4 (&part)[kShrinkWaves][RT][64]) {
+  constexpr int UN = !VEC || RT * MT > 8 ? 1 : RT * MT > 2 ? 2 : 4;  // turns whose loads are in flight together
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, grp = lane >> 4;
-  const int64_t m = (int64_t)blockIdx.x * 16 + col;
-  const int my = row_adapter(ids, m, M, adapters);
-  const int64_t k0 = (int64_t)blockIdx.y * k_slice;
-  const int64_t k1 = k0 + k_slice < K ? k0 + k_slice : K;
-  const T* xr = x + (m < M ? m : M - 1) * x_stride;
-  TileAdapters tile(my);
-  for (int i = tile.next((int)blockIdx.z); i >= 0; i = tile.next((int)gridDim.z - 1)) {
-    const T* ai = a + (int64_t)i * R * K;
-    f32x4 acc[RT];
+  const int any = __builtin_amdgcn_readfirstlane(rowlist);
+  int row[MT];
+  const T* xr[MT];
 #pragma unroll
-    for (int q = 0; q < RT; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int64_t kb = k0 + 32 * wave; kb < k1; kb += 32 * kShrinkWaves * UN) {
-      typename Frag<T>::v8 xf[UN], af[UN][RT];
+  for (int i = 0; i < MT; ++i) {
+    row[i] = __shfl(rowlist, 16 * i + col, MK_WAVE);
+    xr[i] = x + (int64_t)(row[i] < 0 ? any : row[i]) * x_stride;
+  }
+  f32x4 acc[RT][MT];
 #pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int64_t k = kb + 32 * kShrinkWaves * u + 8 * grp;
-        xf[u] = load_frag<T, VEC>(xr, k, k1);
+  for (int q = 0; q < RT; ++q)
 #pragma unroll
-        for (int q = 0; q < RT; ++q) {
-          const int r = 16 * q + col;
-          af[u][q] = load_frag<T, VEC>(ai + (int64_t)(r < R ? r : 0) * K, k, r < R ? k1 : 0);
-        }
+    for (int i = 0; i < MT; ++i) acc[q][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int64_t kb = k0 + 32 * UN * wave; kb < k1; kb += 32 * kShrinkWaves * UN) {
+    typename Frag<T>::v8 xf[UN][MT], af[UN][RT];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int64_t k = kb + 32 * u + 8 * grp;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xf[u][i] = load_frag<T, VEC>(xr[i], k, k1);
+#pragma unroll
+      for (int q = 0; q < RT; ++q) {
+        const int r = 16 * q + col;
+        af[u][q] = load_frag<T, VEC>(ai + (int64_t)(r < R ? r : 0) * K, k, r < R ? k1 : 0);
       }
-#pragma unroll
-      for (int u = 0; u < UN; ++u)
-#pragma unroll
-        for (int q = 0; q < RT; ++q) acc[q] = Frag<T>::mfma(af[u][q], xf[u], acc[q]);
     }
-    __syncthreads();  // the last adapter's sums are read
 #pragma unroll
-    for (int q = 0; q < RT; ++q) part[wave][q][lane] = acc[q];
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int q = 0; q < RT; ++q)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[q][i] = Frag<T>::mfma(af[u][q], xf[u][i], acc[q][i]);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    if (i) __syncthreads();  // the last rows' sums are read
+#pragma unroll
+    for (int q = 0; q < RT; ++q) part[wave][q][lane] = acc[q][i];
     __syncthreads();
     for (int q = wave; q < RT; q += kShrinkWaves) {
       f32x4 s = part[0][q][lane];
 #pragma unroll
       for (int w = 1; w < kShrinkWaves; ++w) s += part[w][q][lane];
-      if (my == i)
-        *reinterpret_cast<f32x4*>(t + ((int64_t)blockIdx.y * M + m) * (16 * RT) + 16 * q + 4 * grp) = s;
+      if (row[i] >= 0) *reinterpret_cast<f32x4*>(t + (int64_t)row[i] * (16 * RT) + 16 * q + 4 * grp) = s;
+    }
+  }
+}
+
+template <typename T, int RT, bool VEC>
+__global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(Groups gs, const T* __restrict__ x,
+                                                                        int64_t x_stride, const T* __restrict__ a,
+                                                                        float* __restrict__ t, int64_t K, int R,
+                                                                        int64_t k_slice) {
+  __shared__ f32x4 part[kShrinkWaves][RT][64];
+  int adapter, rowlist;
+  const int n = find_group(gs, (int)blockIdx.x, &adapter, &rowlist);
+  if (n == 0 || adapter < 0) return;
+  const int64_t k0 = (int64_t)blockIdx.y * k_slice;
+  const int64_t k1 = k0 + k_slice < K ? k0 + k_slice : K;
+  const T* ai = a + (int64_t)adapter * R * K;
+  t += (int64_t)blockIdx.y * gs.M * (16 * RT);
+  if constexpr (VEC) {
+    if (n <= 16) shrink_group<T, RT, 1, VEC>(x, x_stride, ai, t, K, R, k0, k1, rowlist, part);
+    else shrink_group<T, RT, 4, VEC>(x, x_stride, ai, t, K, R, k0, k1, rowlist, part);
+  } else {  // values one by one: 16 rows at a time leave the registers for them
+    for (int i = 0; i < n; i += 16) {
+      const int at = ((int)threadIdx.x & 63) + i;
+      const int row = __shfl(rowlist, at & 63, MK_WAVE);
+      if (i) __syncthreads();  // the last rows' sums are read
+      shrink_group<T, RT, 1, VEC>(x, x_stride, ai, t, K, R, k0, k1, at < 64 ? row : -1, part);
     }
   }
 }
 
 // ---------------------------------------------------------------------------
-// out = base + s B t: a wave has 64 outputs of up to kRowTiles tiles of rows.
-// The product is B (outputs down) times t (rows across).  The outputs of
-// instruction j are 16 (r / 4) + 4 j + r % 4 for its rows r, so that a lane
-// ends with 16 outputs side by side of one row: 32 bytes of base and out.
+// out = base + s B t: a workgroup of 4 waves has a group and `blocks` times
+// 256 outputs.  It puts both parts of t of its rows into LDS; then each wave
+// takes 64 outputs at a time.  The product is B (outputs down) times t (rows
+// across).  The outputs of instruction j are 16 (r / 4) + 4 j + r % 4 for its
+// rows r, so that a lane ends with 16 outputs side by side of one row: 32
+// bytes of base and out.
 // ---------------------------------------------------------------------------
 
-constexpr int kRowTiles = 4;
-
 template <typename T, int RT, bool VEC>
-__global__ __launch_bounds__(256) void lora_expand_kernel(
-    const T* __restrict__ base, int64_t base_stride, const T* __restrict__ b, const int32_t* __restrict__ ids,
-    const float* __restrict__ scales, const float* __restrict__ t, T* out, int64_t out_stride, int64_t M, int64_t N,
-    int R, int adapters, int slices, int row_tiles, bool wide) {
+__global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* base, int64_t base_stride,
+                                                          const T* __restrict__ b, const float* __restrict__ scales,
+                                                          const float* __restrict__ t, T* out, int64_t out_stride,
+                                                          int64_t N, int R, int slices, int blocks, bool wide) {
   typedef typename Frag<T>::v8 v8;
-  // up to 16 ranks: both parts of t in one instruction, over B twice
-  constexpr int KS = RT == 1 ? 1 : (RT + 1) / 2;
+  constexpr int RP = 16 * RT;               // ranks, whole tiles
+  constexpr int KS = RT == 1 ? 1 : RT / 2;  // up to 16 ranks: both parts in one instruction, over B twice
+  constexpr int CH = RP / 8;                // chunks of 8 ranks
+  constexpr int STRIDE = 2 * RP + 8;        // of a row in LDS: both parts, and 16 bytes that spread the rows over the banks
+  __shared__ T parts[kGroupRows][STRIDE];
+  __shared__ float backs[kGroupRows];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, grp = lane >> 4;
-  const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * 64;
-  if (n0 >= N) return;
-  const int64_t n = n0 + 16 * grp;  // this lane's first output
-  v8 bf[4][KS];
-  int held = -1;  // the adapter in bf
-  for (int rt = 0; rt < row_tiles; ++rt) {
-    const int64_t m0 = ((int64_t)blockIdx.y * row_tiles + rt) * 16;
-    if (m0 >= M) return;
-    const int64_t m = m0 + col;
-    const int my = row_adapter(ids, m, M, adapters);
-    float keep[16];
+  int adapter, rowlist;
+  const int n = find_group(gs, (int)blockIdx.y, &adapter, &rowlist);
+  if (n == 0 || (adapter < 0 && base == out)) return;
+  if (adapter >= 0) {
+    const float scale = scales ? scales[adapter] : 1.0f;
+    const int chunks = ((n + 15) & ~15) * CH;  // CH lanes a row, a power of two
+    for (int at0 = 0; at0 < chunks; at0 += 256) {
+      const int at = at0 + (int)threadIdx.x, i = at / CH, c = at % CH;
+      const int row = __shfl(rowlist, i & 63, MK_WAVE);  // (every lane: the source has to be active)
+      const int m = at < chunks ? row : -1;
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (m >= 0) {
+        const float* tr = t + (int64_t)m * RP + 8 * c;
+        for (int z = 0; z < slices; ++z, tr += gs.M * RP) {
+          const f32x4 lo = *reinterpret_cast<const f32x4*>(tr), hi = *reinterpret_cast<const f32x4*>(tr + 4);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) keep[e] = 0.0f;
-    bool mine = my < 0 && blockIdx.z == 0 && base != out;
-    TileAdapters tile(my);
-    for (int i = tile.next((int)blockIdx.z); i >= 0; i = tile.next((int)gridDim.z - 1)) {
-      if (i != held) {
-        held = i;
-        const T* bi = b + (int64_t)i * N * R;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t row = n0 + 16 * (col >> 2) + 4 * j + (col & 3);
-#pragma unroll
-          for (int s = 0; s < KS; ++s)
-            bf[j][s] = load_frag<T, VEC>(bi + (row < N ? row : N - 1) * R, RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp, R);
-        }
-      }
-      // t of this lane's row, its slices joined
-      float tv[KS][8];
-      float top = 0.0f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int at = RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) tv[s][e] = 0.0f;
-        if (my == i && at < 16 * RT) {
-          const float* tr = t + m * (16 * RT) + at;
-          for (int z = 0; z < slices; ++z, tr += M * (16 * RT)) {
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(tr), hi = *reinterpret_cast<const f32x4*>(tr + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              tv[s][e] += lo[e];
-              tv[s][4 + e] += hi[e];
-            }
+          for (int e = 0; e < 4; ++e) {
+            v[e] += lo[e];
+            v[4 + e] += hi[e];
           }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(tv[s][e]));
       }
-      float back = scales ? scales[i] : 1.0f;
-      if constexpr (sizeof(T) == 2 && __is_same(T, f16)) {
-        // the row's largest value to [2^13, 2^14)
-        top = fmaxf(top, __shfl_xor(top, 16, MK_WAVE));
-        top = fmaxf(top, __shfl_xor(top, 32, MK_WAVE));
-        int e = 0;
+      float back = scale;
+      if constexpr (__is_same(T, f16)) {  // the row's largest value to [2^13, 2^14)
+        float top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+#pragma unroll
+        for (int o = 1; o < CH; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, MK_WAVE));
+        int e = 14;
         if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
-        else e = 14;
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-          for (int q = 0; q < 8; ++q) tv[s][q] = ldexpf(tv[s][q], 14 - e);
+        for (int q = 0; q < 8; ++q) v[q] = ldexpf(v[q], 14 - e);
         back = ldexpf(back, e - 14);
       }
-      f32x4 acc[4];
+      v8 hi, lo;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        v8 hi, lo;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          hi[q] = from_f32<T>(tv[s][q]);
-          const float left = tv[s][q] - to_f32(hi[q]);
-          lo[q] = from_f32<T>(fabsf(tv[s][q]) < INFINITY ? left : 0.0f);
-        }
-        if constexpr (RT == 1) {
-          const v8 both = grp < 2 ? hi : lo;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(bf[j][s], both, acc[j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(bf[j][s], hi, acc[j]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(bf[j][s], lo, acc[j]);
-        }
+      for (int e = 0; e < 8; ++e) {
+        hi[e] = from_f32<T>(v[e]);
+        const float left = v[e] - to_f32(hi[e]);
+        lo[e] = from_f32<T>(fabsf(v[e]) < INFINITY ? left : 0.0f);
       }
-      if (my == i) {
-        mine = true;
+      if (at >= chunks) continue;
+      *reinterpret_cast<v8*>(&parts[i][8 * c]) = hi;
+      *reinterpret_cast<v8*>(&parts[i][RP + 8 * c]) = lo;
+      if (c == 0) backs[i] = back;
+    }
+    __syncthreads();
+  }
+  const T* bi = b + (int64_t)(adapter < 0 ? 0 : adapter) * N * R;
+  for (int blk = 0; blk < blocks; ++blk) {
+    const int64_t n0 = (((int64_t)blockIdx.x * blocks + blk) * 4 + wave) * 64;
+    if (n0 >= N) return;
+    const int64_t nn = n0 + 16 * grp;  // this lane's first output
+    v8 bf[4][KS];
+    if (adapter >= 0) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) keep[e] = acc[e >> 2][e & 3] * back;
+      for (int j = 0; j < 4; ++j) {
+        const int64_t r = n0 + 16 * (col >> 2) + 4 * j + (col & 3);
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+          bf[j][s] = load_frag<T, VEC>(bi + (r < N ? r : N - 1) * R, RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp, R);
       }
     }
-    if (!mine || m >= M) continue;
-    const T* br = base + m * base_stride + n;
-    T* orow = out + m * out_stride + n;
+    for (int rt = 0; rt < (n + 15) / 16; ++rt) {
+      const int m = __shfl(rowlist, 16 * rt + col, MK_WAVE);
+      const T* br = base + (int64_t)(m < 0 ? 0 : m) * base_stride + nn;
+      T* orow = out + (int64_t)(m < 0 ? 0 : m) * out_stride + nn;
+      u32x4 w[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (wide && n + 8 * h < N) {  // whole 16-byte chunks
-        const u32x4 w = ldg128(br + 8 * h);
-        u32x4 o;
+      for (int h = 0; h < 2; ++h)
+        if (wide && m >= 0 && nn + 8 * h < N) w[h] = ldg128(br + 8 * h);
+      float add[16];
+      if (adapter >= 0) {
+        f32x4 acc[4];
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float y0 = to_f32(bitcast<T>((uint16_t)w[e >> 1])) + keep[8 * h + e];
-          const float y1 = to_f32(bitcast<T>((uint16_t)(w[e >> 1] >> 16))) + keep[8 * h + e + 1];
-          o[e >> 1] = (uint32_t)bitcast<uint16_t>(from_f32<T>(y0)) |
-                      ((uint32_t)bitcast<uint16_t>(from_f32<T>(y1)) << 16);
+        for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const T* pr = parts[16 * rt + col];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          if constexpr (RT == 1) {  // chunks 0 and 1 of the first part, then of the second
+            const v8 both = *reinterpret_cast<const v8*>(pr + 8 * grp);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(bf[j][s], both, acc[j]);
+          } else {
+            const v8 hi = *reinterpret_cast<const v8*>(pr + 32 * s + 8 * grp);
+            const v8 lo = *reinterpret_cast<const v8*>(pr + RP + 32 * s + 8 * grp);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(bf[j][s], hi, acc[j]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(bf[j][s], lo, acc[j]);
+          }
         }
-        if (my < 0) o = w;
-        *reinterpret_cast<u32x4*>(orow + 8 * h) = o;
-      } else if (!wide) {
+        const float back = backs[16 * rt + col];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (n + 8 * h + e < N)
-            orow[8 * h + e] = my < 0 ? br[8 * h + e] : from_f32<T>(to_f32(br[8 * h + e]) + keep[8 * h + e]);
+        for (int e = 0; e < 16; ++e) add[e] = acc[e >> 2][e & 3] * back;
+      }
+      if (m < 0) continue;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (wide && nn + 8 * h < N) {  // whole 16-byte chunks
+          u32x4 o = w[h];
+          if (adapter >= 0) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const float y0 = to_f32(bitcast<T>((uint16_t)w[h][e >> 1])) + add[8 * h + e];
+              const float y1 = to_f32(bitcast<T>((uint16_t)(w[h][e >> 1] >> 16))) + add[8 * h + e + 1];
+              o[e >> 1] = (uint32_t)bitcast<uint16_t>(from_f32<T>(y0)) |
+                          ((uint32_t)bitcast<uint16_t>(from_f32<T>(y1)) << 16);
+            }
+          }
+          *reinterpret_cast<u32x4*>(orow + 8 * h) = o;
+        } else if (!wide) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (nn + 8 * h + e < N)
+              orow[8 * h + e] = adapter < 0 ? br[8 * h + e] : from_f32<T>(to_f32(br[8 * h + e]) + add[8 * h + e]);
+        }
       }
     }
   }
 }
 
 struct LoraPlan {
-  int64_t tiles, k_slice;
-  int slices, rank_tiles, adapters_at_once;
+  int64_t groups, k_slice, order_ints;  // most groups that there can be
+  int slices, rank_tiles, blocks;
 };
 
-inline LoraPlan lora_plan(int64_t M, int64_t K, int64_t R, int64_t adapters) {
+inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t adapters) {
   LoraPlan p;
-  p.tiles = (M + 15) / 16;
   p.rank_tiles = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
-  // decode batches: the adapters of a tile side by side; prompts: in turn
-  const int64_t most = M < adapters ? M : adapters;
-  p.adapters_at_once = M <= 64 ? (int)(most < 16 ? (most > 0 ? most : 1) : 16) : 1;
-  // K in slices of four turns of a workgroup where there are few tiles
+  const int64_t kinds = adapters + 1 < M ? adapters + 1 : M;  // adapters that rows can name, and none
+  p.groups = M <= kGroupRows ? kinds : M / kGroupRows + kinds;
+  p.order_ints = M <= kGroupRows ? 0 : (p.groups * (kGroupRows + 1) + 1 + 3) / 4 * 4;
+  // K in slices of four turns of a workgroup where there are few groups
   const int64_t turn = 32 * kShrinkWaves;
   int64_t s = (K + 4 * turn - 1) / (4 * turn);
-  const int64_t fill = (256 + p.tiles - 1) / p.tiles;
+  const int64_t full = (M + kGroupRows - 1) / kGroupRows;
+  const int64_t fill = (256 + full - 1) / full;
   if (s > fill) s = fill;
   p.k_slice = (K + s - 1) / s;
   p.k_slice = (p.k_slice + turn - 1) / turn * turn;
   p.slices = (int)((K + p.k_slice - 1) / p.k_slice);
+  // outputs of a workgroup: 256 to 2048, a thousand workgroups left
+  const int64_t work = (N + 255) / 256 * full;
+  p.blocks = work >= 8192 ? 8 : work >= 4096 ? 4 : work >= 2048 ? 2 : 1;
   return p;
 }
 
@@ -301,46 +429,47 @@ extern "C" {
 
 size_t mk_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t adapters) {
   if (M <= 0 || N <= 0 || K <= 0 || R <= 0 || R > 128 || adapters <= 0) return 0;
-  const LoraPlan p = lora_plan(M, K, R, adapters);
-  return (size_t)p.slices * M * 16 * p.rank_tiles * sizeof(float);
+  const LoraPlan p = lora_plan(M, N, K, R, adapters);
+  return ((size_t)p.order_ints + (size_t)p.slices * M * 16 * p.rank_tiles) * sizeof(float);
 }
 
 int mk_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_stride, const void* a, const void* b,
                 const int32_t* adapter_ids, const float* scales, void* out, int64_t out_stride, int64_t M, int64_t N,
                 int64_t K, int64_t R, int64_t adapters, int dtype, void* workspace, size_t workspace_bytes,
                 void* stream) {
-  MK_REQUIRE(M >= 0 && N >= 0 && K > 0 && R > 0 && R <= 128 && adapters >= 0);
-  MK_REQUIRE(M < (1LL << 20) && N < (1LL << 24) && K < (1LL << 31) && adapters < (1LL << 31));
+  MK_REQUIRE(M >= 0 && N >= 0 && K > 0 && R > 0 && R <= 128 && adapters > 0 && adapters <= kMaxAdapters);
+  MK_REQUIRE(M < (1LL << 20) && N < (1LL << 24) && K < (1LL << 31));
   MK_REQUIRE(x_stride >= K && base_stride >= N && out_stride >= N && (out != base || out_stride == base_stride));
   MK_REQUIRE(dtype == MK_DT_F16 || dtype == MK_DT_BF16);
   if (M == 0 || N == 0) return MK_OK;
-  MK_REQUIRE(x && base && adapter_ids && out && (adapters == 0 || (a && b)));
-  MK_REQUIRE(adapters == 0 || (workspace && workspace_bytes >= mk_lora_workspace_bytes(M, N, K, R, adapters) &&
-                               mk_aligned(workspace, 16)));
+  MK_REQUIRE(x && base && adapter_ids && out && a && b && workspace && mk_aligned(workspace, 16));
+  MK_REQUIRE(workspace_bytes >= mk_lora_workspace_bytes(M, N, K, R, adapters));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  float* t = reinterpret_cast<float*>(workspace);
-  const LoraPlan p = lora_plan(M, K, R, adapters);
+  const LoraPlan p = lora_plan(M, N, K, R, adapters);
+  int32_t* order = reinterpret_cast<int32_t*>(workspace);
+  float* t = reinterpret_cast<float*>(workspace) + p.order_ints;
   const bool vec_a = K % 8 == 0 && x_stride % 8 == 0 && mk_aligned(x, 16) && mk_aligned(a, 16);
   const bool vec_b = R % 8 == 0 && mk_aligned(b, 16);
   const bool wide = N % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && mk_aligned(base, 16) &&
                     mk_aligned(out, 16);
-  const int row_tiles = p.tiles >= kRowTiles ? kRowTiles : 1;
-  const dim3 shrink((unsigned)p.tiles, (unsigned)p.slices, (unsigned)p.adapters_at_once);
-  const dim3 expand((unsigned)((N + 255) / 256), (unsigned)((p.tiles + row_tiles - 1) / row_tiles),
-                    (unsigned)p.adapters_at_once);
-#define MK_SHRINK(T, RT, V)                                                                                      \
-  lora_shrink_kernel<T, RT, V><<<shrink, 64 * kShrinkWaves, 0, st>>>((const T*)x, x_stride, (const T*)a, adapter_ids, \
-                                                                     t, M, K, (int)R, (int)adapters, p.k_slice)
-#define MK_EXPAND(T, RT, V)                                                                                       \
-  lora_expand_kernel<T, RT, V><<<expand, 256, 0, st>>>((const T*)base, base_stride, (const T*)b, adapter_ids, scales, \
-                                                       t, (T*)out, out_stride, M, N, (int)R, (int)adapters, p.slices, \
-                                                       row_tiles, wide)
+  Groups gs = {adapter_ids, nullptr, nullptr, M, (int)adapters};
+  if (M > kGroupRows) {
+    gs.rows = order;
+    gs.adapters = order + p.groups * kGroupRows;
+    lora_group_kernel<<<1, 1024, 0, st>>>(adapter_ids, order, order + p.groups * kGroupRows, M, (int)adapters);
+  }
+  const dim3 shrink((unsigned)p.groups, (unsigned)p.slices);
+  const dim3 expand((unsigned)((N + 256 * p.blocks - 1) / (256 * p.blocks)), (unsigned)p.groups);
+#define MK_SHRINK(T, RT, V)                                                                                         \
+  lora_shrink_kernel<T, RT, V><<<shrink, 64 * kShrinkWaves, 0, st>>>(gs, (const T*)x, x_stride, (const T*)a, t, K, \
+                                                                     (int)R, p.k_slice)
+#define MK_EXPAND(T, RT, V)                                                                                      \
+  lora_expand_kernel<T, RT, V><<<expand, 256, 0, st>>>(gs, (const T*)base, base_stride, (const T*)b, scales, t, \
+                                                       (T*)out, out_stride, N, (int)R, p.slices, p.blocks, wide)
 #define MK_LORA(T, RT)                  \
   do {                                  \
-    if (adapters) {                     \
-      if (vec_a) MK_SHRINK(T, RT, true); \
-      else MK_SHRINK(T, RT, false);     \
-    }                                   \
+    if (vec_a) MK_SHRINK(T, RT, true);  \
+    else MK_SHRINK(T, RT, false);       \
     if (vec_b) MK_EXPAND(T, RT, true);  \
     else MK_EXPAND(T, RT, false);       \
   } while (0)

@@ -18,7 +18,7 @@ from ._common import ACT_DTYPES, as_dense, ci_safe_mode_enabled, values_only
 from .kv_cache_ops import host_checks_enabled
 from .mlp_block_ops import quantized_linear
 
-MAX_RANK = 128
+MAX_RANK, MAX_ADAPTERS = 128, 4096
 
 
 def _validate(x, base, lora_a, lora_b, adapter_ids, scales, out):
@@ -36,8 +36,9 @@ def _validate(x, base, lora_a, lora_b, adapter_ids, scales, out):
     if a_shape[2] != K or lora_b.shape != (adapters, N, R):
         raise ValueError(f"lora_a and lora_b must be [ADAPTERS,R,{K}] and [ADAPTERS,{N},R], got {tuple(lora_a.shape)}, "
                          f"{tuple(lora_b.shape)}")
-    if K < 1 or not 1 <= R <= MAX_RANK:
-        raise ValueError(f"K must be positive and R in [1, {MAX_RANK}], got K={K}, R={R}")
+    if K < 1 or not 1 <= R <= MAX_RANK or adapters > MAX_ADAPTERS:
+        raise ValueError(f"K must be positive, R in [1, {MAX_RANK}] and ADAPTERS at most {MAX_ADAPTERS}, got K={K}, "
+                         f"R={R}, ADAPTERS={adapters}")
     dtype = x.dtype
     if dtype not in ACT_DTYPES:
         raise TypeError(f"x dtype must be float16 or bfloat16, got {x.dtype}")
@@ -141,14 +142,16 @@ def lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None, out=None, bac
         target, out_stride = _rows(out, N)
         if target is None:
             target, out_stride = torch.empty(base.shape, dtype=base.dtype, device=dev), N
-    if M and N:
+    if not adapters:
+        target.copy_(base)
+    elif M and N:
         a, b = lora_a.contiguous(), lora_b.contiguous()
         scales = as_dense(scales, torch.float32)
         size = _lib.load().mk_lora_workspace_bytes(M, N, K, R, adapters)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        _lib.launch("mk_lora_add", dev, x2.data_ptr(), x_stride, b2.data_ptr(), base_stride, a.data_ptr() or None,
-                    b.data_ptr() or None, ids.data_ptr(), _lib.ptr(scales), target.data_ptr(), out_stride, M, N, K, R,
-                    adapters, _lib.dtype_code(x.dtype), ws.data_ptr() or None, size)
+        _lib.launch("mk_lora_add", dev, x2.data_ptr(), x_stride, b2.data_ptr(), base_stride, a.data_ptr(),
+                    b.data_ptr(), ids.data_ptr(), _lib.ptr(scales), target.data_ptr(), out_stride, M, N, K, R,
+                    adapters, _lib.dtype_code(x.dtype), ws.data_ptr(), size)
     if out is not None and target is not out:
         out.copy_(target)
         return out

@@ -19,7 +19,8 @@ DTYPES = [torch.float16, torch.bfloat16]
 SHAPES = [(1, 64, 64, 16, 1), (1, 6144, 4096, 16, 4), (2, 1, 1, 1, 1), (3, 100, 72, 8, 2), (16, 64, 32, 16, 3),
           (17, 65, 33, 17, 2), (5, 40, 30, 4, 3), (33, 130, 264, 32, 9), (20, 48, 520, 33, 20), (64, 256, 96, 64, 4),
           (7, 200, 1000, 128, 2), (65, 72, 2056, 48, 1), (130, 1024, 136, 100, 5), (300, 96, 512, 16, 2),
-          (31, 8, 4100, 2, 3), (48, 4096, 8, 127, 2), (70, 328, 1504, 64, 7)]
+          (31, 8, 4100, 2, 3), (48, 4096, 8, 127, 2), (70, 328, 1504, 64, 7), (64, 40, 64, 8, 80), (2000, 72, 96, 8, 300),
+          (200, 16, 24, 3, 4096), (1100, 300, 520, 128, 2)]
 
 
 def on(dev, *tensors):

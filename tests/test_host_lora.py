@@ -90,6 +90,7 @@ def test_refusals():
     for kw in (dict(x=x[:, :7]), dict(base=base[:3]), dict(base=base[None]), dict(lora_a=a[0]), dict(lora_b=b[:2]),
                dict(lora_b=b[:, :5]), dict(lora_a=a[:, :1]), dict(adapter_ids=ids[:3]), dict(adapter_ids=[0, 1, 2, 3]),
                dict(adapter_ids=[0, 1, 2, -2]), dict(scales=s[:2]), dict(backend="triton"),
+               dict(lora_a=torch.zeros(4097, 2, 8).half(), lora_b=torch.zeros(4097, 6, 2).half(), scales=None),
                dict(lora_a=a[:, :0], lora_b=b[:, :, :0]), dict(x=x[:, :0], lora_a=a[:, :, :0]),
                dict(lora_a=torch.zeros(1, 129, 8).half(), lora_b=torch.zeros(1, 6, 129).half())):
         with pytest.raises(ValueError):
