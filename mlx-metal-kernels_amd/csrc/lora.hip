@@ -37,13 +37,24 @@ struct Frag<bf16> {
   }
 };
 
+// two values in one conversion
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (__is_same(T, bf16)) {
+    return bitcast<uint32_t>(__builtin_convertvector((f32x2){a, b}, bf16x2));
+  } else {
+    return bitcast<uint32_t>(f16x2{(f16)a, (f16)b});
+  }
+}
+
 // 8 values p[at .. at + 8), zeros from `end` on
 template <typename T, bool VEC>
 __device__ __forceinline__ typename Frag<T>::v8 load_frag(const T* p, int64_t at, int64_t end) {
   typename Frag<T>::v8 v;
-  if constexpr (VEC) {  // whole 16-byte chunks
-    u32x4 w = {0u, 0u, 0u, 0u};
-    if (at < end) w = ldg128(p + at);
+  if constexpr (VEC) {  // whole 16-byte chunks; no branch, so that loads stay in flight beside it
+    u32x4 w = ldg128(p + (at < end ? at : 0));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = at < end ? w[e] : 0u;
     v = bitcast<typename Frag<T>::v8>(w);
   } else {
 #pragma unroll
@@ -175,6 +186,7 @@ template <typename T, int RT, int MT, bool VEC>
 __device__ __forceinline__ void shrink_group(const T* x, int64_t x_stride, const T* ai, float* t, int64_t K, int R,
                                              int64_t k0, int64_t k1, int rowlist, f32x4 (&part)[kShrinkWaves][RT][64]) {
   constexpr int UN = !VEC || RT * MT > 8 ? 1 : RT * MT > 2 ? 2 : 4;  // turns whose loads are in flight together
+  constexpr bool AHEAD = VEC && RT * MT <= 16;  // (more would not fit the registers)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, grp = lane >> 4;
   const int any = __builtin_amdgcn_readfirstlane(rowlist);
@@ -190,25 +202,46 @@ __device__ __forceinline__ void shrink_group(const T* x, int64_t x_stride, const
   for (int q = 0; q < RT; ++q)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[q][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int64_t kb = k0 + 32 * UN * wave; kb < k1; kb += 32 * kShrinkWaves * UN) {
-    typename Frag<T>::v8 xf[UN][MT], af[UN][RT];
+  struct Turns {
+    typename Frag<T>::v8 x[UN][MT], a[UN][RT];
+  };
+  auto load = [&](int64_t kb) {
+    Turns f;
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int64_t k = kb + 32 * u + 8 * grp;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) xf[u][i] = load_frag<T, VEC>(xr[i], k, k1);
+      for (int i = 0; i < MT; ++i) f.x[u][i] = load_frag<T, VEC>(xr[i], k, k1);
 #pragma unroll
       for (int q = 0; q < RT; ++q) {
         const int r = 16 * q + col;
-        af[u][q] = load_frag<T, VEC>(ai + (int64_t)(r < R ? r : 0) * K, k, r < R ? k1 : 0);
+        f.a[u][q] = load_frag<T, VEC>(ai + (int64_t)(r < R ? r : 0) * K, k, r < R ? k1 : 0);
       }
     }
+    return f;
+  };
+  auto multiply = [&](const Turns& f) {
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
       for (int q = 0; q < RT; ++q)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[q][i] = Frag<T>::mfma(af[u][q], xf[u][i], acc[q][i]);
+        for (int i = 0; i < MT; ++i) acc[q][i] = Frag<T>::mfma(f.a[u][q], f.x[u][i], acc[q][i]);
+  };
+  constexpr int64_t step = 32 * kShrinkWaves * UN;
+  int64_t kb = k0 + 32 * UN * wave;
+  if constexpr (AHEAD) {  // the next turn is on its way while one is multiplied
+    if (kb < k1) {
+      Turns cur = load(kb);
+      for (kb += step; kb < k1; kb += step) {
+        const Turns next = load(kb);
+        multiply(cur);
+        cur = next;
+      }
+      multiply(cur);
+    }
+  } else {
+    for (; kb < k1; kb += step) multiply(load(kb));
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
@@ -254,10 +287,12 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(Groups g
 // ---------------------------------------------------------------------------
 // out = base + s B t: a workgroup of 4 waves has a group and `blocks` times
 // 256 outputs.  It puts both parts of t of its rows into LDS; then each wave
-// takes 64 outputs at a time.  The product is B (outputs down) times t (rows
-// across).  The outputs of instruction j are 16 (r / 4) + 4 j + r % 4 for its
-// rows r, so that a lane ends with 16 outputs side by side of one row: 32
-// bytes of base and out.
+// takes 64 outputs at a time.  The product is t (rows down) times B (outputs
+// across).  Instruction j has the outputs 4 c + j for its columns c, so that a
+// lane ends with 4 outputs side by side of 4 rows, and an access of 8 bytes a
+// lane covers 128 bytes each of 4 rows.  Bound by the base and out streams, for
+// which the 128 bytes count: copying 4093 rows x 14336 in 64-byte pieces takes
+// 57 us, in these 47.
 // ---------------------------------------------------------------------------
 
 template <typename T, int RT, bool VEC>
@@ -271,13 +306,33 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
   constexpr int CH = RP / 8;                // chunks of 8 ranks
   constexpr int STRIDE = 2 * RP + 8;        // of a row in LDS: both parts, and 16 bytes that spread the rows over the banks
   __shared__ T parts[kGroupRows][STRIDE];
-  __shared__ float backs[kGroupRows];
+  __shared__ f32x4 backs[kGroupRows / 4];
+  __shared__ int64_t at_base[kGroupRows], at_out[kGroupRows];  // where the rows begin: products of 64 bits are slow
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, grp = lane >> 4;
   int adapter, rowlist;
   const int n = find_group(gs, (int)blockIdx.y, &adapter, &rowlist);
   if (n == 0 || (adapter < 0 && base == out)) return;
-  if (adapter >= 0) {
+  if (wave == 0) {
+    at_base[lane] = rowlist * base_stride;
+    at_out[lane] = rowlist * out_stride;
+  }
+  if (adapter < 0) {  // rows without an adapter
+    const int64_t c0 = (int64_t)blockIdx.x * blocks * 256, c1 = c0 + 256 * blocks < N ? c0 + 256 * blocks : N;
+    for (int i = 0; i < n; ++i) {
+      const int64_t m = __builtin_amdgcn_readlane(rowlist, i);
+      const T* br = base + m * base_stride;
+      T* orow = out + m * out_stride;
+      if (wide) {
+        for (int64_t c = c0 + 4 * (int)threadIdx.x; c < c1; c += 4 * 256)
+          *reinterpret_cast<u32x2*>(orow + c) = ldg64(br + c);
+      } else {
+        for (int64_t c = c0 + (int)threadIdx.x; c < c1; c += 256) orow[c] = br[c];
+      }
+    }
+    return;
+  }
+  {
     const float scale = scales ? scales[adapter] : 1.0f;
     const int chunks = ((n + 15) & ~15) * CH;  // CH lanes a row, a power of two
     for (int at0 = 0; at0 < chunks; at0 += 256) {
@@ -319,78 +374,95 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
       if (at >= chunks) continue;
       *reinterpret_cast<v8*>(&parts[i][8 * c]) = hi;
       *reinterpret_cast<v8*>(&parts[i][RP + 8 * c]) = lo;
-      if (c == 0) backs[i] = back;
+      if (c == 0) reinterpret_cast<float*>(backs)[i] = back;
     }
-    __syncthreads();
   }
-  const T* bi = b + (int64_t)(adapter < 0 ? 0 : adapter) * N * R;
+  __syncthreads();
+  const T* bi = b + (int64_t)adapter * N * R;
   for (int blk = 0; blk < blocks; ++blk) {
     const int64_t n0 = (((int64_t)blockIdx.x * blocks + blk) * 4 + wave) * 64;
     if (n0 >= N) return;
-    const int64_t nn = n0 + 16 * grp;  // this lane's first output
+    const int64_t nn = n0 + 4 * col;  // this lane's first output
     v8 bf[4][KS];
-    if (adapter >= 0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t r = n0 + 16 * (col >> 2) + 4 * j + (col & 3);
+    for (int j = 0; j < 4; ++j) {
+      const int64_t r = nn + j;
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-          bf[j][s] = load_frag<T, VEC>(bi + (r < N ? r : N - 1) * R, RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp, R);
+      for (int s = 0; s < KS; ++s)
+        bf[j][s] = load_frag<T, VEC>(bi + (r < N ? r : N - 1) * R, RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp, R);
+    }
+    auto product = [&](int rt, f32x4 (&acc)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const T* pr = parts[16 * rt + col];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        if constexpr (RT == 1) {  // chunks 0 and 1 of the first part, then of the second
+          const v8 both = *reinterpret_cast<const v8*>(pr + 8 * grp);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(both, bf[j][s], acc[j]);
+        } else {
+          const v8 hi = *reinterpret_cast<const v8*>(pr + 32 * s + 8 * grp);
+          const v8 lo = *reinterpret_cast<const v8*>(pr + RP + 32 * s + 8 * grp);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(hi, bf[j][s], acc[j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(lo, bf[j][s], acc[j]);
+        }
+      }
+    };
+    const T* bn = base + nn;
+    T* on = out + nn;
+    int rt = 0;
+    if (wide && n0 + 64 <= N && n >= 16) {
+      // whole tiles, without a branch: base of the next 16 rows is on its way while these are computed
+      const int whole = n / 16;
+      u32x2 w[4], next[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = ldg64(bn + at_base[4 * grp + i]);
+      for (; rt < whole; ++rt) {
+        const int then = 16 * (rt + 1 < whole ? rt + 1 : rt) + 4 * grp;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next[i] = ldg64(bn + at_base[then + i]);
+        f32x4 acc[4];
+        product(rt, acc);
+        const f32x4 back = backs[4 * rt + grp];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          u32x2 o;
+#pragma unroll
+          for (int j = 0; j < 4; j += 2)
+            o[j >> 1] = pack2<T>(fmaf(acc[j][i], back[i], to_f32(bitcast<T>((uint16_t)w[i][j >> 1]))),
+                                 fmaf(acc[j + 1][i], back[i], to_f32(bitcast<T>((uint16_t)(w[i][j >> 1] >> 16)))));
+          *reinterpret_cast<u32x2*>(on + at_out[16 * rt + 4 * grp + i]) = o;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = next[i];
       }
     }
-    for (int rt = 0; rt < (n + 15) / 16; ++rt) {
-      const int m = __shfl(rowlist, 16 * rt + col, MK_WAVE);
-      const T* br = base + (int64_t)(m < 0 ? 0 : m) * base_stride + nn;
-      T* orow = out + (int64_t)(m < 0 ? 0 : m) * out_stride + nn;
-      u32x4 w[2];
+    for (; 16 * rt < n; ++rt) {
+      f32x4 acc[4];
+      product(rt, acc);
+      const f32x4 back = backs[4 * rt + grp];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (wide && m >= 0 && nn + 8 * h < N) w[h] = ldg128(br + 8 * h);
-      float add[16];
-      if (adapter >= 0) {
-        f32x4 acc[4];
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * rt + 4 * grp + i;
+        if (r >= n) continue;
+        const T* br = bn + at_base[r];
+        T* orow = on + at_out[r];
+        if (wide) {  // whole 8-byte chunks
+          if (nn >= N) continue;
+          const u32x2 w = ldg64(br);
+          u32x2 o;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const T* pr = parts[16 * rt + col];
+          for (int j = 0; j < 4; j += 2)
+            o[j >> 1] = pack2<T>(fmaf(acc[j][i], back[i], to_f32(bitcast<T>((uint16_t)w[j >> 1]))),
+                                 fmaf(acc[j + 1][i], back[i], to_f32(bitcast<T>((uint16_t)(w[j >> 1] >> 16)))));
+          *reinterpret_cast<u32x2*>(orow) = o;
+        } else {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          if constexpr (RT == 1) {  // chunks 0 and 1 of the first part, then of the second
-            const v8 both = *reinterpret_cast<const v8*>(pr + 8 * grp);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(bf[j][s], both, acc[j]);
-          } else {
-            const v8 hi = *reinterpret_cast<const v8*>(pr + 32 * s + 8 * grp);
-            const v8 lo = *reinterpret_cast<const v8*>(pr + RP + 32 * s + 8 * grp);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(bf[j][s], hi, acc[j]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(bf[j][s], lo, acc[j]);
-          }
-        }
-        const float back = backs[16 * rt + col];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) add[e] = acc[e >> 2][e & 3] * back;
-      }
-      if (m < 0) continue;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (wide && nn + 8 * h < N) {  // whole 16-byte chunks
-          u32x4 o = w[h];
-          if (adapter >= 0) {
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float y0 = to_f32(bitcast<T>((uint16_t)w[h][e >> 1])) + add[8 * h + e];
-              const float y1 = to_f32(bitcast<T>((uint16_t)(w[h][e >> 1] >> 16))) + add[8 * h + e + 1];
-              o[e >> 1] = (uint32_t)bitcast<uint16_t>(from_f32<T>(y0)) |
-                          ((uint32_t)bitcast<uint16_t>(from_f32<T>(y1)) << 16);
-            }
-          }
-          *reinterpret_cast<u32x4*>(orow + 8 * h) = o;
-        } else if (!wide) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (nn + 8 * h + e < N)
-              orow[8 * h + e] = adapter < 0 ? br[8 * h + e] : from_f32<T>(to_f32(br[8 * h + e]) + add[8 * h + e]);
+          for (int j = 0; j < 4; ++j)
+            if (nn + j < N) orow[j] = from_f32<T>(fmaf(acc[j][i], back[i], to_f32(br[j])));
         }
       }
     }
@@ -450,8 +522,8 @@ int mk_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_
   float* t = reinterpret_cast<float*>(workspace) + p.order_ints;
   const bool vec_a = K % 8 == 0 && x_stride % 8 == 0 && mk_aligned(x, 16) && mk_aligned(a, 16);
   const bool vec_b = R % 8 == 0 && mk_aligned(b, 16);
-  const bool wide = N % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && mk_aligned(base, 16) &&
-                    mk_aligned(out, 16);
+  const bool wide = N % 4 == 0 && base_stride % 4 == 0 && out_stride % 4 == 0 && mk_aligned(base, 8) &&
+                    mk_aligned(out, 8);
   Groups gs = {adapter_ids, nullptr, nullptr, M, (int)adapters};
   if (M > kGroupRows) {
     gs.rows = order;
