@@ -130,14 +130,22 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(const int32_t* __restr
     if (live && bin != lead) at = atomicAdd(&number[bin], 1);
     return at;
   };
-  auto bin_of = [&](int64_t m) {
-    const int i = ids[m];
-    return i < 0 || i >= count ? count : i;
+  constexpr int ROWS = 8;  // of a thread, their ids on the way together
+  int bin[ROWS], at[ROWS];
+  auto read = [&](int64_t m0) {
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      const int64_t m = m0 + 1024 * u + tid;
+      bin[u] = ids[m < M ? m : 0];
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      if (bin[u] < 0 || bin[u] >= count) bin[u] = count;
+      const int64_t m = m0 + 1024 * u;
+      if (m < M) at[u] = take(bin[u], m + tid < M);  // (uniform)
+    }
   };
-  for (int64_t m0 = 0; m0 < M; m0 += 1024) {
-    const int64_t m = m0 + tid;
-    take(m < M ? bin_of(m) : 0, m < M);
-  }
+  for (int64_t m0 = 0; m0 < M; m0 += 1024 * ROWS) read(m0);
   __syncthreads();
   // groups of each adapter, their sum up to it; a thread has a run of adapters
   const int per = (count + 1 + 1023) / 1024, lo = tid * per, hi = min(lo + per, count + 1);
@@ -166,11 +174,13 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(const int32_t* __restr
     number[i] = 0;
   }
   __syncthreads();
-  for (int64_t m0 = 0; m0 < M; m0 += 1024) {
-    const int64_t m = m0 + tid;
-    const int bin = m < M ? bin_of(m) : 0;
-    const int at = take(bin, m < M);
-    if (m < M) rows[(int64_t)first[bin] * kGroupRows + at] = (int32_t)m;
+  for (int64_t m0 = 0; m0 < M; m0 += 1024 * ROWS) {
+    if (M > 1024 * ROWS) read(m0);  // (else the places are those from before)
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      const int64_t m = m0 + 1024 * u + tid;
+      if (m < M) rows[(int64_t)first[bin[u]] * kGroupRows + at[u]] = (int32_t)m;
+    }
   }
 }
 
@@ -332,6 +342,19 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
     }
     return;
   }
+  const T* bi = b + (int64_t)adapter * N * R;
+  v8 bf[4][KS];
+  auto load_b = [&](int64_t n0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t r = n0 + 4 * col + j;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        bf[j][s] = load_frag<T, VEC>(bi + (r < N ? r : N - 1) * R, RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp, R);
+    }
+  };
+  int64_t n0 = ((int64_t)blockIdx.x * blocks * 4 + wave) * 64;
+  load_b(n0);  // on the way while t is joined
   {
     const float scale = scales ? scales[adapter] : 1.0f;
     const int chunks = ((n + 15) & ~15) * CH;  // CH lanes a row, a power of two
@@ -377,20 +400,11 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
       if (c == 0) reinterpret_cast<float*>(backs)[i] = back;
     }
   }
-  __syncthreads();
-  const T* bi = b + (int64_t)adapter * N * R;
-  for (int blk = 0; blk < blocks; ++blk) {
-    const int64_t n0 = (((int64_t)blockIdx.x * blocks + blk) * 4 + wave) * 64;
+  lds_barrier();  // (the loads of B stay in flight)
+  for (int blk = 0; blk < blocks; ++blk, n0 += 256) {
     if (n0 >= N) return;
+    if (blk) load_b(n0);
     const int64_t nn = n0 + 4 * col;  // this lane's first output
-    v8 bf[4][KS];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = nn + j;
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-        bf[j][s] = load_frag<T, VEC>(bi + (r < N ? r : N - 1) * R, RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp, R);
-    }
     auto product = [&](int rt, f32x4 (&acc)[4]) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -441,6 +455,12 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
       }
     }
     for (; 16 * rt < n; ++rt) {
+      u32x2 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * rt + 4 * grp + i;
+        if (wide) w[i] = ldg64(base + at_base[r < n ? r : 0] + (nn < N ? nn : 0));
+      }
       f32x4 acc[4];
       product(rt, acc);
       const f32x4 back = backs[4 * rt + grp];
@@ -448,21 +468,21 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
       for (int i = 0; i < 4; ++i) {
         const int r = 16 * rt + 4 * grp + i;
         if (r >= n) continue;
-        const T* br = bn + at_base[r];
         T* orow = on + at_out[r];
         if (wide) {  // whole 8-byte chunks
           if (nn >= N) continue;
-          const u32x2 w = ldg64(br);
           u32x2 o;
 #pragma unroll
           for (int j = 0; j < 4; j += 2)
-            o[j >> 1] = pack2<T>(fmaf(acc[j][i], back[i], to_f32(bitcast<T>((uint16_t)w[j >> 1]))),
-                                 fmaf(acc[j + 1][i], back[i], to_f32(bitcast<T>((uint16_t)(w[j >> 1] >> 16)))));
+            o[j >> 1] = pack2<T>(fmaf(acc[j][i], back[i], to_f32(bitcast<T>((uint16_t)w[i][j >> 1]))),
+                                 fmaf(acc[j + 1][i], back[i], to_f32(bitcast<T>((uint16_t)(w[i][j >> 1] >> 16)))));
           *reinterpret_cast<u32x2*>(orow) = o;
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < 4; ++j) {
+            const T* br = bn + at_base[r];
             if (nn + j < N) orow[j] = from_f32<T>(fmaf(acc[j][i], back[i], to_f32(br[j])));
+          }
         }
       }
     }
@@ -484,14 +504,18 @@ inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t ad
   const int64_t turn = 32 * kShrinkWaves;
   int64_t s = (K + 4 * turn - 1) / (4 * turn);
   const int64_t full = (M + kGroupRows - 1) / kGroupRows;
-  const int64_t fill = (256 + full - 1) / full;
-  if (s > fill) s = fill;
+  const int64_t fill = 256 / p.groups;  // one round of a workgroup for each CU
+  if (s > fill) s = fill > 1 ? fill : 1;
   p.k_slice = (K + s - 1) / s;
   p.k_slice = (p.k_slice + turn - 1) / turn * turn;
   p.slices = (int)((K + p.k_slice - 1) / p.k_slice);
-  // outputs of a workgroup: 256 to 2048, a thousand workgroups left
+  // Outputs of a workgroup: joining t and finding the group count less over
+  // more of them, and fewer workgroups fill the CUs less.  256 against 512
+  // outputs (us a call): 512 rows x 6144, rank 16 (192 workgroups of 256):
+  // 21.4 / 24.0; 2000 rows x 8192, rank 128 (1024): 74.5 / 62.8; 4093 rows x
+  // 14336, rank 64 (3584): 90.3 / 89.7, and 90.7 with 1024.
   const int64_t work = (N + 255) / 256 * full;
-  p.blocks = work >= 8192 ? 8 : work >= 4096 ? 4 : work >= 2048 ? 2 : 1;
+  p.blocks = work >= 8192 ? 4 : work >= 1024 ? 2 : 1;
   return p;
 }
 
