@@ -8,7 +8,8 @@
 // inputs.  Counts change by integer atomics, whose order does not matter.
 //
 // The moves are bound by memory: a page is read and written once, 16 bytes a
-// lane, by a workgroup per (page, tensor).
+// lane.  509 pages of 16 KB in 64 arrays take 202 us (5.28 TB/s, a large copy's
+// rate); with stores kept in the L2 215.
 #include "common.h"
 
 namespace {
@@ -20,28 +21,78 @@ struct PageTensors {
   int64_t bytes[kMaxTensors];  // of a page
 };
 
-// one page, by a workgroup
-__device__ __forceinline__ void copy_page(uint8_t* base, int64_t bytes, int64_t src, int64_t dst) {
-  const uint8_t* from = base + src * bytes;
-  uint8_t* to = base + dst * bytes;
-  if (((reinterpret_cast<uintptr_t>(base) | (uintptr_t)bytes) & 15) == 0) {
-    for (int64_t o = 16 * (int64_t)threadIdx.x; o < bytes; o += 16 * 256)
-      *reinterpret_cast<u32x4*>(to + o) = ldg128_stream(from + o);
-  } else {
-    for (int64_t o = threadIdx.x; o < bytes; o += 256) to[o] = from[o];
+// Pages src[i] -> dst[i], i < m, in every array: m = *count (n where count is
+// NULL), src = dst + m where src is NULL.  Entries outside [0, num_pages) and
+// pages onto themselves are skipped.  1 << lgl lanes move a page, so a
+// workgroup takes 256 >> lgl of an array (509 pages of 256 bytes in 64 arrays:
+// 5.7 us, 19 with a workgroup a page).  Where the device knows their number,
+// workgroups go round until all are done: those of empty entries would cost a
+// trip to memory each (11 pages of 64 arrays in a list of 32: 16 us).
+__global__ __launch_bounds__(256) void copy_pages_kernel(PageTensors t, int tensors, const int32_t* __restrict__ src,
+                                                         const int32_t* __restrict__ dst,
+                                                         const int32_t* __restrict__ count, int n, int lgl,
+                                                         int64_t num_pages) {
+  const int m = count ? min(*count, n) : n;
+  if (!src) src = dst + m;
+  const int lane = threadIdx.x & ((1 << lgl) - 1), lanes = 1 << lgl;
+  const int per = 256 >> lgl;
+  const int64_t work = (int64_t)((m + per - 1) / per) * tensors;
+  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const int batch = (int)(w / tensors), k = (int)(w - (int64_t)batch * tensors);
+    const int i = batch * per + ((int)threadIdx.x >> lgl);
+    if (i >= m) continue;
+    const int64_t a = src[i], b = dst[i];
+    if (a < 0 || a >= num_pages || b < 0 || b >= num_pages || a == b) continue;
+    uint8_t* base = t.base[k];
+    const int64_t bytes = t.bytes[k];
+    const uint8_t* from = base + a * bytes;
+    uint8_t* to = base + b * bytes;
+    if (((reinterpret_cast<uintptr_t>(base) | (uintptr_t)bytes) & 15) == 0) {
+      constexpr int UN = 4;  // loads in flight before the first store
+      for (int64_t o = 16 * (int64_t)lane; o < bytes; o += 16 * (int64_t)lanes * UN) {
+        u32x4 v[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+          if (o + 16 * lanes * u < bytes) v[u] = ldg128_stream(from + o + 16 * lanes * u);
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+          if (o + 16 * lanes * u < bytes)
+            __builtin_nontemporal_store(v[u], reinterpret_cast<u32x4*>(to + o + 16 * lanes * u));
+      }
+    } else {
+      for (int64_t o = lane; o < bytes; o += lanes) to[o] = from[o];
+    }
   }
 }
 
-// pages src[i] -> dst[i] in every tensor; entries outside [0, num_pages) and
-// pages onto themselves are skipped
-__global__ __launch_bounds__(256) void copy_pages_kernel(PageTensors t, const int32_t* __restrict__ src,
-                                                         const int32_t* __restrict__ dst, int n,
-                                                         int64_t num_pages) {
-  for (int i = blockIdx.x; i < n; i += gridDim.x) {
-    const int64_t a = src[i], b = dst[i];
-    if (a < 0 || a >= num_pages || b < 0 || b >= num_pages || a == b) continue;
-    copy_page(t.base[blockIdx.y], t.bytes[blockIdx.y], a, b);
+// the moves of all arrays, those of pages of one size class in a launch (at
+// most kMaxTensors of them); n: the most pairs that there can be
+int copy_pages(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors, const int32_t* src,
+               const int32_t* dst, const int32_t* count, int64_t n, int64_t num_pages, hipStream_t st) {
+  for (int lgl = 4; lgl <= 8; ++lgl) {
+    int64_t at = 0;
+    while (at < num_tensors) {
+      PageTensors t = {};
+      int k = 0;
+      for (; at < num_tensors && k < kMaxTensors; ++at) {
+        int l = 4;
+        while (l < 8 && (16 << l) < page_bytes[at]) ++l;
+        if (l != lgl || page_bytes[at] == 0) continue;
+        t.base[k] = reinterpret_cast<uint8_t*>(tensors[at]);
+        t.bytes[k++] = page_bytes[at];
+      }
+      if (k == 0) break;
+      const int64_t work = (n + (256 >> lgl) - 1) / (256 >> lgl) * k;
+      // a workgroup for each piece of a known number of pages (64 x 509 pages of
+      // 16 KB: 202 us, 225 with 2048 workgroups going round), else as many as
+      // the CUs hold at a time
+      const int64_t most = count ? 2048 : 1 << 20;
+      copy_pages_kernel<<<(unsigned)(work < most ? work : most), 256, 0, st>>>(t, k, src, dst, count, (int)n, lgl,
+                                                                             num_pages);
+      MK_CHECK_LAUNCH();
+    }
   }
+  return MK_OK;
 }
 
 // ---------------------------------------------------------------------------
@@ -73,9 +124,6 @@ __device__ __forceinline__ int block_scan(int v, int* total, int* lds) {
 __device__ __forceinline__ int load_count(const int32_t* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ void store_count(int32_t* p, int v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 __device__ __forceinline__ void add_count(int32_t* p, int v) {
   __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -84,8 +132,11 @@ __device__ __forceinline__ void add_count(int32_t* p, int v) {
 // fork
 // ---------------------------------------------------------------------------
 
-constexpr int kForkRows = 4096;   // rows of the new table
-constexpr int kForkPerThread = kForkRows / 1024;
+constexpr int kForkRows = 4096;  // rows of the new table
+// What one workgroup does with the counts in LDS: a step of 32 beams over 700
+// pages in 7 us (16.6 with counts in memory, whose atomics and reads go to the
+// L2 one after another).  Beyond, launches over all CUs count the references.
+constexpr int kSmallPages = 8192, kSmallRows = 1024, kSmallNew = 2048, kSmallEntries = 1 << 16;
 
 struct ForkArgs {
   const int32_t* table;    // [B, blocks]
@@ -96,105 +147,113 @@ struct ForkArgs {
   int32_t* new_lengths;    // [n]
   int32_t* new_refs;       // [pages]
   uint8_t* ready;          // [n]
-  int32_t* moves;          // [2, n]: source and destination of each row's copied page, -1 for none
+  int32_t* moves;          // [2, n] + 1: sources and destinations of the copied pages, and their number
   int32_t* ids;            // [max_new]: the pages handed out
   int64_t B, blocks, pages, page_size, reserve, max_new;
   int n;
 };
 
-__device__ __forceinline__ int64_t fork_length(const ForkArgs& a, int r, int64_t* parent) {
-  const int64_t p = a.parents[r];
-  *parent = p;
-  if (p < 0 || p >= a.B) return 0;
-  const int64_t l = a.lengths[p], most = a.blocks * a.page_size;
+// counts and pages handed out: in LDS, or in memory
+template <bool SMALL>
+struct ForkCounts {
+  int32_t* count;
+  int32_t* ids;
+  __device__ __forceinline__ int load(int64_t p) const {
+    if constexpr (SMALL) return count[p];
+    else return load_count(count + p);
+  }
+  __device__ __forceinline__ void add(int64_t p, int v) const {
+    if constexpr (SMALL) atomicAdd(count + p, v);
+    else add_count(count + p, v);
+  }
+};
+
+// the old rows' references off, entries i0, i0 + step, ...
+template <bool SMALL>
+__device__ __forceinline__ void fork_drop(const ForkArgs& a, const ForkCounts<SMALL>& c, int64_t i0, int64_t step) {
+  const int64_t all = a.B * a.blocks;
+  for (int64_t i = i0; i < all; i += step) {
+    const int64_t p = a.table[i];
+    if (p >= 0 && p < a.pages) c.add(p, -1);
+  }
+}
+
+// positions of new row r, and its parent (-1: an empty row)
+__device__ __forceinline__ int fork_length(const ForkArgs& a, int r, int* parent) {
+  const int p = a.parents[r];
+  *parent = p < 0 || p >= a.B ? -1 : p;
+  if (*parent < 0) return 0;
+  const int l = a.lengths[p], most = (int)(a.blocks * a.page_size);  // < 2^31
   return l < 0 ? 0 : (l > most ? most : l);
 }
 
-// counts as they are, then the old rows' references off and the kept ones on
-__device__ __forceinline__ void fork_init(const ForkArgs& a, int64_t i0, int64_t step) {
-  for (int64_t i = i0; i < a.pages; i += step) store_count(a.new_refs + i, a.refs[i]);
-}
-__device__ __forceinline__ void fork_rows(const ForkArgs& a, int64_t i0, int64_t step) {
-  for (int64_t i = i0; i < a.B * a.blocks; i += step) {
-    const int64_t p = a.table[i];
-    if (p >= 0 && p < a.pages) add_count(a.new_refs + p, -1);
-  }
-  for (int64_t i = i0; i < a.n * a.blocks; i += step) {
-    const int r = (int)(i / a.blocks);
-    const int64_t j = i - r * a.blocks;
-    int64_t parent;
-    const int64_t len = fork_length(a, r, &parent);
-    int64_t p = -1;
-    if (j * a.page_size < len) {
-      p = a.table[parent * a.blocks + j];
+// New row r: its length, the kept entries and their references; threads j0,
+// j0 + step, ...  Gives the partly filled last page to the thread that has it.
+template <bool SMALL>
+__device__ __forceinline__ void fork_row(const ForkArgs& a, const ForkCounts<SMALL>& c, int r, int j0, int step,
+                                         int parent, int len, int* last) {
+  const int P = (int)a.page_size, blocks = (int)a.blocks;
+  const int used = (len + P - 1) / P, part = len % P;
+  const int32_t* old = a.table + (int64_t)(parent < 0 ? 0 : parent) * blocks;
+  int32_t* now = a.new_table + (int64_t)r * blocks;
+  for (int j = j0; j < blocks; j += step) {
+    int p = -1;
+    if (j < used) {
+      p = old[j];
       if (p < 0 || p >= a.pages) p = -1;
+      if (p >= 0) c.add(p, 1);
+      if (part && j == used - 1 && last) *last = p;
     }
-    a.new_table[i] = (int32_t)p;
-    if (p >= 0) add_count(a.new_refs + p, 1);
-    if (j == 0) a.new_lengths[r] = (int32_t)len;
+    now[j] = p;
+  }
+  if (j0 == 0) {
+    a.new_lengths[r] = len;
+    if (!part && last) *last = -1;
   }
 }
 
 // New pages for the rows, by one workgroup of 1024 threads.  A partly filled
 // last page stays with the longest of its rows (the first of those) if nobody
-// else holds it; every other row gets a copy.  Row r of thread t is
+// else holds it; every other row gets a copy.  Row k of thread t is
 // t * per + k, so that a thread's rows and the threads are in order.
-__device__ void fork_allot(const ForkArgs& a, int* scan) {
-  __shared__ int last[kForkRows];           // partly filled last page, -1 for none
-  __shared__ int key[kForkRows];            // values in it
+template <bool SMALL, int PER>
+__device__ void fork_allot(const ForkArgs& a, const ForkCounts<SMALL>& c, const int* last, const int* lens,
+                           const int* parents, int* scan) {
   const int tid = threadIdx.x;
   const int per = (a.n + 1023) / 1024;
-  const int64_t P = a.page_size;
-  int64_t len[kForkPerThread];
-  int need[kForkPerThread];
-  bool copies[kForkPerThread], fits[kForkPerThread];
+  const int P = (int)a.page_size, blocks = (int)a.blocks;
+  int need[PER];
+  bool copies[PER], fits[PER];
+  int mine = 0;
 #pragma unroll
-  for (int k = 0; k < kForkPerThread; ++k) {
+  for (int k = 0; k < PER; ++k) {
     const int r = tid * per + k;
-    len[k] = 0;
     need[k] = 0;
     copies[k] = false;
     fits[k] = true;
     if (k >= per || r >= a.n) continue;
-    int64_t parent;
-    len[k] = fork_length(a, r, &parent);
-    const int part = (int)(len[k] % P);
-    int64_t page = -1;
-    if (part) {
-      page = a.table[parent * a.blocks + len[k] / P];
-      if (page < 0 || page >= a.pages) page = -1;
-    }
-    last[r] = (int)page;
-    key[r] = part;
-    a.moves[r] = a.moves[a.n + r] = -1;
-    fits[k] = parent < 0 || parent >= a.B || len[k] + a.reserve <= a.blocks * P;
-    need[k] = parent < 0 || parent >= a.B || !fits[k]
-                  ? 0 : (int)((len[k] + a.reserve + P - 1) / P - (len[k] + P - 1) / P);
-  }
-  __syncthreads();
-  int mine = 0;
-#pragma unroll
-  for (int k = 0; k < kForkPerThread; ++k) {
-    const int r = tid * per + k;
-    if (k >= per || r >= a.n) continue;
-    const int page = last[r];
-    int64_t parent = a.parents[r];
-    if (page >= 0 && fits[k] && parent >= 0 && parent < a.B) {
+    if (parents[r] < 0) continue;
+    const int len = lens[r], page = last[r], part = len % P;
+    const int64_t end = len + a.reserve;
+    fits[k] = end <= (int64_t)blocks * P;
+    if (!fits[k]) continue;
+    need[k] = (int)((end + P - 1) / P) - (len + P - 1) / P;
+    if (page >= 0) {
       int same = 0;
       bool best = true;
       for (int o = 0; o < a.n; ++o) {
         const bool s = last[o] == page;
+        const int other = s ? lens[o] % P : 0;
         same += s;
-        best &= !s || key[o] < key[r] || (key[o] == key[r] && o >= r);
+        best &= !s || other < part || (other == part && o >= r);
       }
-      copies[k] = !(best && load_count(a.new_refs + page) == same);
+      copies[k] = !(best && c.load(page) == same);
       need[k] += copies[k];
     }
     mine += need[k];
   }
   int wanted;
   int off = block_scan(mine, &wanted, scan);
-  __syncthreads();
   // ids of the first free pages; stops where there are enough
   int found = 0;
   for (int64_t base = 0; base < a.pages && found < wanted; base += 8 * 1024) {
@@ -202,7 +261,7 @@ __device__ void fork_allot(const ForkArgs& a, int* scan) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int64_t i = base + 8 * tid + e;
-      const bool f = i < a.pages && load_count(a.new_refs + i) == 0;
+      const bool f = i < a.pages && c.load(i) == 0;
       ok |= (int)f << e;
       cnt += f;
     }
@@ -211,14 +270,26 @@ __device__ void fork_allot(const ForkArgs& a, int* scan) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if ((ok >> e) & 1) {
-        if (at < wanted && at < a.max_new) a.ids[at] = (int32_t)(base + 8 * tid + e);
+        if (at < wanted && at < a.max_new) c.ids[at] = (int32_t)(base + 8 * tid + e);
         ++at;
       }
     found += total;
   }
   __syncthreads();  // ids are written, counts are read
+  int moved = 0, moves;
+  {
+    int o = off;
 #pragma unroll
-  for (int k = 0; k < kForkPerThread; ++k) {
+    for (int k = 0; k < PER; ++k) {
+      copies[k] = copies[k] && o + need[k] <= found;
+      moved += copies[k];
+      o += need[k];
+    }
+  }
+  moved = block_scan(moved, &moves, scan);
+  if (tid == 0) a.moves[2 * a.n] = moves;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
     const int r = tid * per + k;
     if (k >= per || r >= a.n) continue;
     const bool got = fits[k] && (need[k] == 0 || off + need[k] <= found);
@@ -226,33 +297,71 @@ __device__ void fork_allot(const ForkArgs& a, int* scan) {
     if (got && need[k] > 0) {
       int i = off;
       const int end = off + need[k];
-      int64_t j = (len[k] + P - 1) / P;
+      int j = (lens[r] + P - 1) / P;
       if (copies[k]) {
-        a.moves[r] = last[r];
-        a.moves[a.n + r] = a.ids[i];
-        add_count(a.new_refs + last[r], -1);
+        a.moves[moved] = last[r];
+        a.moves[a.n + moved++] = c.ids[i];
+        c.add(last[r], -1);
         --j;
       }
       for (; i < end; ++i, ++j) {
-        a.new_table[(int64_t)r * a.blocks + j] = a.ids[i];
-        add_count(a.new_refs + a.ids[i], 1);
+        a.new_table[(int64_t)r * blocks + j] = c.ids[i];
+        c.add(c.ids[i], 1);
       }
     }
     off += need[k];
   }
 }
 
-__global__ __launch_bounds__(1024) void fork_kernel(ForkArgs a) {
-  __shared__ int scan[16];
-  fork_init(a, threadIdx.x, 1024);
+__global__ __launch_bounds__(1024) void fork_small_kernel(ForkArgs a) {
+  __shared__ int32_t count[kSmallPages], ids[kSmallNew];
+  __shared__ int last[kSmallRows], lens[kSmallRows], parents[kSmallRows], scan[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const ForkCounts<true> c = {count, ids};
+  for (int i = tid; i < (int)a.pages; i += 1024) count[i] = a.refs[i];
+  for (int r = tid; r < a.n; r += 1024) lens[r] = fork_length(a, r, &parents[r]);
   __syncthreads();
-  fork_rows(a, threadIdx.x, 1024);
+  fork_drop(a, c, tid, 1024);
+  for (int r = wave; r < a.n; r += 16) fork_row(a, c, r, lane, MK_WAVE, parents[r], lens[r], &last[r]);
   __syncthreads();
   if (a.reserve > 0) {
-    fork_allot(a, scan);
+    fork_allot<true, 1>(a, c, last, lens, parents, scan);
   } else {
-    for (int r = threadIdx.x; r < a.n; r += 1024) a.ready[r] = 1;
+    for (int r = tid; r < a.n; r += 1024) a.ready[r] = 1;
   }
+  __syncthreads();
+  for (int i = tid; i < (int)a.pages; i += 1024) a.new_refs[i] = count[i];
+}
+
+__global__ __launch_bounds__(256) void fork_init_kernel(ForkArgs a) {
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < a.pages; i += gridDim.x * 256ll) a.new_refs[i] = a.refs[i];
+}
+
+// workgroup r < n: new row r; the others: the old table
+__global__ __launch_bounds__(256) void fork_rows_kernel(ForkArgs a) {
+  const ForkCounts<false> c = {a.new_refs, nullptr};
+  const int r = blockIdx.x;
+  if (r < a.n) {
+    int parent;
+    const int len = fork_length(a, r, &parent);
+    fork_row(a, c, r, threadIdx.x, 256, parent, len, nullptr);
+    if (threadIdx.x == 0 && a.reserve == 0) a.ready[r] = 1;
+  } else {
+    fork_drop(a, c, (r - a.n) * 256ll + threadIdx.x, (gridDim.x - a.n) * 256ll);
+  }
+}
+
+__global__ __launch_bounds__(1024) void fork_allot_kernel(ForkArgs a) {
+  __shared__ int last[kForkRows], lens[kForkRows], parents[kForkRows], scan[16];
+  const ForkCounts<false> c = {a.new_refs, a.ids};
+  for (int r = threadIdx.x; r < a.n; r += 1024) {
+    lens[r] = fork_length(a, r, &parents[r]);
+    int p = -1;
+    if (lens[r] % a.page_size) p = a.new_table[(int64_t)r * a.blocks + lens[r] / a.page_size];
+    last[r] = p;
+  }
+  __syncthreads();
+  fork_allot<false, kForkRows / 1024>(a, c, last, lens, parents, scan);
 }
 
 // ---------------------------------------------------------------------------
@@ -319,22 +428,6 @@ __global__ __launch_bounds__(1024) void compact_kernel(CompactArgs a) {
   }
 }
 
-__global__ __launch_bounds__(256) void copy_compacted_kernel(PageTensors t, const int32_t* __restrict__ list,
-                                                             const int32_t* __restrict__ counts) {
-  const int m = counts[1];
-  for (int i = blockIdx.x; i < m; i += gridDim.x)
-    copy_page(t.base[blockIdx.y], t.bytes[blockIdx.y], list[m + i], list[i]);
-}
-
-inline PageTensors page_tensors(void* const* tensors, const int64_t* bytes, int k) {
-  PageTensors t;
-  for (int i = 0; i < kMaxTensors; ++i) {
-    t.base[i] = i < k ? reinterpret_cast<uint8_t*>(tensors[i]) : nullptr;
-    t.bytes[i] = i < k ? bytes[i] : 0;
-  }
-  return t;
-}
-
 }  // namespace
 
 extern "C" {
@@ -346,15 +439,8 @@ int mk_copy_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t nu
   MK_REQUIRE(n == 0 || (src && dst));
   for (int64_t i = 0; i < num_tensors; ++i) MK_REQUIRE(tensors[i] && page_bytes[i] >= 0);
   if (n == 0) return MK_OK;
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  for (int64_t at = 0; at < num_tensors; at += kMaxTensors) {
-    const int k = (int)(num_tensors - at < kMaxTensors ? num_tensors - at : kMaxTensors);
-    const PageTensors t = page_tensors(tensors + at, page_bytes + at, k);
-    copy_pages_kernel<<<dim3((unsigned)(n < 65536 ? n : 65536), (unsigned)k), 256, 0, st>>>(t, src, dst, (int)n,
-                                                                                          num_pages);
-    MK_CHECK_LAUNCH();
-  }
-  return MK_OK;
+  return copy_pages(tensors, page_bytes, num_tensors, src, dst, nullptr, n, num_pages,
+                    reinterpret_cast<hipStream_t>(stream));
 }
 
 int mk_fork_kv_sequences(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors,
@@ -364,22 +450,31 @@ int mk_fork_kv_sequences(void* const* tensors, const int64_t* page_bytes, int64_
                          int64_t max_blocks, int64_t page_size, int64_t num_pages, int64_t reserve, void* stream) {
   MK_REQUIRE(B >= 0 && n >= 0 && n <= kForkRows && max_blocks > 0 && page_size > 0 && num_pages > 0 && reserve >= 0);
   MK_REQUIRE(max_blocks < (1LL << 31) && page_size < (1LL << 31) && num_pages < (1LL << 31) && reserve < (1LL << 31));
-  MK_REQUIRE(max_blocks * page_size < (1LL << 31) && n * (max_blocks + 1) < (1LL << 31) && B < (1LL << 31));
+  MK_REQUIRE((max_blocks + 1) * page_size < (1LL << 31) && n * (max_blocks + 1) < (1LL << 31) && B < (1LL << 31));
+  MK_REQUIRE(B * max_blocks < (1LL << 40));
   MK_REQUIRE(ref_counts && new_ref_counts && (B == 0 || (block_table && lengths)));
   MK_REQUIRE(n == 0 || (parents && new_table && new_lengths && ready));
   const int64_t most = n * (1 + (reserve + page_size - 1) / page_size);  // pages that the rows can need
   const int64_t max_new = reserve == 0 ? 0 : (most < num_pages ? most : num_pages);
-  MK_REQUIRE(reserve == 0 || n == 0 || (workspace && workspace_ints >= 2 * n + max_new));
+  MK_REQUIRE(reserve == 0 || n == 0 || (workspace && workspace_ints >= 2 * n + 1 + max_new));
   MK_REQUIRE(num_tensors >= 0 && (num_tensors == 0 || (tensors && page_bytes)));
   for (int64_t i = 0; i < num_tensors; ++i) MK_REQUIRE(tensors[i] && page_bytes[i] >= 0);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const ForkArgs a = {block_table, lengths, ref_counts, parents, new_table, new_lengths, new_ref_counts, ready,
-                      workspace, workspace ? workspace + 2 * n : nullptr, B, max_blocks, num_pages, page_size, reserve,
+                      workspace, workspace ? workspace + 2 * n + 1 : nullptr, B, max_blocks, num_pages, page_size, reserve,
                       max_new, (int)n};
-  fork_kernel<<<1, 1024, 0, st>>>(a);
+  if (num_pages <= kSmallPages && n <= kSmallRows && max_new <= kSmallNew && (B + n) * max_blocks <= kSmallEntries) {
+    fork_small_kernel<<<1, 1024, 0, st>>>(a);
+  } else {
+    const int64_t init = (num_pages + 255) / 256;
+    fork_init_kernel<<<(unsigned)(init < 1024 ? init : 1024), 256, 0, st>>>(a);
+    const int64_t drop = (B * max_blocks + 255) / 256;
+    if (n + drop > 0) fork_rows_kernel<<<(unsigned)(n + (drop < 1024 ? drop : 1024)), 256, 0, st>>>(a);
+    if (reserve > 0 && n > 0) fork_allot_kernel<<<1, 1024, 0, st>>>(a);
+  }
   MK_CHECK_LAUNCH();
   if (reserve == 0 || n == 0) return MK_OK;
-  return mk_copy_kv_pages(tensors, page_bytes, num_tensors, workspace, workspace + n, n, num_pages, stream);
+  return copy_pages(tensors, page_bytes, num_tensors, workspace, workspace + n, workspace + 2 * n, n, num_pages, st);
 }
 
 int mk_compact_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors,
@@ -395,15 +490,10 @@ int mk_compact_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t
                          num_pages};
   compact_kernel<<<1, 1024, 0, st>>>(a);
   MK_CHECK_LAUNCH();
-  for (int64_t at = 0; at < num_tensors && num_pages > 1; at += kMaxTensors) {
-    const int k = (int)(num_tensors - at < kMaxTensors ? num_tensors - at : kMaxTensors);
-    const PageTensors t = page_tensors(tensors + at, page_bytes + at, k);
-    const int64_t most = num_pages / 2;  // moved pages: no more than free ones, and no more than live ones
-    copy_compacted_kernel<<<dim3((unsigned)(most < 1024 ? most : 1024), (unsigned)k), 256, 0, st>>>(t, workspace,
-                                                                                                  counts);
-    MK_CHECK_LAUNCH();
-  }
-  return MK_OK;
+  // no more pages move than are free, and than are live
+  return num_pages > 1 ? copy_pages(tensors, page_bytes, num_tensors, nullptr, workspace, counts + 1, num_pages / 2,
+                                    num_pages, st)
+                       : MK_OK;
 }
 
 }  // extern "C"

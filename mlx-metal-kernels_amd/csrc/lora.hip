@@ -513,9 +513,9 @@ inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t ad
   // more of them, and fewer workgroups fill the CUs less.  256 against 512
   // outputs (us a call): 512 rows x 6144, rank 16 (192 workgroups of 256):
   // 21.4 / 24.0; 2000 rows x 8192, rank 128 (1024): 74.5 / 62.8; 4093 rows x
-  // 14336, rank 64 (3584): 90.3 / 89.7, and 90.7 with 1024.
+  // 14336, rank 64 (3584): 90.3 / 89.7 (and 90.7 with 1024).
   const int64_t work = (N + 255) / 256 * full;
-  p.blocks = work >= 8192 ? 4 : work >= 1024 ? 2 : 1;
+  p.blocks = work >= 1024 ? 2 : 1;
   return p;
 }
 

@@ -86,8 +86,8 @@ def count_page_refs(block_table, num_pages: int):
 
 
 def copy_kv_pages(pages, src, dst, *, backend: str = "auto"):
-    """Page src[i] onto page dst[i] in every array of ``pages``, in place, in
-    one launch per 128 arrays; returns ``pages``.  src, dst int32 [n] (device,
+    """Page src[i] onto page dst[i] in every array of ``pages``, in place;
+    returns ``pages``.  src, dst int32 [n] (device,
     host or a list).  No page may be the destination of two pairs, or the
     source of one and the destination of another.  Entries are checked on the
     host unless that is off (``host_checks_enabled``); then pairs with an entry
@@ -193,7 +193,7 @@ def fork_kv_sequences(pages, block_table, lengths, ref_counts, parents, *, reser
     if parents.dim() != 1 or parents.shape[0] > MAX_ROWS:
         raise ValueError(f"parents must be [n] with n <= {MAX_ROWS}, got {tuple(parents.shape)}")
     n = parents.shape[0]
-    if blocks * size >= 2 ** 31 or n * (blocks + 1) >= 2 ** 31:
+    if (blocks + 1) * size >= 2 ** 31 or n * (blocks + 1) >= 2 ** 31:
         raise ValueError(f"a row's positions and a table's entries must fit 31 bits, got {n} rows of {blocks} x {size}")
     if host_checks_enabled(block_table):
         _check_counts(block_table, ref_counts)
@@ -209,7 +209,7 @@ def fork_kv_sequences(pages, block_table, lengths, ref_counts, parents, *, reser
     new_table = torch.empty((n, blocks), dtype=torch.int32, device=dev)
     new_refs = torch.empty_like(refs)
     ready = torch.empty(n, dtype=torch.bool, device=dev)
-    ints = 2 * n + min(num_pages, n * (1 + -(-reserve // size))) if reserve else 0
+    ints = 2 * n + 1 + min(num_pages, n * (1 + -(-reserve // size))) if reserve else 0
     buf = torch.empty(n + ints, dtype=torch.int32, device=dev)  # the new lengths, then the workspace
     at, sizes = _addresses(pages, num_pages)
     base = buf.data_ptr()
