@@ -192,9 +192,10 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(const int32_t* __restr
 
 constexpr int kShrinkWaves = 8;
 
-template <typename T, int RT, int MT, bool VEC>
-__device__ __forceinline__ void shrink_group(const T* x, int64_t x_stride, const T* ai, float* t, int64_t K, int R,
-                                             int64_t k0, int64_t k1, int rowlist, f32x4 (&part)[kShrinkWaves][RT][64]) {
+// put(i, row, r, s): ranks r .. r + 3 of the group's row number i
+template <typename T, int RT, int MT, bool VEC, typename Put>
+__device__ __forceinline__ void shrink_rows(const T* x, int64_t x_stride, const T* ai, int64_t K, int R, int64_t k0,
+                                            int64_t k1, int rowlist, f32x4 (&part)[kShrinkWaves][RT][64], Put put) {
   constexpr int UN = !VEC || RT * MT > 8 ? 1 : RT * MT > 2 ? 2 : 4;  // turns whose loads are in flight together
   constexpr bool AHEAD = VEC && RT * MT <= 16;  // (more would not fit the registers)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -263,7 +264,25 @@ __device__ __forceinline__ void shrink_group(const T* x, int64_t x_stride, const
       f32x4 s = part[0][q][lane];
 #pragma unroll
       for (int w = 1; w < kShrinkWaves; ++w) s += part[w][q][lane];
-      if (row[i] >= 0) *reinterpret_cast<f32x4*>(t + (int64_t)row[i] * (16 * RT) + 16 * q + 4 * grp) = s;
+      put(16 * i + col, row[i], 16 * q + 4 * grp, s);
+    }
+  }
+}
+
+template <typename T, int RT, bool VEC, typename Put>
+__device__ __forceinline__ void shrink_group(const T* x, int64_t x_stride, const T* ai, int64_t K, int R, int64_t k0,
+                                             int64_t k1, int n, int rowlist, f32x4 (&part)[kShrinkWaves][RT][64],
+                                             Put put) {
+  if constexpr (VEC) {
+    if (n <= 16) shrink_rows<T, RT, 1, VEC>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
+    else shrink_rows<T, RT, 4, VEC>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
+  } else {  // values one by one: 16 rows at a time leave the registers for them
+    for (int i = 0; i < n; i += 16) {
+      const int at = ((int)threadIdx.x & 63) + i;
+      const int row = __shfl(rowlist, at & 63, MK_WAVE);
+      if (i) __syncthreads();  // the last rows' sums are read
+      shrink_rows<T, RT, 1, VEC>(x, x_stride, ai, K, R, k0, k1, at < 64 ? row : -1, part,
+                                 [&](int j, int m, int r, const f32x4& s) { put(i + j, m, r, s); });
     }
   }
 }
@@ -281,17 +300,10 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(Groups g
   const int64_t k1 = k0 + k_slice < K ? k0 + k_slice : K;
   const T* ai = a + (int64_t)adapter * R * K;
   t += (int64_t)blockIdx.y * gs.M * (16 * RT);
-  if constexpr (VEC) {
-    if (n <= 16) shrink_group<T, RT, 1, VEC>(x, x_stride, ai, t, K, R, k0, k1, rowlist, part);
-    else shrink_group<T, RT, 4, VEC>(x, x_stride, ai, t, K, R, k0, k1, rowlist, part);
-  } else {  // values one by one: 16 rows at a time leave the registers for them
-    for (int i = 0; i < n; i += 16) {
-      const int at = ((int)threadIdx.x & 63) + i;
-      const int row = __shfl(rowlist, at & 63, MK_WAVE);
-      if (i) __syncthreads();  // the last rows' sums are read
-      shrink_group<T, RT, 1, VEC>(x, x_stride, ai, t, K, R, k0, k1, at < 64 ? row : -1, part);
-    }
-  }
+  shrink_group<T, RT, VEC>(x, x_stride, ai, K, R, k0, k1, n, rowlist, part,
+                           [&](int, int m, int r, const f32x4& s) {
+                             if (m >= 0) *reinterpret_cast<f32x4*>(t + (int64_t)m * (16 * RT) + r) = s;
+                           });
 }
 
 // ---------------------------------------------------------------------------
@@ -305,199 +317,308 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(Groups g
 // 57 us, in these 47.
 // ---------------------------------------------------------------------------
 
-template <typename T, int RT, bool VEC>
-__global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* base, int64_t base_stride,
-                                                          const T* __restrict__ b, const float* __restrict__ scales,
-                                                          const float* __restrict__ t, T* out, int64_t out_stride,
-                                                          int64_t N, int R, int slices, int blocks, bool wide) {
+template <typename T, int RT>
+struct ExpandRows {
   typedef typename Frag<T>::v8 v8;
-  constexpr int RP = 16 * RT;               // ranks, whole tiles
-  constexpr int KS = RT == 1 ? 1 : RT / 2;  // up to 16 ranks: both parts in one instruction, over B twice
-  constexpr int CH = RP / 8;                // chunks of 8 ranks
-  constexpr int STRIDE = 2 * RP + 8;        // of a row in LDS: both parts, and 16 bytes that spread the rows over the banks
-  __shared__ T parts[kGroupRows][STRIDE];
-  __shared__ f32x4 backs[kGroupRows / 4];
-  __shared__ int64_t at_base[kGroupRows], at_out[kGroupRows];  // where the rows begin: products of 64 bits are slow
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = lane & 15, grp = lane >> 4;
-  int adapter, rowlist;
-  const int n = find_group(gs, (int)blockIdx.y, &adapter, &rowlist);
-  if (n == 0 || (adapter < 0 && base == out)) return;
-  if (wave == 0) {
-    at_base[lane] = rowlist * base_stride;
-    at_out[lane] = rowlist * out_stride;
-  }
-  if (adapter < 0) {  // rows without an adapter
-    const int64_t c0 = (int64_t)blockIdx.x * blocks * 256, c1 = c0 + 256 * blocks < N ? c0 + 256 * blocks : N;
-    for (int i = 0; i < n; ++i) {
-      const int64_t m = __builtin_amdgcn_readlane(rowlist, i);
-      const T* br = base + m * base_stride;
-      T* orow = out + m * out_stride;
-      if (wide) {
-        for (int64_t c = c0 + 4 * (int)threadIdx.x; c < c1; c += 4 * 256)
-          *reinterpret_cast<u32x2*>(orow + c) = ldg64(br + c);
-      } else {
-        for (int64_t c = c0 + (int)threadIdx.x; c < c1; c += 256) orow[c] = br[c];
-      }
+  static constexpr int RP = 16 * RT;               // ranks, whole tiles
+  static constexpr int KS = RT == 1 ? 1 : RT / 2;  // up to 16 ranks: both parts in one instruction, over B twice
+  static constexpr int CH = RP / 8;                // chunks of 8 ranks
+  T parts[kGroupRows][2 * RP + 8];                 // both parts of t; 16 bytes that spread the rows over the banks
+  f32x4 backs[kGroupRows / 4];
+  int64_t at_base[kGroupRows], at_out[kGroupRows];  // where the rows begin: products of 64 bits are slow
+
+  // chunk c of row i, by CH lanes side by side, a power of two
+  __device__ __forceinline__ void put(int i, int c, float (&v)[8], float back, bool live) {
+    if constexpr (__is_same(T, f16)) {  // the row's largest value to [2^13, 2^14)
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+#pragma unroll
+      for (int o = 1; o < CH; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, MK_WAVE));
+      int e = 14;
+      if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = ldexpf(v[q], 14 - e);
+      back = ldexpf(back, e - 14);
     }
-    return;
+    v8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      hi[e] = from_f32<T>(v[e]);
+      const float left = v[e] - to_f32(hi[e]);
+      lo[e] = from_f32<T>(fabsf(v[e]) < INFINITY ? left : 0.0f);
+    }
+    if (!live) return;
+    *reinterpret_cast<v8*>(&parts[i][8 * c]) = hi;
+    *reinterpret_cast<v8*>(&parts[i][RP + 8 * c]) = lo;
+    if (c == 0) reinterpret_cast<float*>(backs)[i] = back;
   }
-  const T* bi = b + (int64_t)adapter * N * R;
-  v8 bf[4][KS];
-  auto load_b = [&](int64_t n0) {
+};
+
+// B's fragments of 64 outputs from n0 on
+template <typename T, int RT, bool VEC>
+__device__ __forceinline__ void load_b(const T* bi, int64_t n0, int64_t N, int R,
+                                       typename Frag<T>::v8 (&bf)[4][ExpandRows<T, RT>::KS]) {
+  const int col = threadIdx.x & 15, grp = (threadIdx.x & 63) >> 4;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = n0 + 4 * col + j;
+  for (int j = 0; j < 4; ++j) {
+    const int64_t r = n0 + 4 * col + j;
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-        bf[j][s] = load_frag<T, VEC>(bi + (r < N ? r : N - 1) * R, RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp, R);
+    for (int s = 0; s < ExpandRows<T, RT>::KS; ++s)
+      bf[j][s] = load_frag<T, VEC>(bi + (r < N ? r : N - 1) * R, RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp, R);
+  }
+}
+
+// rows without an adapter: outputs c0 .. c1 of them copied
+template <typename T>
+__device__ __forceinline__ void copy_rows(const T* base, int64_t base_stride, T* out, int64_t out_stride, int64_t c0,
+                                          int64_t c1, int n, int rowlist, bool wide) {
+  for (int i = 0; i < n; ++i) {
+    const int64_t m = __builtin_amdgcn_readlane(rowlist, i);
+    const T* br = base + m * base_stride;
+    T* orow = out + m * out_stride;
+    if (wide) {
+      for (int64_t c = c0 + 4 * (int)threadIdx.x; c < c1; c += 4 * (int)blockDim.x)
+        *reinterpret_cast<u32x2*>(orow + c) = ldg64(br + c);
+    } else {
+      for (int64_t c = c0 + (int)threadIdx.x; c < c1; c += (int)blockDim.x) orow[c] = br[c];
+    }
+  }
+}
+
+// 64 outputs from n0 on of a group's n rows, by a wave
+template <typename T, int RT>
+__device__ __forceinline__ void expand_rows(const ExpandRows<T, RT>& l, const T* base, T* out, int64_t N, int64_t n0,
+                                            int n, bool wide,
+                                            const typename Frag<T>::v8 (&bf)[4][ExpandRows<T, RT>::KS]) {
+  typedef ExpandRows<T, RT> L;
+  typedef typename L::v8 v8;
+  const int col = threadIdx.x & 15, grp = (threadIdx.x & 63) >> 4;
+  const int64_t nn = n0 + 4 * col;  // this lane's first output
+  auto product = [&](int rt, f32x4 (&acc)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const T* pr = l.parts[16 * rt + col];
+#pragma unroll
+    for (int s = 0; s < L::KS; ++s) {
+      if constexpr (RT == 1) {  // chunks 0 and 1 of the first part, then of the second
+        const v8 both = *reinterpret_cast<const v8*>(pr + 8 * grp);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(both, bf[j][s], acc[j]);
+      } else {
+        const v8 hi = *reinterpret_cast<const v8*>(pr + 32 * s + 8 * grp);
+        const v8 lo = *reinterpret_cast<const v8*>(pr + L::RP + 32 * s + 8 * grp);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(hi, bf[j][s], acc[j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(lo, bf[j][s], acc[j]);
+      }
     }
   };
-  int64_t n0 = ((int64_t)blockIdx.x * blocks * 4 + wave) * 64;
-  load_b(n0);  // on the way while t is joined
-  {
-    const float scale = scales ? scales[adapter] : 1.0f;
-    const int chunks = ((n + 15) & ~15) * CH;  // CH lanes a row, a power of two
-    for (int at0 = 0; at0 < chunks; at0 += 256) {
-      const int at = at0 + (int)threadIdx.x, i = at / CH, c = at % CH;
-      const int row = __shfl(rowlist, i & 63, MK_WAVE);  // (every lane: the source has to be active)
-      const int m = at < chunks ? row : -1;
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (m >= 0) {
-        const float* tr = t + (int64_t)m * RP + 8 * c;
-        for (int z = 0; z < slices; ++z, tr += gs.M * RP) {
-          const f32x4 lo = *reinterpret_cast<const f32x4*>(tr), hi = *reinterpret_cast<const f32x4*>(tr + 4);
+  const T* bn = base + nn;
+  T* on = out + nn;
+  int rt = 0;
+  if (wide && n0 + 64 <= N && n >= 16) {
+    // whole tiles, without a branch: base of the next 16 rows is on its way while these are computed
+    const int whole = n / 16;
+    u32x2 w[4], next[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] += lo[e];
-            v[4 + e] += hi[e];
-          }
-        }
-      }
-      float back = scale;
-      if constexpr (__is_same(T, f16)) {  // the row's largest value to [2^13, 2^14)
-        float top = 0.0f;
+    for (int i = 0; i < 4; ++i) w[i] = ldg64(bn + l.at_base[4 * grp + i]);
+    for (; rt < whole; ++rt) {
+      const int then = 16 * (rt + 1 < whole ? rt + 1 : rt) + 4 * grp;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
-#pragma unroll
-        for (int o = 1; o < CH; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, MK_WAVE));
-        int e = 14;
-        if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = ldexpf(v[q], 14 - e);
-        back = ldexpf(back, e - 14);
-      }
-      v8 hi, lo;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        hi[e] = from_f32<T>(v[e]);
-        const float left = v[e] - to_f32(hi[e]);
-        lo[e] = from_f32<T>(fabsf(v[e]) < INFINITY ? left : 0.0f);
-      }
-      if (at >= chunks) continue;
-      *reinterpret_cast<v8*>(&parts[i][8 * c]) = hi;
-      *reinterpret_cast<v8*>(&parts[i][RP + 8 * c]) = lo;
-      if (c == 0) reinterpret_cast<float*>(backs)[i] = back;
-    }
-  }
-  lds_barrier();  // (the loads of B stay in flight)
-  for (int blk = 0; blk < blocks; ++blk, n0 += 256) {
-    if (n0 >= N) return;
-    if (blk) load_b(n0);
-    const int64_t nn = n0 + 4 * col;  // this lane's first output
-    auto product = [&](int rt, f32x4 (&acc)[4]) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const T* pr = parts[16 * rt + col];
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        if constexpr (RT == 1) {  // chunks 0 and 1 of the first part, then of the second
-          const v8 both = *reinterpret_cast<const v8*>(pr + 8 * grp);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(both, bf[j][s], acc[j]);
-        } else {
-          const v8 hi = *reinterpret_cast<const v8*>(pr + 32 * s + 8 * grp);
-          const v8 lo = *reinterpret_cast<const v8*>(pr + RP + 32 * s + 8 * grp);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(hi, bf[j][s], acc[j]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = Frag<T>::mfma(lo, bf[j][s], acc[j]);
-        }
-      }
-    };
-    const T* bn = base + nn;
-    T* on = out + nn;
-    int rt = 0;
-    if (wide && n0 + 64 <= N && n >= 16) {
-      // whole tiles, without a branch: base of the next 16 rows is on its way while these are computed
-      const int whole = n / 16;
-      u32x2 w[4], next[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = ldg64(bn + at_base[4 * grp + i]);
-      for (; rt < whole; ++rt) {
-        const int then = 16 * (rt + 1 < whole ? rt + 1 : rt) + 4 * grp;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) next[i] = ldg64(bn + at_base[then + i]);
-        f32x4 acc[4];
-        product(rt, acc);
-        const f32x4 back = backs[4 * rt + grp];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          u32x2 o;
-#pragma unroll
-          for (int j = 0; j < 4; j += 2)
-            o[j >> 1] = pack2<T>(fmaf(acc[j][i], back[i], to_f32(bitcast<T>((uint16_t)w[i][j >> 1]))),
-                                 fmaf(acc[j + 1][i], back[i], to_f32(bitcast<T>((uint16_t)(w[i][j >> 1] >> 16)))));
-          *reinterpret_cast<u32x2*>(on + at_out[16 * rt + 4 * grp + i]) = o;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = next[i];
-      }
-    }
-    for (; 16 * rt < n; ++rt) {
-      u32x2 w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * rt + 4 * grp + i;
-        if (wide) w[i] = ldg64(base + at_base[r < n ? r : 0] + (nn < N ? nn : 0));
-      }
+      for (int i = 0; i < 4; ++i) next[i] = ldg64(bn + l.at_base[then + i]);
       f32x4 acc[4];
       product(rt, acc);
-      const f32x4 back = backs[4 * rt + grp];
+      const f32x4 back = l.backs[4 * rt + grp];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = 16 * rt + 4 * grp + i;
-        if (r >= n) continue;
-        T* orow = on + at_out[r];
-        if (wide) {  // whole 8-byte chunks
-          if (nn >= N) continue;
-          u32x2 o;
+        u32x2 o;
 #pragma unroll
-          for (int j = 0; j < 4; j += 2)
-            o[j >> 1] = pack2<T>(fmaf(acc[j][i], back[i], to_f32(bitcast<T>((uint16_t)w[i][j >> 1]))),
-                                 fmaf(acc[j + 1][i], back[i], to_f32(bitcast<T>((uint16_t)(w[i][j >> 1] >> 16)))));
-          *reinterpret_cast<u32x2*>(orow) = o;
-        } else {
+        for (int j = 0; j < 4; j += 2)
+          o[j >> 1] = pack2<T>(fmaf(acc[j][i], back[i], to_f32(bitcast<T>((uint16_t)w[i][j >> 1]))),
+                               fmaf(acc[j + 1][i], back[i], to_f32(bitcast<T>((uint16_t)(w[i][j >> 1] >> 16)))));
+        *reinterpret_cast<u32x2*>(on + l.at_out[16 * rt + 4 * grp + i]) = o;
+      }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const T* br = bn + at_base[r];
-            if (nn + j < N) orow[j] = from_f32<T>(fmaf(acc[j][i], back[i], to_f32(br[j])));
-          }
+      for (int i = 0; i < 4; ++i) w[i] = next[i];
+    }
+  }
+  for (; 16 * rt < n; ++rt) {
+    u32x2 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * rt + 4 * grp + i;
+      if (wide) w[i] = ldg64(base + l.at_base[r < n ? r : 0] + (nn < N ? nn : 0));
+    }
+    f32x4 acc[4];
+    product(rt, acc);
+    const f32x4 back = l.backs[4 * rt + grp];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * rt + 4 * grp + i;
+      if (r >= n) continue;
+      T* orow = on + l.at_out[r];
+      if (wide) {  // whole 8-byte chunks
+        if (nn >= N) continue;
+        u32x2 o;
+#pragma unroll
+        for (int j = 0; j < 4; j += 2)
+          o[j >> 1] = pack2<T>(fmaf(acc[j][i], back[i], to_f32(bitcast<T>((uint16_t)w[i][j >> 1]))),
+                               fmaf(acc[j + 1][i], back[i], to_f32(bitcast<T>((uint16_t)(w[i][j >> 1] >> 16)))));
+        *reinterpret_cast<u32x2*>(orow) = o;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const T* br = bn + l.at_base[r];
+          if (nn + j < N) orow[j] = from_f32<T>(fmaf(acc[j][i], back[i], to_f32(br[j])));
         }
       }
     }
   }
 }
 
+template <typename T, int RT, bool VEC>
+__global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* base, int64_t base_stride,
+                                                          const T* __restrict__ b, const float* __restrict__ scales,
+                                                          const float* __restrict__ t, T* out, int64_t out_stride,
+                                                          int64_t N, int R, int slices, int blocks, bool wide) {
+  typedef ExpandRows<T, RT> L;
+  __shared__ L l;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int adapter, rowlist;
+  const int n = find_group(gs, (int)blockIdx.y, &adapter, &rowlist);
+  if (n == 0 || (adapter < 0 && base == out)) return;
+  if (adapter < 0) {
+    const int64_t c0 = (int64_t)blockIdx.x * blocks * 256;
+    copy_rows(base, base_stride, out, out_stride, c0, c0 + 256 * blocks < N ? c0 + 256 * blocks : N, n, rowlist, wide);
+    return;
+  }
+  if (wave == 0) {
+    l.at_base[lane] = rowlist * base_stride;
+    l.at_out[lane] = rowlist * out_stride;
+  }
+  const T* bi = b + (int64_t)adapter * N * R;
+  typename L::v8 bf[4][L::KS];
+  int64_t n0 = ((int64_t)blockIdx.x * blocks * 4 + wave) * 64;
+  load_b<T, RT, VEC>(bi, n0, N, R, bf);  // on the way while t is joined
+  const float scale = scales ? scales[adapter] : 1.0f;
+  const int chunks = ((n + 15) & ~15) * L::CH;
+  for (int at0 = 0; at0 < chunks; at0 += 256) {
+    const int at = at0 + (int)threadIdx.x, i = at / L::CH, c = at % L::CH;
+    const int row = __shfl(rowlist, i & 63, MK_WAVE);  // (every lane: the source has to be active)
+    const int m = at < chunks ? row : -1;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (m >= 0) {
+      const float* tr = t + (int64_t)m * L::RP + 8 * c;
+      for (int z = 0; z < slices; ++z, tr += gs.M * L::RP) {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(tr), hi = *reinterpret_cast<const f32x4*>(tr + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] += lo[e];
+          v[4 + e] += hi[e];
+        }
+      }
+    }
+    l.put(i, c, v, scale, at < chunks);
+  }
+  lds_barrier();  // (the loads of B stay in flight)
+  for (int blk = 0; blk < blocks; ++blk, n0 += 256) {
+    if (n0 >= N) return;
+    if (blk) load_b<T, RT, VEC>(bi, n0, N, R, bf);
+    expand_rows<T, RT>(l, base, out, N, n0, n, wide, bf);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Both in one launch, for a single row of few ranks and a short K: a workgroup
+// of 8 waves has 512 outputs and forms t by itself, reading all of A: a wave
+// has every 8th rank, and reads a kilobyte of a row at a time.  That costs the
+// workgroup K ranks x 2 bytes from the L2, and saves a launch and the way
+// through memory.  One launch against two, us a call in a graph (the host's
+// time falls from 18 to 13 us): K 4096, rank 16: 6.1 / 7.2; K 4096, rank 32:
+// 8.6 / 8.5; K 14336, rank 16: 9.9 / 9.0; K 8192, rank 32: 12.2 / 9.5.  (Two
+// rows would take 10.2 / 7.6: the matrix cores are the better way for more.)
+// ---------------------------------------------------------------------------
+
+constexpr int kOneWaves = 8;
+
+template <typename T, int RT, bool VEC>
+__global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(const int32_t* __restrict__ ids, int adapters,
+                                                                  const T* __restrict__ x, const T* base,
+                                                                  const T* __restrict__ a, const T* __restrict__ b,
+                                                                  const float* __restrict__ scales, T* out, int64_t N,
+                                                                  int64_t K, int R, bool wide) {
+  typedef ExpandRows<T, RT> L;
+  constexpr int RW = L::RP / kOneWaves;  // ranks of a wave
+  constexpr int UN = RT == 1 ? 4 : 2;    // kilobytes of each row in flight
+  __shared__ L l;
+  __shared__ float t[L::RP];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int adapter = ids[0];
+  if (adapter < 0 || adapter >= adapters) {
+    const int64_t c0 = (int64_t)blockIdx.x * 64 * kOneWaves;
+    if (base != out) copy_rows(base, 0, out, 0, c0, c0 + 64 * kOneWaves < N ? c0 + 64 * kOneWaves : N, 1, 0, wide);
+    return;
+  }
+  if (wave == 0) l.at_base[lane] = l.at_out[lane] = 0;
+  const int64_t n0 = ((int64_t)blockIdx.x * kOneWaves + wave) * 64;
+  typename L::v8 bf[4][L::KS];
+  load_b<T, RT, VEC>(b + (int64_t)adapter * N * R, n0, N, R, bf);  // on the way while t is formed
+  const T* ar[RW];
+  float acc[RW];
+#pragma unroll
+  for (int q = 0; q < RW; ++q) {
+    const int r = wave + kOneWaves * q;
+    ar[q] = a + ((int64_t)adapter * R + (r < R ? r : 0)) * K;
+    acc[q] = 0.0f;
+  }
+  for (int64_t k0 = 8 * lane; k0 < K; k0 += 512 * UN) {
+    typename L::v8 av[UN][RW], xv[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+#pragma unroll
+      for (int q = 0; q < RW; ++q) av[u][q] = load_frag<T, VEC>(ar[q], k0 + 512 * u, K);
+      xv[u] = load_frag<T, VEC>(x, k0 + 512 * u, K);
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int q = 0; q < RW; ++q) acc[q] = fmaf(to_f32((T)av[u][q][e]), to_f32((T)xv[u][e]), acc[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < RW; ++q) {
+    const float s = wave_sum(acc[q]);
+    const int r = wave + kOneWaves * q;
+    if (lane == 0) t[r] = r < R ? s : 0.0f;
+  }
+  lds_barrier();
+  {
+    const int i = (int)threadIdx.x / L::CH, c = (int)threadIdx.x % L::CH;  // 16 rows, zeros behind the first
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (i == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = t[8 * c + e];
+    }
+    l.put(i & 15, c, v, scales ? scales[adapter] : 1.0f, i < 16);
+  }
+  lds_barrier();
+  if (n0 < N) expand_rows<T, RT>(l, base, out, N, n0, 1, wide, bf);
+}
+
 struct LoraPlan {
   int64_t groups, k_slice, order_ints;  // most groups that there can be
   int slices, rank_tiles, blocks;
+  bool one;  // one launch, no workspace
 };
 
 inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t adapters) {
   LoraPlan p;
   p.rank_tiles = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
   const int64_t kinds = adapters + 1 < M ? adapters + 1 : M;  // adapters that rows can name, and none
+  p.one = M == 1 && R <= 32 && K * p.rank_tiles <= 8192;
   p.groups = M <= kGroupRows ? kinds : M / kGroupRows + kinds;
   p.order_ints = M <= kGroupRows ? 0 : (p.groups * (kGroupRows + 1) + 1 + 3) / 4 * 4;
   // K in slices of four turns of a workgroup where there are few groups
@@ -526,6 +647,7 @@ extern "C" {
 size_t mk_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t adapters) {
   if (M <= 0 || N <= 0 || K <= 0 || R <= 0 || R > 128 || adapters <= 0) return 0;
   const LoraPlan p = lora_plan(M, N, K, R, adapters);
+  if (p.one) return 0;
   return ((size_t)p.order_ints + (size_t)p.slices * M * 16 * p.rank_tiles) * sizeof(float);
 }
 
@@ -538,8 +660,9 @@ int mk_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_
   MK_REQUIRE(x_stride >= K && base_stride >= N && out_stride >= N && (out != base || out_stride == base_stride));
   MK_REQUIRE(dtype == MK_DT_F16 || dtype == MK_DT_BF16);
   if (M == 0 || N == 0) return MK_OK;
-  MK_REQUIRE(x && base && adapter_ids && out && a && b && workspace && mk_aligned(workspace, 16));
-  MK_REQUIRE(workspace_bytes >= mk_lora_workspace_bytes(M, N, K, R, adapters));
+  MK_REQUIRE(x && base && adapter_ids && out && a && b && mk_aligned(workspace, 16));
+  const size_t need = mk_lora_workspace_bytes(M, N, K, R, adapters);
+  MK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const LoraPlan p = lora_plan(M, N, K, R, adapters);
   int32_t* order = reinterpret_cast<int32_t*>(workspace);
@@ -554,6 +677,25 @@ int mk_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_
     gs.adapters = order + p.groups * kGroupRows;
     lora_group_kernel<<<1, 1024, 0, st>>>(adapter_ids, order, order + p.groups * kGroupRows, M, (int)adapters);
   }
+#define MK_ONE(T, RT, V)                                                                                             \
+  lora_one_kernel<T, RT, V><<<(unsigned)((N + 64 * kOneWaves - 1) / (64 * kOneWaves)), 64 * kOneWaves, 0, st>>>( \
+      adapter_ids, (int)adapters, (const T*)x, (const T*)base, (const T*)a, (const T*)b, scales, (T*)out, N, K,  \
+      (int)R, wide)
+#define MK_ONE_VEC(T, RT)                     \
+  do {                                        \
+    if (vec_a && vec_b) MK_ONE(T, RT, true);  \
+    else MK_ONE(T, RT, false);                \
+  } while (0)
+  if (p.one) {
+    if (dtype == MK_DT_F16 && p.rank_tiles == 1) MK_ONE_VEC(f16, 1);
+    else if (dtype == MK_DT_F16) MK_ONE_VEC(f16, 2);
+    else if (p.rank_tiles == 1) MK_ONE_VEC(bf16, 1);
+    else MK_ONE_VEC(bf16, 2);
+    MK_CHECK_LAUNCH();
+    return MK_OK;
+  }
+#undef MK_ONE_VEC
+#undef MK_ONE
   const dim3 shrink((unsigned)p.groups, (unsigned)p.slices);
   const dim3 expand((unsigned)((N + 256 * p.blocks - 1) / (256 * p.blocks)), (unsigned)p.groups);
 #define MK_SHRINK(T, RT, V)                                                                                         \

@@ -148,10 +148,10 @@ def lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None, out=None, bac
         a, b = lora_a.contiguous(), lora_b.contiguous()
         scales = as_dense(scales, torch.float32)
         size = _lib.load().mk_lora_workspace_bytes(M, N, K, R, adapters)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         _lib.launch("mk_lora_add", dev, x2.data_ptr(), x_stride, b2.data_ptr(), base_stride, a.data_ptr(),
                     b.data_ptr(), ids.data_ptr(), _lib.ptr(scales), target.data_ptr(), out_stride, M, N, K, R,
-                    adapters, _lib.dtype_code(x.dtype), ws.data_ptr(), size)
+                    adapters, _lib.dtype_code(x.dtype), _lib.ptr(ws), size)
     if out is not None and target is not out:
         out.copy_(target)
         return out

@@ -20,7 +20,8 @@ SHAPES = [(1, 64, 64, 16, 1), (1, 6144, 4096, 16, 4), (2, 1, 1, 1, 1), (3, 100, 
           (17, 65, 33, 17, 2), (5, 40, 30, 4, 3), (33, 130, 264, 32, 9), (20, 48, 520, 33, 20), (64, 256, 96, 64, 4),
           (7, 200, 1000, 128, 2), (65, 72, 2056, 48, 1), (130, 1024, 136, 100, 5), (300, 96, 512, 16, 2),
           (31, 8, 4100, 2, 3), (48, 4096, 8, 127, 2), (70, 328, 1504, 64, 7), (64, 40, 64, 8, 80), (2000, 72, 96, 8, 300),
-          (200, 16, 24, 3, 4096), (1100, 300, 520, 128, 2)]
+          (200, 16, 24, 3, 4096), (1100, 300, 520, 128, 2),
+          (1, 520, 4096, 32, 2), (1, 1030, 520, 20, 3), (1, 513, 1100, 7, 2), (1, 64, 14336, 16, 2), (1, 4096, 8, 128, 3)]
 
 
 def on(dev, *tensors):
@@ -72,6 +73,9 @@ def test_strides_and_alignment(dev, dtype):
     check_lora(got.reshape(M, N), *case[:4], per.repeat_interleave(4), case[5])
     turned = x3.transpose(0, 1).contiguous().transpose(0, 1)  # rows not at one stride
     assert torch.equal(lo.lora_add(turned, base3.transpose(0, 1).contiguous().transpose(0, 1), a, b, per, scales=s), got)
+    for i in (-1, 2):  # a single row, with and without an adapter
+        args = x[:1], base[:1], a, b, torch.tensor([i], dtype=torch.int32, device=dev)
+        check_lora(lo.lora_add(*args, scales=s), case[0][:1], case[1][:1], case[2], case[3], torch.tensor([i]), case[5])
     out = torch.zeros_like(base3).transpose(0, 1).contiguous().transpose(0, 1)
     assert lo.lora_add(x3, base3, a, b, per, scales=s, out=out) is out and torch.equal(out, got)
     assert lo.lora_add(x[:0], base[:0], a, b, ids[:0]).shape == (0, N)
