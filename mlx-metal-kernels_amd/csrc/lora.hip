@@ -535,10 +535,11 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
 // of 8 waves has 512 outputs and forms t by itself, reading all of A: a wave
 // has every 8th rank, and reads a kilobyte of a row at a time.  That costs the
 // workgroup K ranks x 2 bytes from the L2, and saves a launch and the way
-// through memory.  One launch against two, us a call in a graph (the host's
-// time falls from 18 to 13 us): K 4096, rank 16: 6.1 / 7.2; K 4096, rank 32:
-// 8.6 / 8.5; K 14336, rank 16: 9.9 / 9.0; K 8192, rank 32: 12.2 / 9.5.  (Two
-// rows would take 10.2 / 7.6: the matrix cores are the better way for more.)
+// through memory.  One launch against two, us a call in a graph (the host's time
+// falls from 18 to 14 us): K 4096, rank 16: 5.3 / 7.2; K 4096, rank 32: 6.6 /
+// 8.4; K 14336, rank 16: 8.8 / 8.9; K 8192, rank 32: 9.0 / 9.5; K 14336, rank
+// 32: 14.4 / 11.0.  (Two rows at K 4096, rank 16 would take 10.2 / 7.6: the
+// matrix cores are the better way for more.)
 // ---------------------------------------------------------------------------
 
 constexpr int kOneWaves = 8;
@@ -618,7 +619,7 @@ inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t ad
   LoraPlan p;
   p.rank_tiles = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
   const int64_t kinds = adapters + 1 < M ? adapters + 1 : M;  // adapters that rows can name, and none
-  p.one = M == 1 && R <= 32 && K * p.rank_tiles <= 8192;
+  p.one = M == 1 && R <= 32 && K * p.rank_tiles <= 16384;
   p.groups = M <= kGroupRows ? kinds : M / kGroupRows + kinds;
   p.order_ints = M <= kGroupRows ? 0 : (p.groups * (kGroupRows + 1) + 1 + 3) / 4 * 4;
   // K in slices of four turns of a workgroup where there are few groups

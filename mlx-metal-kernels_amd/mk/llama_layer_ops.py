@@ -136,6 +136,24 @@ class LlamaLayerKernelWeights:
     down_zeros: Any | None = None
     bits: int = 4
     group_size: int = 32
+    # beyond the reference: norms of q and k heads [head_dim], the rotary layout ("interleaved" or "half"; the
+    # tables' width says how much of a head turns), adapters (lora_ops.LoraAdapters) beside qkv and o
+    q_norm_weight: Any | None = None
+    k_norm_weight: Any | None = None
+    rope_layout: str = "interleaved"
+    qkv_lora: Any | None = None
+    o_lora: Any | None = None
+
+    def block_options(self, cos, config: LlamaLikeConfig, adapter_ids=None) -> dict:
+        """What the decode block takes for these fields (nothing for a layer without them)."""
+        out = {}
+        if self.q_norm_weight is not None or self.k_norm_weight is not None:
+            out.update(q_norm_weight=self.q_norm_weight, k_norm_weight=self.k_norm_weight)
+        if self.rope_layout != "interleaved" or 2 * cos.shape[1] != config.head_dim:
+            out.update(rope_layout=self.rope_layout, rotary_dim=2 * cos.shape[1])
+        if adapter_ids is not None:
+            out.update(qkv_lora=self.qkv_lora, out_lora=self.o_lora, adapter_ids=adapter_ids)
+        return out
 
     def validate(self, config: LlamaLikeConfig) -> "LlamaLayerKernelWeights":
         """ops/llama_layer_ops.py:110-134."""
@@ -143,6 +161,8 @@ class LlamaLayerKernelWeights:
             raise ValueError(f"bits must be 4 or 8, got {self.bits}")
         if self.group_size <= 0:
             raise ValueError(f"group_size must be positive, got {self.group_size}")
+        if (self.q_norm_weight is None) != (self.k_norm_weight is None):
+            raise ValueError("give q_norm_weight and k_norm_weight, or neither")
         H = config.hidden_size
         for name in ("input_layernorm_weight", "post_attention_layernorm_weight"):
             if tuple(getattr(getattr(self, name), "shape", ())) != (H,):
@@ -209,7 +229,7 @@ def _check_decode(x, config: LlamaLikeConfig, cache, cache_layout: str):
 
 def llama_layer_decode_step(x, weights: LlamaLayerKernelWeights, cache, cos, sin, position, config,
                             *, cache_layout: str = "contiguous", return_intermediates: bool = False, lengths=None,
-                            verify_width: int = 1):
+                            verify_width: int = 1, adapter_ids=None):
     """ops/llama_layer_ops.py:234-428, all stages on HIP.  x [B,1,hidden];
     cache (K_pages, V_pages, block_table) for cache_layout="paged" or
     (K_cache, V_cache) [B,MAX_S,Hkv,D] for "contiguous", updated in place;
@@ -217,7 +237,9 @@ def llama_layer_decode_step(x, weights: LlamaLayerKernelWeights, cache, cos, sin
     (out, cache, intermediates).  The input RMSNorm runs inside the qkv
     matvec and the residual add inside the o-proj matvec; ``lengths``
     (extension) = position + 1 as a device tensor shared by all layers;
-    ``verify_width`` (extension): see paged_quantized_decode_block."""
+    ``verify_width`` (extension): see paged_quantized_decode_block;
+    ``adapter_ids`` (extension) int32 [B]: each row's adapter in the weights'
+    ``qkv_lora`` and ``o_lora`` (-1: none; None: the layer without adapters)."""
     config = config.validate()
     weights.validate(config)
     K_pages, V_pages, block_table, restore = _check_decode(x, config, cache, cache_layout)
@@ -229,7 +251,7 @@ def llama_layer_decode_step(x, weights: LlamaLayerKernelWeights, cache, cos, sin
         group_size=weights.group_size, H=config.num_attention_heads, num_key_value_heads=config.num_key_value_heads,
         head_dim=config.head_dim, return_intermediates=return_intermediates, residual=x,
         norm_weight=weights.input_layernorm_weight, eps=config.rms_norm_eps, lengths=lengths,
-        verify_width=verify_width)
+        verify_width=verify_width, **weights.block_options(cos, config, adapter_ids))
     h, K_pages, V_pages = blk[:3]
     qkv, attn_out = (blk[3], blk[4]) if return_intermediates else (None, None)
     res = quantized_mlp_block(h, _zero_residual(h), weights.post_attention_layernorm_weight, weights.gate_w,
@@ -247,7 +269,8 @@ def llama_layer_decode_step(x, weights: LlamaLayerKernelWeights, cache, cos, sin
 
 
 def reference_llama_layer_decode_step(x, weights: LlamaLayerKernelWeights, cache, cos, sin, position, config,
-                                      *, cache_layout: str = "contiguous", return_intermediates: bool = False):
+                                      *, cache_layout: str = "contiguous", return_intermediates: bool = False,
+                                      adapter_ids=None):
     """ops/llama_layer_ops.py:214-231 (every stage on the torch reference
     path; the cache is updated functionally, the input cache untouched)."""
     config = config.validate()
@@ -258,7 +281,8 @@ def reference_llama_layer_decode_step(x, weights: LlamaLayerKernelWeights, cache
         x_norm, weights.qkv_w, weights.qkv_scales, weights.o_w, weights.o_scales, K_pages, V_pages, block_table, cos,
         sin, position, qkv_zeros=weights.qkv_zeros, out_zeros=weights.o_zeros, bits=weights.bits,
         group_size=weights.group_size, H=config.num_attention_heads, num_key_value_heads=config.num_key_value_heads,
-        head_dim=config.head_dim, return_intermediates=True)
+        head_dim=config.head_dim, return_intermediates=True, eps=config.rms_norm_eps,
+        **weights.block_options(cos, config, adapter_ids))
     h = (x.float() + attn_proj.float()).to(x.dtype)
     res = reference_quantized_mlp_block(h, torch.zeros_like(h), weights.post_attention_layernorm_weight, weights.gate_w,
                                         weights.gate_scales, weights.up_w, weights.up_scales, weights.down_w,
@@ -279,7 +303,7 @@ _LOOP_PRESETS = ("reference", "metal", "tiled", "fused_experimental")
 
 def llama_layer_decode_loop(inputs, weights: LlamaLayerKernelWeights, cache, cos, sin, config, *,
                             backend_preset: str = "fused_experimental", cache_layout: str = "contiguous",
-                            T: int | None = None, return_final_cache: bool = True):
+                            T: int | None = None, return_final_cache: bool = True, adapter_ids=None):
     """ops/llama_layer_ops.py:431-467: decode inputs [B, T, hidden] one step
     at a time, step t at position t of every sequence.  Preset "reference"
     runs every stage on the torch reference path (functional cache updates);
@@ -294,7 +318,8 @@ def llama_layer_decode_loop(inputs, weights: LlamaLayerKernelWeights, cache, cos
     outputs = []
     running = cache
     for t in range(T):
-        out_t, running = step(inputs[:, t:t + 1, :], weights, running, cos, sin, t, config, cache_layout=cache_layout)
+        out_t, running = step(inputs[:, t:t + 1, :], weights, running, cos, sin, t, config, cache_layout=cache_layout,
+                              adapter_ids=adapter_ids)
         outputs.append(out_t)
     out = torch.cat(outputs, dim=1) if len(outputs) > 1 else outputs[0]
     return (out, running) if return_final_cache else out

@@ -156,7 +156,7 @@ def greedy_sample(logits):
 
 def llama_stack_decode_step(x, stack_weights: LlamaStackWeights, stack_cache: LlamaStackCache, cos, sin, position,
                             config: LlamaLikeConfig, *, return_intermediates: bool = False, reference: bool = False,
-                            float_logits: bool = True, verify_width: int = 1):
+                            float_logits: bool = True, verify_width: int = 1, adapter_ids=None):
     """ops/llama_stack_ops.py:352-411 on paged caches.  Returns (logits,
     final_hidden, cache) when the weights carry an lm_head, else
     (final_hidden, cache); with return_intermediates the per-layer hidden
@@ -165,7 +165,9 @@ def llama_stack_decode_step(x, stack_weights: LlamaStackWeights, stack_cache: Ll
     exact, so an argmax over either agrees).  ``verify_width`` W > 1
     (extension): the rows are W draft rows per sequence (row b * W + w at
     position[b * W + w], consecutive positions, block tables repeated W
-    times), whose attention runs as one verify launch per layer."""
+    times), whose attention runs as one verify launch per layer.
+    ``adapter_ids`` (extension) int32 [rows]: each row's low-rank adapter in
+    every layer's ``qkv_lora`` and ``o_lora`` (-1: none)."""
     config = config.validate()
     hidden = x
     layers_out = []
@@ -179,11 +181,12 @@ def llama_stack_decode_step(x, stack_weights: LlamaStackWeights, stack_cache: Ll
     for li, lw in enumerate(stack_weights.layers):
         if reference:
             hidden, cache = reference_llama_layer_decode_step(hidden, lw, stack_cache.layer_caches[li], cos, sin,
-                                                              position, config, cache_layout=stack_cache.cache_layout)
+                                                              position, config, cache_layout=stack_cache.cache_layout,
+                                                              adapter_ids=adapter_ids)
         else:
             hidden, cache = llama_layer_decode_step(hidden, lw, stack_cache.layer_caches[li], cos, sin, position,
                                                     config, cache_layout=stack_cache.cache_layout, lengths=lengths,
-                                                    verify_width=verify_width)
+                                                    verify_width=verify_width, adapter_ids=adapter_ids)
         new_caches.append(cache)
         if return_intermediates:
             layers_out.append(hidden)
@@ -314,15 +317,18 @@ class DecodeGraph:
     given positions, ``first_tokens`` holds that step's output, ``tokens`` is
     the input of the first ``step()`` (equal to ``first_tokens``) and
     ``positions`` has advanced by one.  So the tokens of a greedy run are
-    ``first_tokens`` followed by the output of each ``step()``."""
+    ``first_tokens`` followed by the output of each ``step()``.
+    ``adapter_ids`` (int32 [B], device): every row's low-rank adapter, read
+    anew by each step, so a caller may change them in place."""
 
     def __init__(self, stack_weights: LlamaStackWeights, stack_cache: LlamaStackCache, cos, sin,
-                 config: LlamaLikeConfig, token_ids, positions):
+                 config: LlamaLikeConfig, token_ids, positions, *, adapter_ids=None):
         if stack_weights.embedding is None or stack_weights.lm_head is None:
             raise ValueError("DecodeGraph needs an embedding and an lm_head")
         self.w, self.cache, self.cos, self.sin, self.config = stack_weights, stack_cache, cos, sin, config
         self.tokens = token_ids.clone()
         self.positions = positions.to(torch.int32).clone()
+        self.adapter_ids = adapter_ids
         self.stream = torch.cuda.Stream(device=self.tokens.device)
         self.stream.wait_stream(torch.cuda.current_stream(self.tokens.device))
         with torch.cuda.stream(self.stream):
@@ -335,7 +341,7 @@ class DecodeGraph:
     def _run(self):
         x = embed_token_ids(self.tokens, self.w.embedding)
         logits, _, _ = llama_stack_decode_step(x, self.w, self.cache, self.cos, self.sin, self.positions, self.config,
-                                               float_logits=False)
+                                               float_logits=False, adapter_ids=self.adapter_ids)
         nxt = greedy_sample(logits)
         self.tokens.copy_(nxt)
         self.positions.add_(1)

@@ -10,6 +10,8 @@ zeros), ``scales`` fp32 [ADAPTERS] (None: 1).
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
+from typing import Any
 
 import torch
 
@@ -19,6 +21,16 @@ from .kv_cache_ops import host_checks_enabled
 from .mlp_block_ops import quantized_linear
 
 MAX_RANK, MAX_ADAPTERS = 128, 4096
+
+
+@dataclass
+class LoraAdapters:
+    """The adapters beside one projection [N, K]: a [ADAPTERS, R, K], b
+    [ADAPTERS, N, R], scales fp32 [ADAPTERS] or None."""
+
+    a: Any
+    b: Any
+    scales: Any | None = None
 
 
 def _validate(x, base, lora_a, lora_b, adapter_ids, scales, out):

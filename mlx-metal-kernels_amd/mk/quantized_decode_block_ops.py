@@ -20,8 +20,14 @@ import torch
 
 from . import _lib
 from ._common import as_u8, scales_for_kernel
-from .gqa_ops import paged_gqa_decode_block_from_qkv, reference_paged_gqa_decode_block_from_qkv
+from .gqa_ops import (
+    paged_gqa_decode_attention,
+    paged_gqa_decode_block_from_qkv,
+    paged_qk_norm_rope_update,
+    reference_paged_gqa_decode_block_from_qkv,
+)
 from .kv_cache_ops import normalize_positions
+from .lora_ops import lora_add
 from .norm_ops import reference_rms_norm
 from .paged_kv_ops import _hip_paged_attention, _i32
 from .quant_ops import (
@@ -229,7 +235,9 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
                                  position, *, qkv_zeros=None, out_zeros=None, bits=4, group_size=32, H=None,
                                  num_key_value_heads=None, head_dim=None, D=None, scale=None,
                                  matvec_backend="metal_parallel", block_backend="auto", return_intermediates=False,
-                                 residual=None, norm_weight=None, eps=1e-5, lengths=None, verify_width=1):
+                                 residual=None, norm_weight=None, eps=1e-5, lengths=None, verify_width=1,
+                                 q_norm_weight=None, k_norm_weight=None, rope_layout="interleaved", rotary_dim=None,
+                                 qkv_lora=None, out_lora=None, adapter_ids=None):
     """ops/quantized_decode_block_ops.py:446-552: returns (projected [B,1,H*D
     -> hidden], K_pages, V_pages) or with (qkv, attn_out) appended.
 
@@ -244,7 +252,14 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
     position[b * W + w], the block table repeated W times); the attention
     then runs as mk_paged_verify_attention over the sequences' own table rows
     (one K/V read for the W rows), with ``lengths`` (required) per sequence,
-    the last row's position + 1."""
+    the last row's position + 1.
+
+    Models with norms of q and k heads (``q_norm_weight``, ``k_norm_weight``
+    [D], at ``eps``), half-layout rotary positions or rotation of a part of
+    each head (``rope_layout``, ``rotary_dim``) take ``paged_qk_norm_rope_update``
+    between the projection and the attention.  ``qkv_lora``, ``out_lora``
+    (``LoraAdapters``) with ``adapter_ids`` [rows] add every row's adapter to
+    the two projections (``lora_add``; to the output one behind the residual)."""
     x2d, _, _ = normalize_hidden_input(x)
     H, kv_heads, D = _block_dims(qkv_w, H, num_key_value_heads, head_dim, D, bits)
     validate_quantized_weight_shapes(x2d, qkv_w, qkv_scales, qkv_zeros, bits=bits, group_size=group_size,
@@ -253,7 +268,11 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
     validate_quantized_weight_shapes(x2d.new_empty((x2d.shape[0], H * D)), out_w, out_scales, out_zeros, bits=bits,
                                      group_size=group_size, expected_in_dim=H * D, name="output_projection")
     reference = matvec_backend.lower() == "reference"
-    fuse_front = (norm_weight is not None and not reference and not return_intermediates and
+    if (qkv_lora is not None or out_lora is not None) and adapter_ids is None:
+        raise ValueError("qkv_lora and out_lora need adapter_ids")
+    other_rope = (q_norm_weight is not None or k_norm_weight is not None or rope_layout != "interleaved"
+                  or rotary_dim not in (None, D))
+    fuse_front = (norm_weight is not None and not other_rope and qkv_lora is None and not reference and not return_intermediates and
                   block_backend.lower() != "reference" and K_pages.dtype == x2d.dtype and
                   K_pages.dtype in (torch.float16, torch.bfloat16))
     if fuse_front:
@@ -277,15 +296,30 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
                                             pos + 1 if lengths is None else lengths, sc).unsqueeze(1)
     elif norm_weight is not None and not reference:
         qkv = q_rmsnorm_matvec(x2d, norm_weight, qkv_w, qkv_scales, qkv_zeros, bits=bits, group_size=group_size,
-                               eps=eps).reshape(x2d.shape[0], 1, -1)
+                               eps=eps, return_normed=qkv_lora is not None)
+        if qkv_lora is not None:
+            qkv, x2d = qkv
+        qkv = qkv.reshape(x2d.shape[0], 1, -1)
     else:
         if norm_weight is not None:
             x2d = reference_rms_norm(x2d[:, None], norm_weight, eps=eps)[:, 0]
         qkv = quantized_qkv_projection(x2d, qkv_w, qkv_scales, qkv_zeros, bits=bits, group_size=group_size,
                                        backend=matvec_backend)
+    if qkv_lora is not None:
+        qkv = lora_add(x2d[:, None], qkv, qkv_lora.a, qkv_lora.b, adapter_ids, scales=qkv_lora.scales,
+                       backend="reference" if reference else "auto")
     block_fn = reference_paged_gqa_decode_block_from_qkv if block_backend.lower() == "reference" else None
     if fuse_front:
         pass
+    elif other_rope:
+        plain = "reference" if block_fn is not None else "auto"
+        q, K_pages, V_pages = paged_qk_norm_rope_update(
+            qkv, K_pages, V_pages, block_table, cos, sin, position, num_attention_heads=H,
+            num_key_value_heads=kv_heads, head_dim=D, q_weight=q_norm_weight, k_weight=k_norm_weight, eps=eps,
+            layout=rope_layout, rotary_dim=rotary_dim, backend=plain)
+        if lengths is None or verify_width > 1:  # verify rows here: one sequence each
+            lengths = (position if isinstance(position, int) else torch.as_tensor(position)) + 1
+        attn_out = paged_gqa_decode_attention(q, K_pages, V_pages, block_table, lengths, scale, backend=plain)
     elif block_fn is not None:
         attn_out, K_pages, V_pages = block_fn(qkv, K_pages, V_pages, block_table, cos, sin, position,
                                               num_attention_heads=H, num_key_value_heads=kv_heads, head_dim=D,
@@ -306,6 +340,9 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
                                                 backend=matvec_backend)
         if residual is not None:
             projected = (residual.reshape(B, 1, -1).float() + projected.float()).to(projected.dtype)
+    if out_lora is not None:
+        projected = lora_add(a2d[:, None], projected, out_lora.a, out_lora.b, adapter_ids, scales=out_lora.scales,
+                             backend="reference" if reference else "auto")
     if return_intermediates:
         return projected, K_pages, V_pages, qkv, attn_out
     return projected, K_pages, V_pages
@@ -314,12 +351,14 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
 def reference_paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_pages, V_pages, block_table,
                                            cos, sin, position, *, qkv_zeros=None, out_zeros=None, bits=4,
                                            group_size=32, H=None, num_key_value_heads=None, head_dim=None, D=None,
-                                           scale=None, return_intermediates=False):
+                                           scale=None, return_intermediates=False, **options):
     """ops/quantized_decode_block_ops.py:395-443 (reference matvecs and
-    reference paged block; K_pages / V_pages are updated functionally)."""
+    reference paged block; K_pages / V_pages are updated functionally).
+    ``options``: eps, head norms, rotary layout and adapters as
+    ``paged_quantized_decode_block`` takes them."""
     return paged_quantized_decode_block(
         x, qkv_w, qkv_scales, out_w, out_scales, K_pages.clone(), V_pages.clone(), block_table, cos, sin, position,
         qkv_zeros=qkv_zeros, out_zeros=out_zeros, bits=bits, group_size=group_size, H=H,
         num_key_value_heads=num_key_value_heads, head_dim=head_dim, D=D, scale=scale, matvec_backend="reference",
-        block_backend="reference", return_intermediates=return_intermediates)
+        block_backend="reference", return_intermediates=return_intermediates, **options)
 

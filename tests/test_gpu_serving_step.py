@@ -1,0 +1,176 @@
+"""The operators of a server together: a stack with norms of q and k heads,
+half-layout rotation of a part of each head and adapters, over cache pages
+that are reserved, forked, freed and compacted between its steps."""
+
+import numpy as np
+import pytest
+import torch
+
+from mk import gqa_ops, kv_page_ops
+from mk import llama_layer_ops as ll
+from mk import llama_stack_ops as ls
+from mk.lora_ops import LoraAdapters
+from mk.paged_kv_ops import make_identity_block_table
+from mk.rope_ops import build_scaled_rope_tables
+from tests._data import assert_close
+
+pytestmark = pytest.mark.gpu
+
+CFG = ll.LlamaLikeConfig(hidden_size=256, intermediate_size=512, num_attention_heads=4, num_key_value_heads=2,
+                         head_dim=64, num_hidden_layers=2, max_position_embeddings=256, vocab_size=512).validate()
+ROTARY = 32
+
+
+def _weights(dev, bits=4, dtype=torch.float16):
+    w = ls.create_random_quantized_llama_stack_weights(CFG, bits=bits, dtype=dtype, seed=3, device=dev)
+    g = torch.Generator(device=dev).manual_seed(4)
+
+    def lora(n, k):
+        a = torch.randn(3, 8, k, generator=g, device=dev) / k ** 0.5
+        b = torch.randn(3, n, 8, generator=g, device=dev) * 0.1
+        return LoraAdapters(a.to(dtype), b.to(dtype), torch.tensor([0.5, 1.0, 2.0], device=dev))
+
+    for layer in w.layers:
+        layer.q_norm_weight, layer.k_norm_weight = (
+            (1 + 0.2 * torch.randn(CFG.head_dim, generator=g, device=dev)).to(dtype) for _ in range(2))
+        layer.rope_layout = "half"
+        layer.qkv_lora, layer.o_lora = lora(CFG.qkv_output_dim(), CFG.hidden_size), lora(CFG.hidden_size, CFG.hidden_size)
+    return w
+
+
+def _tables(dev):
+    return build_scaled_rope_tables(CFG.max_position_embeddings, ROTARY, device=dev,
+                                    scaling={"type": "yarn", "factor": 4, "original_max_position": 64})
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("layout", ["paged", "contiguous"])
+def test_layer_against_reference_backend(dev, bits, dtype, layout):
+    torch.manual_seed(bits)
+    w = _weights(dev, bits, dtype).layers[0]
+    cos, sin = _tables(dev)
+    B, S = 5, 48
+    cache = ll.init_llama_layer_cache(CFG, B, S, cache_layout=layout, dtype=dtype, device=dev)
+    for t in cache[:2]:
+        t.copy_(torch.randn(t.shape, device=dev))
+    x = torch.randn(B, 1, CFG.hidden_size, device=dev).to(dtype)
+    pos = torch.tensor([0, 47, 16, 15, 30], dtype=torch.int32, device=dev)
+    ids = torch.tensor([2, -1, 0, 1, 2], dtype=torch.int32, device=dev)
+    kw = dict(cache_layout=layout, adapter_ids=ids)
+    ref, ref_cache = ll.reference_llama_layer_decode_step(x, w, cache, cos, sin, pos, CFG, **kw)
+    got, got_cache = ll.llama_layer_decode_step(x, w, tuple(t.clone() for t in cache), cos, sin, pos, CFG, **kw)
+    # the bound of the layer's other test against its reference path; bf16 rounds 8 times as coarsely
+    scale = 1 if dtype == torch.float16 else 8
+    assert_close(got, ref.float().cpu().numpy(), what="layer", rtol=1e-2 * scale, atol=1e-3 * scale)
+    for a, b in zip(got_cache[:2], ref_cache[:2]):
+        assert_close(a, b.float().cpu().numpy(), what="cache", rtol=1e-2 * scale, atol=1e-3 * scale)
+    plain, _ = ll.llama_layer_decode_step(x, w, tuple(t.clone() for t in cache), cos, sin, pos, CFG,
+                                          cache_layout=layout)
+    none, _ = ll.llama_layer_decode_step(x, w, tuple(t.clone() for t in cache), cos, sin, pos, CFG,
+                                         cache_layout=layout, adapter_ids=torch.full_like(ids, -1))
+    assert torch.equal(plain, none) and not torch.equal(got, plain) and torch.equal(got[1], plain[1])
+
+
+def _own_pages(caches, table, lengths, P, blocks):
+    """Every row's history in pages of its own, under an identity table."""
+    B = table.shape[0]
+    own = make_identity_block_table(B, blocks * P, P, device=table.device)
+    out = []
+    for K, V, _ in caches:
+        pair = []
+        for t in (K, V):
+            rows = t[table.clamp(min=0).long()].reshape(B * blocks, *t.shape[1:])
+            pair.append(rows.clone())
+        out.append((*pair, own))
+    return out
+
+
+def test_forked_decode_steps(dev):
+    """Two prompts written through their reserved pages; then steps whose rows fork, end and are compacted: each gives
+    bit by bit what the same step gives on pages that nobody shares."""
+    torch.manual_seed(0)
+    rng = np.random.default_rng(0)
+    w, (cos, sin) = _weights(dev), _tables(dev)
+    P, blocks, NP, L = 8, 8, 40, CFG.num_hidden_layers
+    Hq, Hkv, D = CFG.num_attention_heads, CFG.num_key_value_heads, CFG.head_dim
+    pages = [torch.randn(NP, P, Hkv, D, device=dev).half() for _ in range(2 * L)]
+    table = torch.full((2, blocks), -1, dtype=torch.int32, device=dev)
+    refs = torch.zeros(NP, dtype=torch.int32, device=dev)
+    prompt = [21, 9]
+    table, lengths, refs, ready = kv_page_ops.fork_kv_sequences(pages, table, [0, 0], refs, [0, 1], reserve=max(prompt))
+    assert all(ready.tolist())
+    seq = torch.tensor([0] * prompt[0] + [1] * prompt[1], dtype=torch.int32, device=dev)
+    pos = torch.tensor(list(range(prompt[0])) + list(range(prompt[1])), dtype=torch.int32, device=dev)
+    for i, layer in enumerate(w.layers):
+        qkv = torch.randn(sum(prompt), CFG.qkv_output_dim(), device=dev).half()
+        gqa_ops.paged_qk_norm_rope_update(qkv, pages[2 * i], pages[2 * i + 1], table, cos, sin, pos,
+                                          num_attention_heads=Hq, num_key_value_heads=Hkv, head_dim=D,
+                                          q_weight=layer.q_norm_weight, k_weight=layer.k_norm_weight, sequences=seq,
+                                          layout="half", rotary_dim=ROTARY)
+    lengths = torch.tensor(prompt, dtype=torch.int32, device=dev)
+    for step in range(12):
+        alive = [b for b in range(table.shape[0]) if int(lengths[b]) > 0]
+        parents = torch.tensor([int(rng.choice(alive)) for _ in range(5)], dtype=torch.int32, device=dev)
+        table, lengths, refs, ready = kv_page_ops.fork_kv_sequences(pages, table, lengths, refs, parents)
+        assert all(ready.tolist())
+        if step % 3 == 2:
+            table, refs, _, live = kv_page_ops.compact_kv_pages(pages, table, refs)
+            assert (refs[int(live):] == 0).all()
+        ids = torch.from_numpy(rng.integers(-1, 3, size=5)).to(torch.int32).to(dev)
+        x = torch.randn(5, 1, CFG.hidden_size, device=dev).half()
+        shared = [(pages[2 * i], pages[2 * i + 1], table) for i in range(L)]
+        own = _own_pages(shared, table, lengths, P, blocks)
+        outs = []
+        for caches in (shared, own):
+            cache = ls.LlamaStackCache(caches, "paged", blocks * P, P)
+            outs.append(ls.llama_stack_decode_step(x, w, cache, cos, sin, lengths, CFG, adapter_ids=ids)[0])
+        assert torch.equal(outs[0], outs[1]) and outs[0].isfinite().all(), step
+        for (K, V, _), (Ko, Vo, to) in zip(shared, own):  # the new token, where each table says
+            for b in range(5):
+                j, o = int(lengths[b]) // P, int(lengths[b]) % P
+                assert torch.equal(K[table[b, j], o], Ko[to[b, j], o]) and torch.equal(V[table[b, j], o], Vo[to[b, j], o])
+        lengths = lengths + 1
+
+
+def test_decode_graph_with_adapters(dev):
+    """The captured step of such a stack, adapters changed between replays, against eager steps."""
+    w, (cos, sin) = _weights(dev), _tables(dev)
+    B, S = 4, 64
+    caches = [ls.LlamaStackCache([ll.init_llama_layer_cache(CFG, B, S, cache_layout="paged", device=dev)
+                                  for _ in range(CFG.num_hidden_layers)], "paged", S, 16) for _ in range(2)]
+    tokens = torch.tensor([3, 5, 7, 11], device=dev)
+    pos = torch.zeros(B, dtype=torch.int32, device=dev)
+    ids = torch.tensor([0, 1, 2, -1], dtype=torch.int32, device=dev)
+    graph = ls.DecodeGraph(w, caches[0], cos, sin, CFG, tokens, pos, adapter_ids=ids)
+    got, want = [graph.first_tokens.clone()], []
+    order = [ids.clone()]
+    for i in range(6):
+        ids.copy_(torch.roll(ids, 1))
+        order.append(ids.clone())
+        got.append(graph.step().clone())
+    t, p = tokens, pos.clone()
+    for step_ids in order:
+        x = ls.embed_token_ids(t, w.embedding)
+        logits, _, caches[1] = ls.llama_stack_decode_step(x, w, caches[1], cos, sin, p, CFG, float_logits=False,
+                                                          adapter_ids=step_ids)
+        t, p = ls.greedy_sample(logits), p + 1
+        want.append(t)
+    assert torch.equal(torch.stack(got), torch.stack(want))
+    for a, b in zip(caches[0].layer_caches, caches[1].layer_caches):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_block_refusals(dev):
+    w, (cos, sin) = _weights(dev), _tables(dev)
+    cache = ll.init_llama_layer_cache(CFG, 1, 16, cache_layout="paged", device=dev)
+    x = torch.zeros(1, 1, CFG.hidden_size, device=dev).half()
+    layer = w.layers[0]
+    layer.k_norm_weight = None
+    with pytest.raises(ValueError, match="q_norm_weight and k_norm_weight"):
+        ll.llama_layer_decode_step(x, layer, cache, cos, sin, 0, CFG, cache_layout="paged")
+    from mk.quantized_decode_block_ops import paged_quantized_decode_block
+
+    with pytest.raises(ValueError, match="need adapter_ids"):
+        paged_quantized_decode_block(x, layer.qkv_w, layer.qkv_scales, layer.o_w, layer.o_scales, *cache, cos, sin, 0,
+                                     H=4, num_key_value_heads=2, head_dim=64, qkv_lora=layer.qkv_lora)
