@@ -10,12 +10,25 @@
 // are copied.  fp32 throughout and one rounding into the storage type.
 //
 // Both are bound by memory: a head's D values are read and written once.  A
-// unit of work is 16 values, two 16-byte chunks that hold the partners of
-// each other's values (chunks u and u + R/16 in the half layout, 2u and
-// 2u + 1 in the interleaved one), so a lane rotates without lane exchange and
-// needs one run of 8 cos and 8 sin values; the lanes of a wave that hold the
-// same unit of several heads read the same table bytes.  A head is D/16 lanes,
-// and its sum of squares goes over those lanes by shuffles.
+// unit of work is 16 values, two pieces of 8 that hold the partners of each
+// other's values: 8 values and those R/2 further in the half layout, 16 in a
+// row in the interleaved one and past R.  So a lane rotates without lane
+// exchange and needs 8 cos and 8 sin values; the lanes of a wave that hold the
+// same unit of several heads read the same table bytes.  The lanes of a head
+// have its sum of squares by shuffles.
+//
+// WHOLE kernels have D and R in whole units and every address on 16 bytes.
+// The others take any sizes and alignment: the last piece of a region starts 8
+// values before the region's end, over values that an earlier piece has too
+// (both write the same bits), loads are 16 bytes from any address, and only a
+// region of under 8 values goes value by value.
+//
+// 4 x 2047 tokens of 32 heads of 128, bf16: 27 us with R = 64 or 128 (5.1 TB/s,
+// what a copy of that size reaches), 30 us with R = 120 (94 us value by value,
+// a wave a head).  Norms, rotation and cache write of 8191 tokens of 32 + 2 x 8
+// such heads: 43 us (4.8 TB/s), with R = 120 62 us, for 9 of a head's 16 lanes
+// have a unit (252 us value by value).  A single token's take 2 and 3 us: they
+// are the launch.
 #include "common.h"
 #include "paged_common.h"
 
@@ -24,12 +37,73 @@ namespace {
 constexpr int kLayoutInterleaved = 0;
 constexpr int kLayoutHalf = 1;
 
-// first and second chunk (of 8 values) of unit u of a head with ru rotated units
-template <int LAYOUT>
-__device__ __forceinline__ void unit_chunks(int u, int ru, int* c0, int* c1) {
+struct Piece {
+  int at, n, skip;  // n <= 8 values from `at` on; the first `skip` are an earlier piece's too
+};
+
+// the piece that starts at `at` in the region [lo, hi), moved back into it
+__device__ __forceinline__ Piece piece_in(int at, int lo, int hi) {
+  const int start = hi - lo < 8 ? lo : at < hi - 8 ? at : hi - 8;
+  return {start, hi - lo < 8 ? hi - lo : 8, at - start};
+}
+
+// both pieces of unit u of a head of D values, rd of them rotated
+template <int LAYOUT, bool WHOLE>
+__device__ __forceinline__ void unit_pieces(int u, int rd, int D, Piece* a, Piece* b) {
+  const int ru = WHOLE ? rd >> 4 : (rd + 15) >> 4;
   const bool half = LAYOUT == kLayoutHalf && u < ru;
-  *c0 = half ? u : 2 * u;
-  *c1 = half ? u + ru : 2 * u + 1;
+  if constexpr (WHOLE) {
+    *a = {half ? 8 * u : 16 * u, 8, 0};
+    *b = {half ? 8 * u + (rd >> 1) : 16 * u + 8, 8, 0};
+  } else if (half) {
+    *a = *b = piece_in(8 * u, 0, rd >> 1);
+    b->at += rd >> 1;
+  } else {
+    const int lo = u < ru ? 0 : rd, hi = u < ru ? rd : D, at = u < ru ? 16 * u : rd + 16 * (u - ru);
+    *a = piece_in(at, lo, hi);
+    *b = piece_in(at + 8, lo, hi);
+  }
+}
+
+template <bool WHOLE>
+__device__ __forceinline__ u32x4 load_piece(const uint16_t* p, int n) {
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if constexpr (WHOLE) return ldg128(p);
+  else if (n == 8) __builtin_memcpy(&v, p, 16);
+  else {
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < n) v[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+  }
+  return v;
+}
+
+template <bool WHOLE>
+__device__ __forceinline__ void store_piece(uint16_t* p, int n, const u32x4& v) {
+  if constexpr (WHOLE) *reinterpret_cast<u32x4*>(p) = v;
+  else if (n == 8) __builtin_memcpy(p, &v, 16);
+  else {
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < n) p[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
+// N fp32 values, n of them there (0 where the others are)
+template <bool WHOLE, int N>
+__device__ __forceinline__ void load_floats(const float* p, int n, float* v) {
+  if constexpr (WHOLE) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+      const u32x4 a = ldg128(p + e);
+      __builtin_memcpy(v + e, &a, 16);
+    }
+  } else if (n == N) {
+    __builtin_memcpy(v, p, 4 * N);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = e < n ? p[e] : 0.0f;
+  }
 }
 
 template <typename T>
@@ -52,15 +126,20 @@ __device__ __forceinline__ void pack16(const float (&v)[16], u32x4* a, u32x4* b)
   }
 }
 
-// the 8 pairs of a unit, with the 8 angles from cr and sr on
-template <int LAYOUT>
-__device__ __forceinline__ void rotate16(float (&v)[16], const float* cr, const float* sr) {
+// the 8 pairs of a rotated unit by the angles of the rows cr and sr
+template <int LAYOUT, bool WHOLE>
+__device__ __forceinline__ void rotate16(float (&v)[16], const Piece& pa, const Piece& pb, const float* cr,
+                                         const float* sr) {
   float c[8], s[8];
-  const u32x4 c0 = ldg128(cr), c1 = ldg128(cr + 4), s0 = ldg128(sr), s1 = ldg128(sr + 4);
-  __builtin_memcpy(c, &c0, 16);
-  __builtin_memcpy(c + 4, &c1, 16);
-  __builtin_memcpy(s, &s0, 16);
-  __builtin_memcpy(s + 4, &s1, 16);
+  if constexpr (LAYOUT == kLayoutHalf) {
+    load_floats<WHOLE, 8>(cr + pa.at, pa.n, c);
+    load_floats<WHOLE, 8>(sr + pa.at, pa.n, s);
+  } else {
+    load_floats<WHOLE, 4>(cr + (pa.at >> 1), pa.n >> 1, c);
+    load_floats<WHOLE, 4>(cr + (pb.at >> 1), pb.n >> 1, c + 4);
+    load_floats<WHOLE, 4>(sr + (pa.at >> 1), pa.n >> 1, s);
+    load_floats<WHOLE, 4>(sr + (pb.at >> 1), pb.n >> 1, s + 4);
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int a = LAYOUT == kLayoutHalf ? i : 2 * i;
@@ -72,20 +151,7 @@ __device__ __forceinline__ void rotate16(float (&v)[16], const float* cr, const 
   }
 }
 
-// value i of a rotated head, from its source values f(0 .. D-1)
-template <int LAYOUT, typename F>
-__device__ __forceinline__ float rotated_value(int i, int rd, const float* cr, const float* sr, F f) {
-  if (i >= rd) return f(i);
-  const int half = rd >> 1;
-  const int j = LAYOUT == kLayoutHalf ? (i < half ? i : i - half) : i >> 1;
-  const int a = LAYOUT == kLayoutHalf ? j : 2 * j;
-  const int b = LAYOUT == kLayoutHalf ? j + half : 2 * j + 1;
-  float ya, yb;
-  rope_pair(f(a), f(b), cr[j], sr[j], &ya, &yb);
-  return i == a ? ya : yb;
-}
-
-// where the token of row (b, s) stands: offset + s, pos[b] + s or pos[b, s];
+// where the token of row (b, s) stands: offset + s, pos[b] + offset + s or pos[b, s];
 // -1 (a row of zeros) for negative entries and positions outside the tables
 constexpr int kPosOffset = 0, kPosFirst = 1, kPosEach = 2;
 __device__ __forceinline__ int64_t row_position(const int32_t* pos, int mode, int64_t offset, int64_t b, int64_t s,
@@ -93,72 +159,45 @@ __device__ __forceinline__ int64_t row_position(const int32_t* pos, int mode, in
   int64_t p = offset + s;
   if (mode != kPosOffset) {
     p = pos[mode == kPosFirst ? b : b * S + s];
-    if (p >= 0 && mode == kPosFirst) p += s;
+    if (p >= 0 && mode == kPosFirst) p += offset + s;
   }
   return p < 0 || p >= rows ? -1 : p;
 }
 
 struct RopeDims {
-  int64_t S, H, sb, ss, sh, rows, offset;  // strides of x in values; its last dimension is dense
-  int D, rd, mode;
+  int64_t S, sb, ss, sh, rows, offset;  // strides of x in values; its last dimension is dense
+  int H, D, rd, mode;
 };
 
-// a unit per thread; units < 2^31
-template <typename T, int LAYOUT>
-__global__ __launch_bounds__(256) void rope_vec_kernel(const T* __restrict__ x, const float* __restrict__ cos_t,
-                                                       const float* __restrict__ sin_t,
-                                                       const int32_t* __restrict__ pos, T* __restrict__ y,
-                                                       uint32_t units, RopeDims d) {
+// a unit per thread, upr of them a head
+template <typename T, int LAYOUT, bool WHOLE>
+__global__ __launch_bounds__(256) void rope_kernel(const T* __restrict__ x, const float* __restrict__ cos_t,
+                                                   const float* __restrict__ sin_t, const int32_t* __restrict__ pos,
+                                                   T* __restrict__ y, uint32_t units, uint32_t upr, RopeDims d) {
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   if (i >= units) return;
-  const uint32_t upr = (uint32_t)d.D >> 4;
-  const int ru = d.rd >> 4;
   const uint32_t row = i / upr, t = row / (uint32_t)d.H, b = t / (uint32_t)d.S;
   const int u = (int)(i - row * upr);
   const uint32_t h = row - t * (uint32_t)d.H, s = t - b * (uint32_t)d.S;
-  int c0, c1;
-  unit_chunks<LAYOUT>(u, ru, &c0, &c1);
-  const T* xr = x + (int64_t)b * d.sb + (int64_t)s * d.ss + (int64_t)h * d.sh;
-  const u32x4 x0 = ldg128(xr + 8 * c0), x1 = ldg128(xr + 8 * c1);
+  Piece pa, pb;
+  unit_pieces<LAYOUT, WHOLE>(u, d.rd, d.D, &pa, &pb);
+  const uint16_t* xr = reinterpret_cast<const uint16_t*>(x) + (int64_t)b * d.sb + (int64_t)s * d.ss + (int64_t)h * d.sh;
+  const u32x4 x0 = load_piece<WHOLE>(xr + pa.at, pa.n), x1 = load_piece<WHOLE>(xr + pb.at, pb.n);
   const int64_t p = row_position(pos, d.mode, d.offset, b, s, d.S, d.rows);
   u32x4 y0 = {0u, 0u, 0u, 0u}, y1 = {0u, 0u, 0u, 0u};
   if (p >= 0) {
     y0 = x0;
     y1 = x1;
-    if (u < ru) {
+    if (16 * u < d.rd) {
       float v[16];
       unpack16<T>(x0, x1, v);
-      const size_t at = (size_t)p * (d.rd >> 1) + 8 * u;
-      rotate16<LAYOUT>(v, cos_t + at, sin_t + at);
+      rotate16<LAYOUT, WHOLE>(v, pa, pb, cos_t + (size_t)p * (d.rd >> 1), sin_t + (size_t)p * (d.rd >> 1));
       pack16<T>(v, &y0, &y1);
     }
   }
-  T* yr = y + (size_t)row * d.D;
-  *reinterpret_cast<u32x4*>(yr + 8 * c0) = y0;
-  *reinterpret_cast<u32x4*>(yr + 8 * c1) = y1;
-}
-
-// any sizes and alignment: a wave per head
-template <typename T, int LAYOUT>
-__global__ __launch_bounds__(256) void rope_any_kernel(const T* __restrict__ x, const float* __restrict__ cos_t,
-                                                       const float* __restrict__ sin_t,
-                                                       const int32_t* __restrict__ pos, T* __restrict__ y,
-                                                       int64_t heads, RopeDims d) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t row = blockIdx.x * 4ll + (threadIdx.x >> 6); row < heads; row += gridDim.x * 4ll) {
-    const int64_t t = row / d.H, b = t / d.S;
-    const int64_t h = row - t * d.H, s = t - b * d.S;
-    const T* xr = x + b * d.sb + s * d.ss + h * d.sh;
-    T* yr = y + row * d.D;
-    const int64_t p = row_position(pos, d.mode, d.offset, b, s, d.S, d.rows);
-    const float* cr = cos_t + (p < 0 ? 0 : p) * (d.rd >> 1);
-    const float* sr = sin_t + (p < 0 ? 0 : p) * (d.rd >> 1);
-    for (int i = lane; i < d.D; i += MK_WAVE) {
-      if (p < 0) yr[i] = from_f32<T>(0.0f);
-      else if (i >= d.rd) yr[i] = xr[i];
-      else yr[i] = from_f32<T>(rotated_value<LAYOUT>(i, d.rd, cr, sr, [&](int j) { return to_f32(xr[j]); }));
-    }
-  }
+  uint16_t* yr = reinterpret_cast<uint16_t*>(y) + (size_t)row * d.D;
+  store_piece<WHOLE>(yr + pa.at, pa.n, y0);
+  store_piece<WHOLE>(yr + pb.at, pb.n, y1);
 }
 
 // ---------------------------------------------------------------------------
@@ -171,26 +210,17 @@ struct QkDims {
   float eps;
 };
 
-__device__ __forceinline__ float norm_weight(const void* w, int wdt, int i) {
-  if (wdt == MK_DT_F16) return to_f32(reinterpret_cast<const f16*>(w)[i]);
-  if (wdt == MK_DT_BF16) return to_f32(reinterpret_cast<const bf16*>(w)[i]);
-  return reinterpret_cast<const float*>(w)[i];
-}
-
-// norm weights of a unit's two chunks, 16-byte loads
-__device__ __forceinline__ void norm_weights16(const void* w, int wdt, int c0, int c1, float (&v)[16]) {
+// norm weights of a unit's two pieces
+template <bool WHOLE>
+__device__ __forceinline__ void norm_weights16(const void* w, int wdt, const Piece& pa, const Piece& pb,
+                                               float (&v)[16]) {
   if (wdt == MK_DT_F32) {
-    const float* p = reinterpret_cast<const float*>(w);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const u32x4 a = ldg128(p + 8 * (h ? c1 : c0)), b = ldg128(p + 8 * (h ? c1 : c0) + 4);
-      __builtin_memcpy(v + 8 * h, &a, 16);
-      __builtin_memcpy(v + 8 * h + 4, &b, 16);
-    }
+    load_floats<WHOLE, 8>(reinterpret_cast<const float*>(w) + pa.at, pa.n, v);
+    load_floats<WHOLE, 8>(reinterpret_cast<const float*>(w) + pb.at, pb.n, v + 8);
     return;
   }
-  const u32x4 a = ldg128(reinterpret_cast<const uint16_t*>(w) + 8 * c0);
-  const u32x4 b = ldg128(reinterpret_cast<const uint16_t*>(w) + 8 * c1);
+  const u32x4 a = load_piece<WHOLE>(reinterpret_cast<const uint16_t*>(w) + pa.at, pa.n);
+  const u32x4 b = load_piece<WHOLE>(reinterpret_cast<const uint16_t*>(w) + pb.at, pb.n);
   if (wdt == MK_DT_F16) unpack16<f16>(a, b, v);
   else unpack16<bf16>(a, b, v);
 }
@@ -221,118 +251,103 @@ __device__ __forceinline__ int64_t token_write_slot(const int32_t* pos, const in
 }
 
 // A workgroup has 128 lanes of one token's heads (q heads, then k, then v),
-// 1 << lgl lanes a head, of which D / 16 hold a unit each.
-template <typename T, int LAYOUT>
-__global__ __launch_bounds__(128) void qk_norm_rope_vec_kernel(
+// 1 << lgl <= 64 lanes a head, each with its units u, u + (1 << lgl), ...  The
+// first one stays in registers between the sum of squares and the rotation;
+// with over 64 units in a head the others are read twice.
+template <typename T, int LAYOUT, bool WHOLE>
+__global__ __launch_bounds__(128) void qk_norm_rope_kernel(
     const T* __restrict__ qkv, const void* __restrict__ qw, const void* __restrict__ kw,
     const float* __restrict__ cos_t, const float* __restrict__ sin_t, const int32_t* __restrict__ pos,
     const int32_t* __restrict__ seq, const int32_t* __restrict__ bt, T* __restrict__ Kp, T* __restrict__ Vp,
     T* __restrict__ q_out, int lgl, QkDims d) {
   const int t = blockIdx.x;
   const int at = (int)blockIdx.y * 128 + (int)threadIdx.x;
-  const int head = at >> lgl, u = at & ((1 << lgl) - 1);
-  const int ru = d.rd >> 4;
-  const bool has = head < d.Hq + 2 * d.Hkv && u < (d.D >> 4);
+  const int head = at >> lgl, u0 = at & ((1 << lgl) - 1);
   const bool is_q = head < d.Hq, is_v = head >= d.Hq + d.Hkv;
-  int c0, c1;
-  unit_chunks<LAYOUT>(u, is_v ? 0 : ru, &c0, &c1);
+  const int rd = is_v ? 0 : d.rd;
+  const int units = WHOLE ? d.D >> 4 : ((rd + 15) >> 4) + ((d.D - rd + 15) >> 4);
+  const bool has = head < d.Hq + 2 * d.Hkv && u0 < units;
+  const uint16_t* xr = reinterpret_cast<const uint16_t*>(qkv) + t * d.row_stride + (int64_t)head * d.D;
+  Piece pa, pb;
+  unit_pieces<LAYOUT, WHOLE>(u0, rd, d.D, &pa, &pb);
   u32x4 x0 = {0u, 0u, 0u, 0u}, x1 = {0u, 0u, 0u, 0u};
   if (has) {
-    const T* xr = qkv + t * d.row_stride + (int64_t)head * d.D;
-    x0 = ldg128(xr + 8 * c0);
-    x1 = ldg128(xr + 8 * c1);
+    x0 = load_piece<WHOLE>(xr + pa.at, pa.n);
+    x1 = load_piece<WHOLE>(xr + pb.at, pb.n);
   }
   const int64_t p = pos[t];
   const bool live = p >= 0 && p < d.rows && (!seq || (seq[t] >= 0 && seq[t] < d.B));
   int64_t slot = -1;
   // (the last lane's head says whether the workgroup has any to write to the cache)
   if (live && (((int)blockIdx.y * 128 + 127) >> lgl) >= d.Hq) slot = token_write_slot(pos, seq, bt, d, t);
-  if (live && !is_v) {
-    float v[16];
-    unpack16<T>(x0, x1, v);
-    const void* w = is_q ? qw : kw;
-    if (qw != nullptr) {
-      float ss = 0.0f;
+  const bool norm = qw != nullptr && live && !is_v;
+  float inv = 1.0f;
+  if (norm) {
+    float v[16], ss = 0.0f;
+    auto add = [&]() {  // the values of x0 and x1 that no earlier unit has (those past a piece's end are 0)
+      unpack16<T>(x0, x1, v);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ss += v[e] * v[e];
-      for (int o = 0; o < lgl; ++o) ss += __shfl_xor(ss, 1 << o, MK_WAVE);
-      const float inv = rsqrtf(ss / (float)d.D + d.eps);
+      for (int e = 0; e < 8; ++e) {
+        if (WHOLE || e >= pa.skip) ss += v[e] * v[e];
+        if (WHOLE || e >= pb.skip) ss += v[8 + e] * v[8 + e];
+      }
+    };
+    add();
+    if (units > MK_WAVE) {
+      for (int u = u0 + MK_WAVE; has && u < units; u += MK_WAVE) {
+        unit_pieces<LAYOUT, WHOLE>(u, rd, d.D, &pa, &pb);
+        x0 = load_piece<WHOLE>(xr + pa.at, pa.n);
+        x1 = load_piece<WHOLE>(xr + pb.at, pb.n);
+        add();
+      }
       if (has) {
+        unit_pieces<LAYOUT, WHOLE>(u0, rd, d.D, &pa, &pb);
+        x0 = load_piece<WHOLE>(xr + pa.at, pa.n);
+        x1 = load_piece<WHOLE>(xr + pb.at, pb.n);
+      }
+    }
+    for (int o = 0; o < lgl; ++o) ss += __shfl_xor(ss, 1 << o, MK_WAVE);
+    inv = rsqrtf(ss / (float)d.D + d.eps);
+  }
+  if (!has || (!is_q && slot < 0)) return;
+  uint16_t* out = reinterpret_cast<uint16_t*>(is_q ? q_out : is_v ? Vp : Kp);
+  if (is_q) out += ((size_t)t * d.Hq + head) * d.D;
+  else out += ((size_t)slot * d.Hkv + (head - d.Hq - (is_v ? d.Hkv : 0))) * d.D;
+  for (int u = u0;;) {
+    if (!live) x0 = x1 = u32x4{0u, 0u, 0u, 0u};
+    else if (norm || 16 * u < rd) {
+      float v[16];
+      unpack16<T>(x0, x1, v);
+      if (norm) {
         float wv[16];
-        norm_weights16(w, d.wdt, c0, c1, wv);
+        norm_weights16<WHOLE>(is_q ? qw : kw, d.wdt, pa, pb, wv);
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = v[e] * inv * wv[e];
       }
+      if (16 * u < rd)
+        rotate16<LAYOUT, WHOLE>(v, pa, pb, cos_t + (size_t)p * (d.rd >> 1), sin_t + (size_t)p * (d.rd >> 1));
+      pack16<T>(v, &x0, &x1);
     }
-    if (has && u < ru) {
-      const size_t a = (size_t)p * (d.rd >> 1) + 8 * u;
-      rotate16<LAYOUT>(v, cos_t + a, sin_t + a);
-    }
-    if (qw != nullptr || u < ru) pack16<T>(v, &x0, &x1);
+    store_piece<WHOLE>(out + pa.at, pa.n, x0);
+    store_piece<WHOLE>(out + pb.at, pb.n, x1);
+    u += MK_WAVE;
+    if (u >= units) return;
+    unit_pieces<LAYOUT, WHOLE>(u, rd, d.D, &pa, &pb);
+    x0 = load_piece<WHOLE>(xr + pa.at, pa.n);
+    x1 = load_piece<WHOLE>(xr + pb.at, pb.n);
   }
-  if (!has) return;
-  T* out;
-  if (is_q) {
-    if (!live) x0 = x1 = u32x4{0u, 0u, 0u, 0u};
-    out = q_out + ((size_t)t * d.Hq + head) * d.D;
-  } else {
-    if (slot < 0) return;
-    out = (is_v ? Vp : Kp) + ((size_t)slot * d.Hkv + (head - d.Hq - (is_v ? d.Hkv : 0))) * d.D;
-  }
-  *reinterpret_cast<u32x4*>(out + 8 * c0) = x0;
-  *reinterpret_cast<u32x4*>(out + 8 * c1) = x1;
 }
 
-// any sizes and alignment: a wave per head, four heads of a token a workgroup
-template <typename T, int LAYOUT>
-__global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(
-    const T* __restrict__ qkv, const void* __restrict__ qw, const void* __restrict__ kw,
-    const float* __restrict__ cos_t, const float* __restrict__ sin_t, const int32_t* __restrict__ pos,
-    const int32_t* __restrict__ seq, const int32_t* __restrict__ bt, T* __restrict__ Kp, T* __restrict__ Vp,
-    T* __restrict__ q_out, QkDims d) {
-  const int t = blockIdx.x, lane = threadIdx.x & 63;
-  const int head = (int)blockIdx.y * 4 + ((int)threadIdx.x >> 6);
-  const int64_t p = pos[t];
-  const bool live = p >= 0 && p < d.rows && (!seq || (seq[t] >= 0 && seq[t] < d.B));
-  int64_t slot = -1;
-  if (live && (int)blockIdx.y * 4 + 3 >= d.Hq) slot = token_write_slot(pos, seq, bt, d, t);
-  if (head >= d.Hq + 2 * d.Hkv) return;
-  const bool is_q = head < d.Hq, is_v = head >= d.Hq + d.Hkv;
-  const T* xr = qkv + t * d.row_stride + (int64_t)head * d.D;
-  T* out = nullptr;
-  if (is_q) out = q_out + ((size_t)t * d.Hq + head) * d.D;
-  else if (slot >= 0) out = (is_v ? Vp : Kp) + ((size_t)slot * d.Hkv + (head - d.Hq - (is_v ? d.Hkv : 0))) * d.D;
-  if (!out) return;
-  if (!live || is_v) {
-    for (int i = lane; i < d.D; i += MK_WAVE) out[i] = live ? xr[i] : from_f32<T>(0.0f);
-    return;
-  }
-  const void* w = is_q ? qw : kw;
-  float inv = 1.0f;
-  if (w) {
-    float ss = 0.0f;
-    for (int i = lane; i < d.D; i += MK_WAVE) {
-      const float v = to_f32(xr[i]);
-      ss += v * v;
-    }
-    inv = rsqrtf(wave_sum(ss) / (float)d.D + d.eps);
-  }
-  const float* cr = cos_t + (size_t)p * (d.rd >> 1);
-  const float* sr = sin_t + (size_t)p * (d.rd >> 1);
-  auto value = [&](int i) {
-    const float v = to_f32(xr[i]);
-    return w ? v * inv * norm_weight(w, d.wdt, i) : v;
-  };
-  for (int i = lane; i < d.D; i += MK_WAVE) out[i] = from_f32<T>(rotated_value<LAYOUT>(i, d.rd, cr, sr, value));
-}
+// units of a head
+int64_t units_of(int64_t D, int64_t rd) { return (rd + 15) / 16 + (D - rd + 15) / 16; }
 
-// a call of the kernel for the storage type and the layout
-#define MK_ROPE_LAUNCH(KERNEL)                                                        \
+// a call of the kernel for the storage type, the layout and whole or other units
+#define MK_ROPE_LAUNCH(KERNEL, W)                                                     \
   do {                                                                                \
-    if (dtype == MK_DT_F16 && layout == kLayoutHalf) KERNEL(f16, kLayoutHalf);        \
-    else if (dtype == MK_DT_F16) KERNEL(f16, kLayoutInterleaved);                     \
-    else if (layout == kLayoutHalf) KERNEL(bf16, kLayoutHalf);                        \
-    else KERNEL(bf16, kLayoutInterleaved);                                            \
+    if (dtype == MK_DT_F16 && layout == kLayoutHalf) KERNEL(f16, kLayoutHalf, W);     \
+    else if (dtype == MK_DT_F16) KERNEL(f16, kLayoutInterleaved, W);                  \
+    else if (layout == kLayoutHalf) KERNEL(bf16, kLayoutHalf, W);                     \
+    else KERNEL(bf16, kLayoutInterleaved, W);                                         \
   } while (0)
 
 }  // namespace
@@ -351,28 +366,33 @@ int mk_apply_rope(const void* x, const float* cos_t, const float* sin_t, const i
   MK_REQUIRE(B < (1LL << 31) && S < (1LL << 31) && H < (1LL << 20) && B * S < (1LL << 40));
   if (B == 0 || S == 0 || H == 0) return MK_OK;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const int64_t heads = B * S * H;
-  const RopeDims d = {S, H, stride_b, stride_s, stride_h, cos_rows, position_offset, (int)D, (int)rotary_dim,
-                      positions ? (per_token ? kPosEach : kPosFirst) : kPosOffset};
-  // whole units, 16-byte chunks at 16-byte addresses, unit numbers in 32 bits
-  const bool vec = D % 16 == 0 && rotary_dim % 16 == 0 && stride_b % 8 == 0 && stride_s % 8 == 0 &&
-                   stride_h % 8 == 0 && heads < (1LL << 31) / (D / 16) && mk_aligned(x, 16) && mk_aligned(y, 16) &&
-                   mk_aligned(cos_t, 16) && mk_aligned(sin_t, 16);
-  if (vec) {
-    const uint32_t units = (uint32_t)(heads * (D / 16));
-#define MK_RV(T, L)                                                                                             \
-  rope_vec_kernel<T, L><<<(units + 255) / 256, 256, 0, st>>>((const T*)x, cos_t, sin_t, positions, (T*)y, units, d)
-    MK_ROPE_LAUNCH(MK_RV);
-#undef MK_RV
-  } else {
-    const int64_t want = (heads + 3) / 4;
-    const unsigned blocks = (unsigned)(want < 65536 ? want : 65536);
-#define MK_RA(T, L) \
-  rope_any_kernel<T, L><<<blocks, 256, 0, st>>>((const T*)x, cos_t, sin_t, positions, (T*)y, heads, d)
-    MK_ROPE_LAUNCH(MK_RA);
-#undef MK_RA
+  const int64_t upr = units_of(D, rotary_dim), token = H * upr;
+  MK_REQUIRE(token < (1LL << 31));
+  // whole units, 16-byte pieces at 16-byte addresses
+  const bool whole = D % 16 == 0 && rotary_dim % 16 == 0 && stride_b % 8 == 0 && stride_s % 8 == 0 &&
+                     stride_h % 8 == 0 && mk_aligned(x, 16) && mk_aligned(y, 16) && mk_aligned(cos_t, 16) &&
+                     mk_aligned(sin_t, 16);
+  // unit numbers fit in 31 bits: a launch for whole sequences or, of longer ones, for some rows of one
+  const int64_t most = ((1LL << 31) - 1) / token;
+  const int64_t nb = S <= most ? most / S : 1, ns = S <= most ? S : most;
+  for (int64_t b0 = 0; b0 < B; b0 += nb) {
+    for (int64_t s0 = 0; s0 < S; s0 += ns) {
+      const int64_t b = B - b0 < nb ? B - b0 : nb, s = S - s0 < ns ? S - s0 : ns;
+      const RopeDims d = {s, stride_b, stride_s, stride_h, cos_rows, (positions ? 0 : position_offset) + s0, (int)H,
+                          (int)D, (int)rotary_dim, positions ? (per_token ? kPosEach : kPosFirst) : kPosOffset};
+      const uint16_t* xs = (const uint16_t*)x + b0 * stride_b + s0 * stride_s;
+      uint16_t* ys = (uint16_t*)y + (b0 * S + s0) * H * D;
+      const int32_t* ps = positions ? positions + (per_token ? b0 * S + s0 : b0) : nullptr;
+      const uint32_t units = (uint32_t)(b * s * token);
+#define MK_R(T, L, W)                                                                                       \
+  rope_kernel<T, L, W><<<(units + 255) / 256, 256, 0, st>>>((const T*)xs, cos_t, sin_t, ps, (T*)ys, units, \
+                                                            (uint32_t)upr, d)
+      if (whole) MK_ROPE_LAUNCH(MK_R, true);
+      else MK_ROPE_LAUNCH(MK_R, false);
+#undef MK_R
+      MK_CHECK_LAUNCH();
+    }
   }
-  MK_CHECK_LAUNCH();
   return MK_OK;
 }
 
@@ -398,28 +418,22 @@ int mk_qk_norm_rope_paged_update(const void* qkv, int64_t row_stride, const void
   const QkDims d = {row_stride, page_size, max_blocks, num_pages, cos_rows, (int)T, (int)B, (int)Hq, (int)Hkv,
                     (int)D, (int)rotary_dim, weight_dtype, eps};
   const int64_t heads = Hq + 2 * Hkv;
-  // a head's units on at most one wave's lanes
-  const bool vec = D % 16 == 0 && D <= 16 * MK_WAVE && rotary_dim % 16 == 0 && row_stride % 8 == 0 &&
-                   mk_aligned(qkv, 16) && mk_aligned(q_out, 16) && mk_aligned(K_pages, 16) &&
-                   mk_aligned(V_pages, 16) && mk_aligned(cos_t, 16) && mk_aligned(sin_t, 16) &&
-                   mk_aligned(q_weight, 16) && mk_aligned(k_weight, 16);
+  const bool whole = D % 16 == 0 && rotary_dim % 16 == 0 && row_stride % 8 == 0 && mk_aligned(qkv, 16) &&
+                     mk_aligned(q_out, 16) && mk_aligned(K_pages, 16) && mk_aligned(V_pages, 16) &&
+                     mk_aligned(cos_t, 16) && mk_aligned(sin_t, 16) && mk_aligned(q_weight, 16) &&
+                     mk_aligned(k_weight, 16);
   int lgl = 0;
-  while (vec && (16 << lgl) < D) ++lgl;
-  const int64_t gy = vec ? ((heads << lgl) + 127) / 128 : (heads + 3) / 4;
+  while ((1 << lgl) < MK_WAVE && (1 << lgl) < units_of(D, rotary_dim)) ++lgl;
+  const int64_t gy = ((heads << lgl) + 127) / 128;
   MK_REQUIRE(gy < 65536);
   const dim3 grid((unsigned)T, (unsigned)gy);
-#define MK_QV(TT, L)                                                                                              \
-  qk_norm_rope_vec_kernel<TT, L><<<grid, 128, 0, st>>>((const TT*)qkv, q_weight, k_weight, cos_t, sin_t, positions, \
-                                                       sequences, block_table, (TT*)K_pages, (TT*)V_pages,         \
-                                                       (TT*)q_out, lgl, d)
-#define MK_QA(TT, L)                                                                                              \
-  qk_norm_rope_any_kernel<TT, L><<<grid, 256, 0, st>>>((const TT*)qkv, q_weight, k_weight, cos_t, sin_t, positions, \
-                                                       sequences, block_table, (TT*)K_pages, (TT*)V_pages,         \
-                                                       (TT*)q_out, d)
-  if (vec) MK_ROPE_LAUNCH(MK_QV);
-  else MK_ROPE_LAUNCH(MK_QA);
-#undef MK_QV
-#undef MK_QA
+#define MK_Q(TT, L, W)                                                                                              \
+  qk_norm_rope_kernel<TT, L, W><<<grid, 128, 0, st>>>((const TT*)qkv, q_weight, k_weight, cos_t, sin_t, positions, \
+                                                      sequences, block_table, (TT*)K_pages, (TT*)V_pages,          \
+                                                      (TT*)q_out, lgl, d)
+  if (whole) MK_ROPE_LAUNCH(MK_Q, true);
+  else MK_ROPE_LAUNCH(MK_Q, false);
+#undef MK_Q
   MK_CHECK_LAUNCH();
   return MK_OK;
 }

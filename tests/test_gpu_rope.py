@@ -213,3 +213,45 @@ def test_qk_stream_and_graph(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip((*eager, Ke, Ve), (*out, Kg, Vg))), i
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_every_size(dev, layout):
+    """Every part of heads of 2 .. 40 values and some larger ones, from addresses of 2 bytes: pieces that overlap, regions
+    of fewer values than a piece, heads that begin anywhere; the norms' sums count every value once."""
+    g = torch.Generator().manual_seed(21)
+    for D in [*range(2, 41), 90, 120, 250]:
+        flat = torch.randn(6 * 3 * D + 1, generator=g).half().to(dev)
+        x = flat[1:].view(2, 3, 3, D)
+        for rd in sorted({2, D // 4 * 2, *range(2, min(D, 40) + 1, 4 if D % 4 else 2), D // 2 * 2} - {0}):
+            cos, sin = (torch.randn(9, rd // 2, generator=g).to(dev) for _ in range(2))
+            got = rope.apply_rope(x, cos, sin, 2, layout=layout, rotary_dim=rd)
+            check_rope(x, cos, sin, np.broadcast_to(2 + np.arange(3), (2, 3)), layout, rd, got)
+            if D % 2:
+                continue  # (heads with a cache are even)
+            case = qk_case(D + rd, 2, 2, 2, 1, D, rd, 2, 3, torch.float16, True)
+            qkv, K, V, bt, c, s, pos, kw = case
+            wide = torch.zeros(2, 4 * D + 1, dtype=torch.float16, device=dev)
+            wide[:, 1:] = qkv.to(dev)
+            out = gqa.paged_qk_norm_rope_update(
+                wide[:, 1:], K.to(dev), V.to(dev), bt.to(dev), c.to(dev), s.to(dev), pos.to(dev), layout=layout,
+                **{k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in kw.items()})
+            check_qk(out, case, torch.float16, layout)
+
+
+@pytest.mark.parametrize("B,S,H", [(3, 2 ** 30 - 5, 2), (1, 2 ** 30 + 9, 4)])
+def test_rope_long(dev, B, S, H):
+    """More units of work than a launch numbers: sequences, and parts of one, in launches of their own.  Only rows of
+    position 0 .. 9 are inside of the tables, which are asked for at both sides of each seam."""
+    g = torch.Generator().manual_seed(B)
+    x = torch.randn(1, 1, H, 2, generator=g).half().to(dev).expand(B, S, H, 2)
+    cos, sin = torch.randn(10, 1, generator=g).to(dev), torch.randn(10, 1, generator=g).to(dev)
+    for at in ([0, 2 ** 29 - 6, S - 10] if B == 1 else [0, S - 10]):
+        pos = torch.full((B, S), -1, dtype=torch.int32, device=dev)
+        pos[:, at:at + 10] = torch.arange(10, dtype=torch.int32, device=dev)
+        got = rope.apply_rope(x, cos, sin, positions=pos, rotary_dim=2)
+        check_rope(x[:, :10].contiguous(), cos, sin, np.broadcast_to(np.arange(10), (B, 10)), "interleaved", 2,
+                   got[:, at:at + 10].contiguous())
+        live = sum(int((row != 0).any(-1).any(-1).sum()) for part in got.split(2 ** 26, 1) for row in part)
+        assert live == 10 * B
+        del got, pos
