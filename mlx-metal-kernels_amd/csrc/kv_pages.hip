@@ -134,7 +134,7 @@ __device__ __forceinline__ void add_count(int32_t* p, int v) {
 
 constexpr int kForkRows = 4096;  // rows of the new table
 // What one workgroup does with the counts in LDS: a step of 32 beams over 700
-// pages in 7 us (16.6 with counts in memory, whose atomics and reads go to the
+// pages in 11.9 us (16.6 with counts in memory, whose atomics and reads go to the
 // L2 one after another).  Beyond, launches over all CUs count the references.
 constexpr int kSmallPages = 8192, kSmallRows = 1024, kSmallNew = 2048, kSmallEntries = 1 << 16;
 
@@ -461,8 +461,8 @@ int mk_fork_kv_sequences(void* const* tensors, const int64_t* page_bytes, int64_
   for (int64_t i = 0; i < num_tensors; ++i) MK_REQUIRE(tensors[i] && page_bytes[i] >= 0);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const ForkArgs a = {block_table, lengths, ref_counts, parents, new_table, new_lengths, new_ref_counts, ready,
-                      workspace, workspace ? workspace + 2 * n + 1 : nullptr, B, max_blocks, num_pages, page_size, reserve,
-                      max_new, (int)n};
+                      workspace, workspace ? workspace + 2 * n + 1 : nullptr, B, max_blocks, num_pages, page_size,
+                      reserve, max_new, (int)n};
   if (num_pages <= kSmallPages && n <= kSmallRows && max_new <= kSmallNew && (B + n) * max_blocks <= kSmallEntries) {
     fork_small_kernel<<<1, 1024, 0, st>>>(a);
   } else {

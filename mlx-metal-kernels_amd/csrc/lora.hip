@@ -301,7 +301,9 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(Groups g
   const T* ai = a + (int64_t)adapter * R * K;
   t += (int64_t)blockIdx.y * gs.M * (16 * RT);
   shrink_group<T, RT, VEC>(x, x_stride, ai, K, R, k0, k1, n, rowlist, part,
-                           [&](int, int m, int r, const f32x4& s) {
+                           [&](int, int m, int r, f32x4 s) {
+#pragma unroll
+                             for (int e = 0; e < 4; ++e) s[e] = r + e < R ? s[e] : 0.0f;  // (0 x infinity behind R)
                              if (m >= 0) *reinterpret_cast<f32x4*>(t + (int64_t)m * (16 * RT) + r) = s;
                            });
 }
@@ -329,14 +331,14 @@ struct ExpandRows {
 
   // chunk c of row i, by CH lanes side by side, a power of two
   __device__ __forceinline__ void put(int i, int c, float (&v)[8], float back, bool live) {
-    if constexpr (__is_same(T, f16)) {  // the row's largest value to [2^13, 2^14)
+    if constexpr (__is_same(T, f16)) {  // the row's largest finite value to [2^13, 2^14)
       float top = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+      for (int e = 0; e < 8; ++e) top = fabsf(v[e]) < INFINITY ? fmaxf(top, fabsf(v[e])) : top;
 #pragma unroll
       for (int o = 1; o < CH; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, MK_WAVE));
       int e = 14;
-      if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
+      if (top > 0.0f) (void)frexpf(top, &e);
 #pragma unroll
       for (int q = 0; q < 8; ++q) v[q] = ldexpf(v[q], 14 - e);
       back = ldexpf(back, e - 14);

@@ -313,6 +313,8 @@ def _qk_norm_rope_prep(qkv, K_pages, V_pages, block_table, cos, sin, position, H
             raise TypeError("q_weight and k_weight must share a float16, bfloat16, or float32 dtype, got "
                             f"{q_weight.dtype}, {k_weight.dtype}")
     B = table[0]
+    if T >= (65536 if sequences is None else 2 ** 24):
+        raise ValueError(f"at most 65535 rows, 2^24 - 1 with sequences, got {T}")
     dev = block_table.device
     rows = min(rope[0], table[1] * pages[1])
     if isinstance(position, int):

@@ -87,8 +87,7 @@ def count_page_refs(block_table, num_pages: int):
 
 def copy_kv_pages(pages, src, dst, *, backend: str = "auto"):
     """Page src[i] onto page dst[i] in every array of ``pages``, in place;
-    returns ``pages``.  src, dst int32 [n] (device,
-    host or a list).  No page may be the destination of two pairs, or the
+    returns ``pages``.  src, dst int32 [n] (device, host or a list).  No page may be the destination of two pairs, or the
     source of one and the destination of another.  Entries are checked on the
     host unless that is off (``host_checks_enabled``); then pairs with an entry
     outside of the pages are skipped."""
@@ -120,7 +119,8 @@ def copy_kv_pages(pages, src, dst, *, backend: str = "auto"):
     if n and num_pages:
         src, dst = src.contiguous(), dst.contiguous()
         at, size = _addresses(pages, num_pages)
-        _lib.launch("mk_copy_kv_pages", dev, at.buffer_info()[0], size.buffer_info()[0], len(pages), src.data_ptr(), dst.data_ptr(), n, num_pages)
+        _lib.launch("mk_copy_kv_pages", dev, at.buffer_info()[0], size.buffer_info()[0], len(pages), src.data_ptr(),
+                    dst.data_ptr(), n, num_pages)
     return pages
 
 
@@ -213,10 +213,10 @@ def fork_kv_sequences(pages, block_table, lengths, ref_counts, parents, *, reser
     buf = torch.empty(n + ints, dtype=torch.int32, device=dev)  # the new lengths, then the workspace
     at, sizes = _addresses(pages, num_pages)
     base = buf.data_ptr()
-    _lib.launch("mk_fork_kv_sequences", dev, at.buffer_info()[0], sizes.buffer_info()[0], len(pages), table.data_ptr() or None, lengths.data_ptr() or None,
-                refs.data_ptr(), parents.data_ptr() or None, new_table.data_ptr() or None, base or None,
-                new_refs.data_ptr(), ready.data_ptr() or None, base + 4 * n if ints else None, ints, B, n, blocks,
-                size, num_pages, reserve)
+    _lib.launch("mk_fork_kv_sequences", dev, at.buffer_info()[0], sizes.buffer_info()[0], len(pages),
+                table.data_ptr() or None, lengths.data_ptr() or None, refs.data_ptr(), parents.data_ptr() or None,
+                new_table.data_ptr() or None, base or None, new_refs.data_ptr(), ready.data_ptr() or None,
+                base + 4 * n if ints else None, ints, B, n, blocks, size, num_pages, reserve)
     return new_table, buf[:n], new_refs, ready
 
 
@@ -305,7 +305,7 @@ def compact_kv_pages(pages, block_table, ref_counts, *, backend: str = "auto"):
     buf = torch.empty(2 + num_pages, dtype=torch.int32, device=dev)  # live and moved pages, then the workspace
     at, sizes = _addresses(pages, num_pages)
     base = buf.data_ptr()
-    _lib.launch("mk_compact_kv_pages", dev, at.buffer_info()[0], sizes.buffer_info()[0], len(pages), table.data_ptr() or None, refs.data_ptr(),
-                new_table.data_ptr() or None, new_refs.data_ptr(), page_map.data_ptr(), base, base + 8, num_pages,
-                table.numel(), num_pages)
+    _lib.launch("mk_compact_kv_pages", dev, at.buffer_info()[0], sizes.buffer_info()[0], len(pages),
+                table.data_ptr() or None, refs.data_ptr(), new_table.data_ptr() or None, new_refs.data_ptr(),
+                page_map.data_ptr(), base, base + 8, num_pages, table.numel(), num_pages)
     return new_table, new_refs, page_map, buf[:1]

@@ -21,6 +21,7 @@ from .kv_cache_ops import host_checks_enabled
 from .mlp_block_ops import quantized_linear
 
 MAX_RANK, MAX_ADAPTERS = 128, 4096
+MAX_ROWS, MAX_OUTPUTS = 2 ** 20 - 1, 2 ** 24 - 1
 
 
 @dataclass
@@ -123,7 +124,9 @@ def lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None, out=None, bac
     of the rows' shape, flat, or one for each sequence of [B,S,...] rows; -1 is
     a row without an adapter.  Both products are summed in fp32 and the result
     is rounded once.  ``out``: a tensor to write, ``base`` itself among them
-    (the rows may be strided; no other overlap).
+    (the rows may be strided; no other overlap).  At most 2^20 - 1 rows and
+    2^24 - 1 outputs.  An infinity in lora_b may come back as a NaN of its
+    outputs; one in x, base or lora_a is what the formula makes of it.
 
     ids are checked on the host unless that is off (``host_checks_enabled``);
     then one outside [0, ADAPTERS) is a row without an adapter.  Backend
@@ -137,6 +140,8 @@ def lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None, out=None, bac
         y = reference_lora_add(x, base, lora_a, lora_b, adapter_ids, scales=scales)
         return y if out is None else out.copy_(y)
     M, N, K, R, adapters, ids = _validate(x, base, lora_a, lora_b, adapter_ids, scales, out)
+    if M > MAX_ROWS or N > MAX_OUTPUTS:
+        raise ValueError(f"at most {MAX_ROWS} rows and {MAX_OUTPUTS} outputs, got {M}, {N}")
     dev = _lib.require_device(x, base, lora_a, lora_b, scales)
     x2, x_stride = _rows(x, K)
     if x2 is None:

@@ -162,3 +162,26 @@ def test_stream_and_graph(dev):
             g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(eager, outs)), i
+
+
+@pytest.mark.parametrize("M", [1, 5, 70])
+@pytest.mark.parametrize("R", [3, 12, 20, 40, 100])
+def test_infinity_in_a_row(dev, R, M):
+    """With positive adapters an infinity in a row gives infinities, whatever lies between the ranks and whole tiles."""
+    g = torch.Generator().manual_seed(R)
+    x, base = torch.rand(M, 40, generator=g).half(), torch.rand(M, 72, generator=g).half()
+    a, b = 0.1 + torch.rand(2, R, 40, generator=g).half(), 0.1 + torch.rand(2, 72, R, generator=g).half()
+    x[M // 2, 5] = float("inf")
+    got = lo.lora_add(*on(dev, x, base, a, b, torch.zeros(M, dtype=torch.int32))).cpu()
+    assert (got[M // 2] == float("inf")).all()
+    assert got[[m for m in range(M) if m != M // 2]].isfinite().all()
+
+
+@pytest.mark.parametrize("M", [1, 5, 70])
+def test_infinity_beside_large_sums(dev, M):
+    """An infinity of one rank leaves the others, above fp16's range, finite."""
+    x, base = torch.full((M, 40), 64.0).half(), torch.zeros(M, 64).half()
+    a, b = torch.full((1, 4, 40), 100.0).half(), torch.full((1, 64, 4), 2.0 ** -10).half()
+    a[0, 2, 7], b[0, 32:, 2] = float("inf"), 2.0 ** -5
+    got = lo.lora_add(*on(dev, x, base, a, b, torch.zeros(M, dtype=torch.int32))).cpu()
+    assert (got == float("inf")).all()

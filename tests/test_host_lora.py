@@ -101,3 +101,11 @@ def test_refusals():
             lo.lora_add(**{**ok, **kw})
     with pytest.raises(ValueError, match="ROCm device"):
         lo.lora_add(**{**ok, "backend": "auto"})
+
+
+def test_limits():
+    """More rows or outputs than a call takes are refused before anything is read."""
+    z = lambda *shape: torch.zeros(1, dtype=torch.float16).expand(*shape)  # noqa: E731
+    for M, N in ((lo.MAX_ROWS + 1, 1), (1, lo.MAX_OUTPUTS + 1)):
+        with pytest.raises(ValueError, match="at most"):
+            lo.lora_add(z(M, 1), z(M, N), z(1, 1, 1), z(1, N, 1), torch.zeros(M, dtype=torch.int32))

@@ -216,3 +216,14 @@ def test_qk_refusals():
         gqa.paged_qk_norm_rope_update(**{**ok, "backend": "auto", "qkv": qkv.clone().requires_grad_()})
     with pytest.raises(ValueError, match="ROCm device"):
         gqa.paged_qk_norm_rope_update(**{**ok, "backend": "auto"})
+
+
+@pytest.mark.parametrize("T,ragged", [(65536, False), (2 ** 24, True)])
+def test_qk_row_limits(T, ragged):
+    z = lambda *shape: torch.zeros(1, dtype=torch.float16).expand(*shape)  # noqa: E731
+    one = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="at most"):
+        gqa.paged_qk_norm_rope_update(z(T, 6), z(1, 1, 1, 2).contiguous(), z(1, 1, 1, 2).contiguous(),
+                                      one.expand(1 if ragged else T, 1), torch.ones(1, 1), torch.ones(1, 1),
+                                      one.expand(T), sequences=one.expand(T) if ragged else None,
+                                      num_attention_heads=1, num_key_value_heads=1, head_dim=2)
