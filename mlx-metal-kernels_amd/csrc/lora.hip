@@ -185,9 +185,10 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(const int32_t* __restr
 }
 
 // ---------------------------------------------------------------------------
-// t = A x: a workgroup of 8 waves has a group and a slice of K; its waves take
-// turns of 32 values of K and are summed through LDS.  The product is A (ranks
-// down) times x (rows across): a lane ends with 4 ranks of a row.
+// t = A x: a workgroup of 8 waves has a group, or half of one, and a slice of
+// K; its waves take turns of 32 values of K and are summed through LDS.  The
+// product is A (ranks down) times x (rows across): a lane ends with 4 ranks of
+// a row.
 // ---------------------------------------------------------------------------
 
 constexpr int kShrinkWaves = 8;
@@ -275,6 +276,7 @@ __device__ __forceinline__ void shrink_group(const T* x, int64_t x_stride, const
                                              Put put) {
   if constexpr (VEC) {
     if (n <= 16) shrink_rows<T, RT, 1, VEC>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
+    else if (n <= 32) shrink_rows<T, RT, 2, VEC>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
     else shrink_rows<T, RT, 4, VEC>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
   } else {  // values one by one: 16 rows at a time leave the registers for them
     for (int i = 0; i < n; i += 16) {
@@ -291,11 +293,17 @@ template <typename T, int RT, bool VEC>
 __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(Groups gs, const T* __restrict__ x,
                                                                         int64_t x_stride, const T* __restrict__ a,
                                                                         float* __restrict__ t, int64_t K, int R,
-                                                                        int64_t k_slice) {
+                                                                        int64_t k_slice, int rows) {
   __shared__ f32x4 part[kShrinkWaves][RT][64];
   int adapter, rowlist;
-  const int n = find_group(gs, (int)blockIdx.x, &adapter, &rowlist);
-  if (n == 0 || adapter < 0) return;
+  const int parts = kGroupRows / rows, r0 = (int)blockIdx.x % parts * rows;
+  int n = find_group(gs, (int)blockIdx.x / parts, &adapter, &rowlist);
+  if (n <= r0 || adapter < 0) return;
+  if (r0 > 0 || n > rows) {
+    n = n - r0 < rows ? n - r0 : rows;
+    const int lane = (int)threadIdx.x & 63, row = __shfl(rowlist, (r0 + lane) & 63, MK_WAVE);
+    rowlist = lane < n ? row : -1;
+  }
   const int64_t k0 = (int64_t)blockIdx.y * k_slice;
   const int64_t k1 = k0 + k_slice < K ? k0 + k_slice : K;
   const T* ai = a + (int64_t)adapter * R * K;
@@ -614,7 +622,7 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(const int32_t*
 
 struct LoraPlan {
   int64_t groups, k_slice, order_ints;  // most groups that there can be
-  int slices, rank_tiles, blocks;
+  int slices, rank_tiles, blocks, rows;  // rows of a workgroup of the first product
   bool one;  // one launch, no workspace
 };
 
@@ -625,11 +633,16 @@ inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t ad
   p.one = M == 1 && R <= 32 && K * p.rank_tiles <= 16384;
   p.groups = M <= kGroupRows ? kinds : M / kGroupRows + kinds;
   p.order_ints = M <= kGroupRows ? 0 : (p.groups * (kGroupRows + 1) + 1 + 3) / 4 * 4;
-  // K in slices of four turns of a workgroup where there are few groups
+  // Half a group is more workgroups and reads A twice as often; K 4096, N 4096,
+  // 5 adapters, 32 / 64 rows of a workgroup, us a call: 500 rows of rank 16
+  // 17.5 / 19.5, of rank 128 31.4 / 35.1; 2000 rows 24.0 / 24.9, 41.9 / 42.8;
+  // 4093 rows 36.2 / 34.1, 70.6 / 61.0.
+  p.rows = M > kGroupRows && M <= 2048 ? 32 : kGroupRows;
+  // K in slices of four turns of a workgroup where there are few of them
   const int64_t turn = 32 * kShrinkWaves;
   int64_t s = (K + 4 * turn - 1) / (4 * turn);
   const int64_t full = (M + kGroupRows - 1) / kGroupRows;
-  const int64_t fill = 256 / p.groups;  // one round of a workgroup for each CU
+  const int64_t fill = 256 / ((M + p.rows - 1) / p.rows + kinds);  // one round of a workgroup for each CU
   if (s > fill) s = fill > 1 ? fill : 1;
   p.k_slice = (K + s - 1) / s;
   p.k_slice = (p.k_slice + turn - 1) / turn * turn;
@@ -700,11 +713,11 @@ int mk_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_
   }
 #undef MK_ONE_VEC
 #undef MK_ONE
-  const dim3 shrink((unsigned)p.groups, (unsigned)p.slices);
+  const dim3 shrink((unsigned)(p.groups * (kGroupRows / p.rows)), (unsigned)p.slices);
   const dim3 expand((unsigned)((N + 256 * p.blocks - 1) / (256 * p.blocks)), (unsigned)p.groups);
 #define MK_SHRINK(T, RT, V)                                                                                         \
   lora_shrink_kernel<T, RT, V><<<shrink, 64 * kShrinkWaves, 0, st>>>(gs, (const T*)x, x_stride, (const T*)a, t, K, \
-                                                                     (int)R, p.k_slice)
+                                                                     (int)R, p.k_slice, p.rows)
 #define MK_EXPAND(T, RT, V)                                                                                      \
   lora_expand_kernel<T, RT, V><<<expand, 256, 0, st>>>(gs, (const T*)base, base_stride, (const T*)b, scales, t, \
                                                        (T*)out, out_stride, N, (int)R, p.slices, p.blocks, wide)
