@@ -42,6 +42,16 @@ def as_dense(t, dtype):
     return t.to(dtype).contiguous()
 
 
+def narrow_i32(t: torch.Tensor, device) -> torch.Tensor:
+    """Ids or positions (int32 / int64) as dense int32 on ``device``.  What does not fit 32 bits becomes their end,
+    which is outside of every range as the value was."""
+    if t.dtype != torch.int32:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+    elif t.device == device and t.is_contiguous():
+        return t
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
 def values_only(*tensors: torch.Tensor) -> bool:
     """Whether a kernel that reads the tensors' memory does all that tensor ops
     would: no gradient to record, no forward-mode tangent, no function transform

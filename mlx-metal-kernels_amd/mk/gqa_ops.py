@@ -20,7 +20,7 @@ import math
 import torch
 
 from . import _contig, _lib
-from ._common import ACT_DTYPES, ci_safe_mode_enabled
+from ._common import ACT_DTYPES, ci_safe_mode_enabled, narrow_i32
 from .kv_cache_ops import host_checks_enabled, normalize_positions, reference_kv_cache_update
 from .paged_kv_ops import (
     _gather_pages,
@@ -343,7 +343,7 @@ def _qk_norm_rope_prep(qkv, K_pages, V_pages, block_table, cos, sin, position, H
             slots = slots[slots >= 0]
             if slots.unique().numel() != slots.numel():
                 raise ValueError("two tokens of one call have the same cache slot")
-    return x, _i32(position, dev), None if sequences is None else _i32(sequences, dev)
+    return x, narrow_i32(position, dev), None if sequences is None else narrow_i32(sequences, dev)
 
 
 def _slots(p, s, bt, num_pages, P):
@@ -437,7 +437,7 @@ def paged_qk_norm_rope_update(qkv, K_pages, V_pages, block_table, cos, sin, posi
         return q_out, K_pages, V_pages
     if q_weight is not None:
         q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
-    c, s, bt = _tables(cos, dev), _tables(sin, dev), _i32(block_table, dev)
+    c, s, bt = _tables(cos, dev), _tables(sin, dev), narrow_i32(block_table, dev)
     num_pages, P, _, _ = K_pages.shape
     _lib.launch("mk_qk_norm_rope_paged_update", dev, x.data_ptr(), row, _lib.ptr(q_weight), _lib.ptr(k_weight),
                 float(eps), c.data_ptr(), s.data_ptr(), pos.data_ptr(), _lib.ptr(seq), bt.data_ptr(),

@@ -23,9 +23,8 @@ from operator import attrgetter
 import torch
 
 from . import _lib
-from ._common import ci_safe_mode_enabled
+from ._common import ci_safe_mode_enabled, narrow_i32
 from .kv_cache_ops import host_checks_enabled
-from .paged_kv_ops import _i32
 
 MAX_ROWS = 4096  # rows of a forked table
 _SHAPE, _NBYTES = attrgetter("shape"), attrgetter("nbytes")
@@ -71,7 +70,7 @@ def _ids(t, device, name):
         t = torch.as_tensor(t, dtype=torch.int32)
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
-    return t if t.device == device and t.dtype == torch.int32 else t.to(device=device, dtype=torch.int32)
+    return narrow_i32(t, device)
 
 
 def count_page_refs(block_table, num_pages: int):
@@ -87,10 +86,11 @@ def count_page_refs(block_table, num_pages: int):
 
 def copy_kv_pages(pages, src, dst, *, backend: str = "auto"):
     """Page src[i] onto page dst[i] in every array of ``pages``, in place;
-    returns ``pages``.  src, dst int32 [n] (device, host or a list).  No page may be the destination of two pairs, or the
-    source of one and the destination of another.  Entries are checked on the
-    host unless that is off (``host_checks_enabled``); then pairs with an entry
-    outside of the pages are skipped."""
+    returns ``pages``.  src, dst int32 [n] (device, host or a list).  No
+    page may be the destination of two pairs, or the source of one and the
+    destination of another.  Entries are checked on the host unless that is off
+    (``host_checks_enabled``); then pairs with an entry outside of the pages are
+    skipped."""
     reference = _backend(backend)
     if len(pages) == 0:
         raise ValueError("no page arrays given")
@@ -117,7 +117,6 @@ def copy_kv_pages(pages, src, dst, *, backend: str = "auto"):
         return pages
     _lib.require_device(pages[0])
     if n and num_pages:
-        src, dst = src.contiguous(), dst.contiguous()
         at, size = _addresses(pages, num_pages)
         _lib.launch("mk_copy_kv_pages", dev, at.buffer_info()[0], size.buffer_info()[0], len(pages), src.data_ptr(),
                     dst.data_ptr(), n, num_pages)
@@ -204,8 +203,7 @@ def fork_kv_sequences(pages, block_table, lengths, ref_counts, parents, *, reser
     if reference:
         return _reference_fork(pages, block_table, lengths, ref_counts, parents, reserve, size)
     _lib.require_device(block_table)
-    table, lengths, parents = _i32(block_table, dev), lengths.contiguous(), parents.contiguous()
-    refs = _i32(ref_counts, dev)
+    table, refs = narrow_i32(block_table, dev), narrow_i32(ref_counts, dev)
     new_table = torch.empty((n, blocks), dtype=torch.int32, device=dev)
     new_refs = torch.empty_like(refs)
     ready = torch.empty(n, dtype=torch.bool, device=dev)
@@ -299,7 +297,7 @@ def compact_kv_pages(pages, block_table, ref_counts, *, backend: str = "auto"):
             t[dst] = t[src]
         return table.to(torch.int32), refs.to(torch.int32), page_map.to(torch.int32), live
     _lib.require_device(block_table)
-    table, refs = _i32(block_table, dev), _i32(ref_counts, dev)
+    table, refs = narrow_i32(block_table, dev), narrow_i32(ref_counts, dev)
     new_table = torch.empty_like(table)
     new_refs, page_map = torch.empty_like(refs), torch.empty_like(refs)
     buf = torch.empty(2 + num_pages, dtype=torch.int32, device=dev)  # live and moved pages, then the workspace

@@ -16,7 +16,7 @@ from typing import Any
 import torch
 
 from . import _lib
-from ._common import ACT_DTYPES, as_dense, ci_safe_mode_enabled, values_only
+from ._common import ACT_DTYPES, as_dense, ci_safe_mode_enabled, narrow_i32, values_only
 from .kv_cache_ops import host_checks_enabled
 from .mlp_block_ops import quantized_linear
 
@@ -83,9 +83,7 @@ def _validate(x, base, lora_a, lora_b, adapter_ids, scales, out):
         lo, hi = int(ids.min()), int(ids.max())
         if lo < -1 or hi >= adapters:
             raise ValueError(f"adapter_ids must be in [-1, {adapters}), got {lo} to {hi}")
-    if ids.dtype != torch.int32 or ids.device != x.device:
-        ids = ids.to(device=x.device, dtype=torch.int32)
-    return M, N, K, R, adapters, ids.contiguous()
+    return M, N, K, R, adapters, narrow_i32(ids, x.device)
 
 
 def reference_lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None):

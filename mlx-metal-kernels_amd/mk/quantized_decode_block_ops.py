@@ -272,8 +272,8 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
         raise ValueError("qkv_lora and out_lora need adapter_ids")
     other_rope = (q_norm_weight is not None or k_norm_weight is not None or rope_layout != "interleaved"
                   or rotary_dim not in (None, D))
-    fuse_front = (norm_weight is not None and not other_rope and qkv_lora is None and not reference and not return_intermediates and
-                  block_backend.lower() != "reference" and K_pages.dtype == x2d.dtype and
+    fuse_front = (norm_weight is not None and not other_rope and qkv_lora is None and not reference and
+                  not return_intermediates and block_backend.lower() != "reference" and K_pages.dtype == x2d.dtype and
                   K_pages.dtype in (torch.float16, torch.bfloat16))
     if fuse_front:
         # norm + qkv + RoPE + cache write in one launch, then the attention

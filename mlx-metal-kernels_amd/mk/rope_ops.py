@@ -17,7 +17,7 @@ import math
 import torch
 
 from . import _lib
-from ._common import ci_safe_mode_enabled, values_only
+from ._common import ci_safe_mode_enabled, narrow_i32, values_only
 from .kv_cache_ops import host_checks_enabled
 
 _LAYOUTS = {"interleaved": 0, "half": 1}
@@ -95,9 +95,7 @@ def _validate_positions(positions, B: int, S: int, rows: int, device):
         lo, hi = int(positions.min()), int(positions.max()) + (S if positions.ndim == 1 else 1)
         if lo < -1 or hi > rows:
             raise ValueError(f"positions must be in [-1, {rows}) with S={S}, got {lo} to {hi - 1}")
-    if dtype == torch.int32 and positions.device == device:
-        return positions.contiguous()
-    return positions.to(device=device, dtype=torch.int32).contiguous()
+    return narrow_i32(positions, device)
 
 
 def reference_apply_rope(x, cos, sin, position_offset: int = 0, *, positions=None, layout: str = "interleaved",

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from mk import gqa_ops, kv_page_ops
+from mk import gqa_ops, kv_page_ops, lora_ops, rope_ops
 from mk import llama_layer_ops as ll
 from mk import llama_stack_ops as ls
 from mk.lora_ops import LoraAdapters
@@ -174,3 +174,33 @@ def test_block_refusals(dev):
     with pytest.raises(ValueError, match="need adapter_ids"):
         paged_quantized_decode_block(x, layer.qkv_w, layer.qkv_scales, layer.o_w, layer.o_scales, *cache, cos, sin, 0,
                                      H=4, num_key_value_heads=2, head_dim=64, qkv_lora=layer.qkv_lora)
+
+
+def test_numbers_past_32_bits(dev, monkeypatch):
+    """Unread int64 ids and positions that do not fit 32 bits are outside of every range, as they were."""
+    monkeypatch.setenv("MK_SKIP_DEVICE_RANGE_CHECKS", "1")
+    far = 2 ** 32
+    ids = lambda *v: torch.tensor(v, device=dev)  # noqa: E731
+    x = torch.randn(3, 1, 4, 16, device=dev).half()
+    cos, sin = torch.ones(8, 8, device=dev), torch.zeros(8, 8, device=dev)
+    y = rope_ops.apply_rope(x, cos, sin, positions=ids(1, far + 1, -far))
+    assert torch.equal(y[0], x[0]) and not y[1:].any()
+    K, V = torch.zeros(2, 4, 4, 1, 16, device=dev).half()
+    kw = dict(num_attention_heads=2, num_key_value_heads=1, head_dim=16)
+    q, _, _ = gqa_ops.paged_qk_norm_rope_update(x, K, V, ids([0, far], [far + 1, 3], [2, 2]), cos, sin,
+                                                ids(1, 2, far), **kw)
+    assert q[:2].any() and not q[2].any() and K.any(-1).sum() == 1 and V[0, 1].any()
+    q, _, _ = gqa_ops.paged_qk_norm_rope_update(x, K, V, ids([3, 3], [3, 3], [3, 3]), cos, sin, ids(1, 2, 3),
+                                                sequences=ids(far, -far, far + 2), **kw)
+    assert not q.any() and not K[3].any()
+    pages = torch.arange(4, device=dev).half()[:, None].expand(4, 8).contiguous()
+    kv_page_ops.copy_kv_pages([pages], ids(0, far + 1, 2), ids(3, 1, far))
+    assert pages[:, 0].tolist() == [0, 1, 2, 0]
+    table, lengths, refs, _ = kv_page_ops.fork_kv_sequences([], ids([0, far]), ids(far), ids(1, 0, 0),
+                                                            ids(0, far, -far), reserve=0, page_size=2)
+    assert table.tolist() == [[0, -1], [-1, -1], [-1, -1]]
+    assert lengths.tolist() == [4, 0, 0] and refs.tolist() == [1, 0, 0]
+    base = torch.randn(2, 8, device=dev).half()
+    a, b = torch.ones(1, 2, 4, device=dev).half(), torch.ones(1, 8, 2, device=dev).half()
+    out = lora_ops.lora_add(torch.ones(2, 4, device=dev).half(), base, a, b, ids(far, 0))
+    assert torch.equal(out[0], base[0]) and (out[1] != base[1]).all()
