@@ -134,7 +134,7 @@ __device__ __forceinline__ void add_count(int32_t* p, int v) {
 
 constexpr int kForkRows = 4096;  // rows of the new table
 // What one workgroup does with the counts in LDS: a step of 32 beams over 700
-// pages in 11.9 us (16.6 with counts in memory, whose atomics and reads go to the
+// pages in 9.2 us (16.6 with counts in memory, whose atomics and reads go to the
 // L2 one after another).  Beyond, launches over all CUs count the references.
 constexpr int kSmallPages = 8192, kSmallRows = 1024, kSmallNew = 2048, kSmallEntries = 1 << 16;
 
@@ -168,13 +168,17 @@ struct ForkCounts {
   }
 };
 
-// the old rows' references off, entries i0, i0 + step, ...
+// the old rows' references off, entries i0, i0 + step, ..., eight of them on their way together
 template <bool SMALL>
 __device__ __forceinline__ void fork_drop(const ForkArgs& a, const ForkCounts<SMALL>& c, int64_t i0, int64_t step) {
   const int64_t all = a.B * a.blocks;
-  for (int64_t i = i0; i < all; i += step) {
-    const int64_t p = a.table[i];
-    if (p >= 0 && p < a.pages) c.add(p, -1);
+  for (int64_t i = i0; i < all; i += 8 * step) {
+    int p[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) p[u] = i + u * step < all ? a.table[i + u * step] : -1;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (p[u] >= 0 && p[u] < a.pages) c.add(p[u], -1);
   }
 }
 
@@ -196,15 +200,20 @@ __device__ __forceinline__ void fork_row(const ForkArgs& a, const ForkCounts<SMA
   const int used = (len + P - 1) / P, part = len % P;
   const int32_t* old = a.table + (int64_t)(parent < 0 ? 0 : parent) * blocks;
   int32_t* now = a.new_table + (int64_t)r * blocks;
-  for (int j = j0; j < blocks; j += step) {
-    int p = -1;
-    if (j < used) {
-      p = old[j];
-      if (p < 0 || p >= a.pages) p = -1;
-      if (p >= 0) c.add(p, 1);
-      if (part && j == used - 1 && last) *last = p;
+  for (int64_t jb = j0; jb < blocks; jb += 4 * step) {
+    int p[4];  // on their way together
+#pragma unroll
+    for (int u = 0; u < 4; ++u) p[u] = jb + u * step < used ? old[jb + u * step] : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t j = jb + u * step;
+      if (j >= blocks) break;
+      if (p[u] >= a.pages) p[u] = -1;
+      if (p[u] < 0) p[u] = -1;
+      else c.add(p[u], 1);
+      if (part && j == used - 1 && last) *last = p[u];
+      now[j] = p[u];
     }
-    now[j] = p;
   }
   if (j0 == 0) {
     a.new_lengths[r] = len;
@@ -216,9 +225,10 @@ __device__ __forceinline__ void fork_row(const ForkArgs& a, const ForkCounts<SMA
 // last page stays with the longest of its rows (the first of those) if nobody
 // else holds it; every other row gets a copy.  Row k of thread t is
 // t * per + k, so that a thread's rows and the threads are in order.
+// parts: positions on each row's last page, -1 for a row without a parent.
 template <bool SMALL, int PER>
 __device__ void fork_allot(const ForkArgs& a, const ForkCounts<SMALL>& c, const int* last, const int* lens,
-                           const int* parents, int* scan) {
+                           const int* parts, int* scan) {
   const int tid = threadIdx.x;
   const int per = (a.n + 1023) / 1024;
   const int P = (int)a.page_size, blocks = (int)a.blocks;
@@ -232,8 +242,8 @@ __device__ void fork_allot(const ForkArgs& a, const ForkCounts<SMALL>& c, const 
     copies[k] = false;
     fits[k] = true;
     if (k >= per || r >= a.n) continue;
-    if (parents[r] < 0) continue;
-    const int len = lens[r], page = last[r], part = len % P;
+    const int len = lens[r], page = last[r], part = parts[r];
+    if (part < 0) continue;
     const int64_t end = len + a.reserve;
     fits[k] = end <= (int64_t)blocks * P;
     if (!fits[k]) continue;
@@ -241,9 +251,10 @@ __device__ void fork_allot(const ForkArgs& a, const ForkCounts<SMALL>& c, const 
     if (page >= 0) {
       int same = 0;
       bool best = true;
+#pragma unroll 8
       for (int o = 0; o < a.n; ++o) {
         const bool s = last[o] == page;
-        const int other = s ? lens[o] % P : 0;
+        const int other = parts[o];
         same += s;
         best &= !s || other < part || (other == part && o >= r);
       }
@@ -315,17 +326,20 @@ __device__ void fork_allot(const ForkArgs& a, const ForkCounts<SMALL>& c, const 
 
 __global__ __launch_bounds__(1024) void fork_small_kernel(ForkArgs a) {
   __shared__ int32_t count[kSmallPages], ids[kSmallNew];
-  __shared__ int last[kSmallRows], lens[kSmallRows], parents[kSmallRows], scan[16];
+  __shared__ int last[kSmallRows], lens[kSmallRows], parts[kSmallRows], parents[kSmallRows], scan[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const ForkCounts<true> c = {count, ids};
   for (int i = tid; i < (int)a.pages; i += 1024) count[i] = a.refs[i];
-  for (int r = tid; r < a.n; r += 1024) lens[r] = fork_length(a, r, &parents[r]);
+  for (int r = tid; r < a.n; r += 1024) {
+    lens[r] = fork_length(a, r, &parents[r]);
+    parts[r] = parents[r] < 0 ? -1 : lens[r] % (int)a.page_size;
+  }
   __syncthreads();
   fork_drop(a, c, tid, 1024);
   for (int r = wave; r < a.n; r += 16) fork_row(a, c, r, lane, MK_WAVE, parents[r], lens[r], &last[r]);
   __syncthreads();
   if (a.reserve > 0) {
-    fork_allot<true, 1>(a, c, last, lens, parents, scan);
+    fork_allot<true, 1>(a, c, last, lens, parts, scan);
   } else {
     for (int r = tid; r < a.n; r += 1024) a.ready[r] = 1;
   }
@@ -352,16 +366,17 @@ __global__ __launch_bounds__(256) void fork_rows_kernel(ForkArgs a) {
 }
 
 __global__ __launch_bounds__(1024) void fork_allot_kernel(ForkArgs a) {
-  __shared__ int last[kForkRows], lens[kForkRows], parents[kForkRows], scan[16];
+  __shared__ int last[kForkRows], lens[kForkRows], parts[kForkRows], scan[16];
   const ForkCounts<false> c = {a.new_refs, a.ids};
   for (int r = threadIdx.x; r < a.n; r += 1024) {
-    lens[r] = fork_length(a, r, &parents[r]);
-    int p = -1;
-    if (lens[r] % a.page_size) p = a.new_table[(int64_t)r * a.blocks + lens[r] / a.page_size];
-    last[r] = p;
+    int parent;
+    lens[r] = fork_length(a, r, &parent);
+    const int part = lens[r] % (int)a.page_size;
+    parts[r] = parent < 0 ? -1 : part;
+    last[r] = part ? a.new_table[(int64_t)r * a.blocks + lens[r] / (int)a.page_size] : -1;
   }
   __syncthreads();
-  fork_allot<false, kForkRows / 1024>(a, c, last, lens, parents, scan);
+  fork_allot<false, kForkRows / 1024>(a, c, last, lens, parts, scan);
 }
 
 // ---------------------------------------------------------------------------
