@@ -350,8 +350,8 @@ int mk_copy_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t nu
  * ascending id to rows in order.  ready[r] = 0 where the row's pages do not
  * suffice or the table has no room: such a row gets none of them, shares its
  * last page and must not be appended to.  Pages that only dropped rows held
- * are free, and may be given away by the same call.  n <= 4096 rows; workspace int32, at least 2 n + 1 +
- * min(num_pages, n (1 + ceil(reserve / page_size))). */
+ * are free, and may be given away by the same call.  n <= 4096 rows; workspace
+ * int32, at least 2 n + 1 + min(num_pages, n (1 + ceil(reserve / page_size))). */
 int mk_fork_kv_sequences(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors,
                          const int32_t* block_table, const int32_t* lengths, const int32_t* ref_counts,
                          const int32_t* parents, int32_t* new_table, int32_t* new_lengths, int32_t* new_ref_counts,
@@ -361,7 +361,8 @@ int mk_fork_kv_sequences(void* const* tensors, const int64_t* page_bytes, int64_
 /* Live pages (ref_counts > 0) to ids [0, counts[0]): of the live ones past it
  * the i-th moves onto the i-th free one below.  page_map [num_pages] = where a
  * page is now, -1 for a free one; new_table [entries] = block_table through
- * it.  counts [2]: live and moved pages.  workspace: num_pages int32. */
+ * it.  counts [2]: live and moved pages.  workspace: int32, num_pages +
+ * ceil(num_pages / 8192) of them. */
 int mk_compact_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors,
                         const int32_t* block_table, const int32_t* ref_counts, int32_t* new_table,
                         int32_t* new_ref_counts, int32_t* page_map, int32_t* counts, int32_t* workspace,

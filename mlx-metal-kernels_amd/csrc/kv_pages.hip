@@ -226,9 +226,10 @@ __device__ __forceinline__ void fork_row(const ForkArgs& a, const ForkCounts<SMA
 // else holds it; every other row gets a copy.  Row k of thread t is
 // t * per + k, so that a thread's rows and the threads are in order.
 // parts: positions on each row's last page, -1 for a row without a parent.
+// paired: the rows that get a copy are marked in a.ready already.
 template <bool SMALL, int PER>
 __device__ void fork_allot(const ForkArgs& a, const ForkCounts<SMALL>& c, const int* last, const int* lens,
-                           const int* parts, int* scan) {
+                           const int* parts, int* scan, bool paired) {
   const int tid = threadIdx.x;
   const int per = (a.n + 1023) / 1024;
   const int P = (int)a.page_size, blocks = (int)a.blocks;
@@ -248,7 +249,9 @@ __device__ void fork_allot(const ForkArgs& a, const ForkCounts<SMALL>& c, const 
     fits[k] = end <= (int64_t)blocks * P;
     if (!fits[k]) continue;
     need[k] = (int)((end + P - 1) / P) - (len + P - 1) / P;
-    if (page >= 0) {
+    if (paired) {
+      copies[k] = a.ready[r];
+    } else if (page >= 0) {
       int same = 0;
       bool best = true;
 #pragma unroll 8
@@ -259,23 +262,32 @@ __device__ void fork_allot(const ForkArgs& a, const ForkCounts<SMALL>& c, const 
         best &= !s || other < part || (other == part && o >= r);
       }
       copies[k] = !(best && c.load(page) == same);
-      need[k] += copies[k];
     }
+    need[k] += copies[k];
     mine += need[k];
   }
   int wanted;
   int off = block_scan(mine, &wanted, scan);
-  // ids of the first free pages; stops where there are enough
+  // ids of the first free pages; stops where there are enough (the counts of the next 8192 on their way)
   int found = 0;
+  int next[8];
+  auto read = [&](int64_t base) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t i = base + 8 * tid + e;
+      next[e] = i < a.pages ? c.load(i) : 1;
+    }
+  };
+  if (wanted > 0) read(0);
   for (int64_t base = 0; base < a.pages && found < wanted; base += 8 * 1024) {
     int ok = 0, cnt = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int64_t i = base + 8 * tid + e;
-      const bool f = i < a.pages && c.load(i) == 0;
+      const bool f = next[e] == 0;
       ok |= (int)f << e;
       cnt += f;
     }
+    if (base + 8 * 1024 < a.pages) read(base + 8 * 1024);
     int total;
     int at = found + block_scan(cnt, &total, scan);
 #pragma unroll
@@ -339,7 +351,7 @@ __global__ __launch_bounds__(1024) void fork_small_kernel(ForkArgs a) {
   for (int r = wave; r < a.n; r += 16) fork_row(a, c, r, lane, MK_WAVE, parents[r], lens[r], &last[r]);
   __syncthreads();
   if (a.reserve > 0) {
-    fork_allot<true, 1>(a, c, last, lens, parts, scan);
+    fork_allot<true, 1>(a, c, last, lens, parts, scan, false);
   } else {
     for (int r = tid; r < a.n; r += 1024) a.ready[r] = 1;
   }
@@ -351,32 +363,57 @@ __global__ __launch_bounds__(256) void fork_init_kernel(ForkArgs a) {
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < a.pages; i += gridDim.x * 256ll) a.new_refs[i] = a.refs[i];
 }
 
-// workgroup r < n: new row r; the others: the old table
+// workgroup r < n: new row r, its last page and the positions on it to the
+// workspace (which the moves take later); the others: the old table
 __global__ __launch_bounds__(256) void fork_rows_kernel(ForkArgs a) {
   const ForkCounts<false> c = {a.new_refs, nullptr};
   const int r = blockIdx.x;
   if (r < a.n) {
     int parent;
     const int len = fork_length(a, r, &parent);
-    fork_row(a, c, r, threadIdx.x, 256, parent, len, nullptr);
-    if (threadIdx.x == 0 && a.reserve == 0) a.ready[r] = 1;
+    fork_row(a, c, r, threadIdx.x, 256, parent, len, a.reserve > 0 ? a.moves + r : nullptr);
+    if (threadIdx.x == 0) {
+      if (a.reserve > 0) a.moves[a.n + r] = parent < 0 ? -1 : len % (int)a.page_size;
+      else a.ready[r] = 1;
+    }
   } else {
     fork_drop(a, c, (r - a.n) * 256ll + threadIdx.x, (gridDim.x - a.n) * 256ll);
   }
 }
 
-__global__ __launch_bounds__(1024) void fork_allot_kernel(ForkArgs a) {
+// Workgroup r: whether row r gets a copy of its last page, to a.ready.  Up to
+// kPairRows rows the next kernel looks for itself (4096 rows: the fork in 50 us,
+// 1010 without this launch).
+constexpr int kPairRows = 256;
+__global__ __launch_bounds__(256) void fork_pairs_kernel(ForkArgs a) {
+  const int r = blockIdx.x, page = a.moves[r], part = a.moves[a.n + r];
+  int same = 0, better = 0;
+  if (page >= 0) {
+    for (int o = threadIdx.x; o < a.n; o += 256) {
+      const bool s = a.moves[o] == page;
+      const int other = a.moves[a.n + o];
+      same += s;
+      better |= s && (other > part || (other == part && o < r));
+    }
+  }
+  __shared__ int all;
+  if (threadIdx.x == 0) all = 0;
+  better = __syncthreads_or(better);
+  if (same) atomicAdd(&all, same);
+  __syncthreads();
+  if (threadIdx.x == 0) a.ready[r] = page >= 0 && (better || load_count(a.new_refs + page) != all);
+}
+
+__global__ __launch_bounds__(1024) void fork_allot_kernel(ForkArgs a, bool paired) {
   __shared__ int last[kForkRows], lens[kForkRows], parts[kForkRows], scan[16];
   const ForkCounts<false> c = {a.new_refs, a.ids};
   for (int r = threadIdx.x; r < a.n; r += 1024) {
-    int parent;
-    lens[r] = fork_length(a, r, &parent);
-    const int part = lens[r] % (int)a.page_size;
-    parts[r] = parent < 0 ? -1 : part;
-    last[r] = part ? a.new_table[(int64_t)r * a.blocks + lens[r] / (int)a.page_size] : -1;
+    lens[r] = a.new_lengths[r];
+    last[r] = a.moves[r];
+    parts[r] = a.moves[a.n + r];
   }
   __syncthreads();
-  fork_allot<false, kForkRows / 1024>(a, c, last, lens, parts, scan);
+  fork_allot<false, kForkRows / 1024>(a, c, last, lens, parts, scan, paired);
 }
 
 // ---------------------------------------------------------------------------
@@ -391,56 +428,128 @@ struct CompactArgs {
   int32_t* page_map;  // [pages]: where a page went, -1 for a free one
   int32_t* counts;    // [2]: live pages, moved ones
   int32_t* list;      // [2 * (pages / 2)]: free pages below the live count, then live ones from it on
+  int32_t* live;      // [pages / 8192, rounded up]
   int64_t entries, pages;
 };
 
 // With n live pages, the i-th live page at or past n moves to the i-th free
 // one below n: as many of the one as of the other, and no page is both.
-__global__ __launch_bounds__(1024) void compact_kernel(CompactArgs a) {
-  __shared__ int scan[16];
-  const int tid = threadIdx.x;
-  int mine = 0;
-  for (int64_t i = tid; i < a.pages; i += 1024) mine += a.refs[i] > 0;
-  int n;
-  block_scan(mine, &n, scan);
-  __syncthreads();
-  int found = 0;
-  for (int64_t base = 0; base < a.pages; base += 8 * 1024) {
-    int ok = 0, cnt = 0;
+// list: those free pages, then from m on the live ones, m = how many they are.
+
+// page i of count c, with `live` live ones before it and `below` live ones below n
+__device__ __forceinline__ void place_page(const CompactArgs& a, int64_t i, int c, int n, int live, int below) {
+  if (i < n && c <= 0) a.list[i - live] = (int32_t)i;
+  if (i >= n && c > 0) a.list[n - below + live - below] = (int32_t)i;
+  a.page_map[i] = c > 0 && i < n ? (int32_t)i : -1;
+  a.new_refs[i] = i < n ? c : 0;
+}
+
+// how many of the 8 pages from i on are live and below n
+__device__ __forceinline__ int live_below(const int (&c)[8], int64_t i, int n) {
+  int k = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t i = base + 8 * tid + e;
-      if (i >= a.pages) continue;
-      const int c = a.refs[i];
-      const bool f = i < n ? c <= 0 : c > 0;
-      ok |= (int)f << e;
-      cnt += f;
-      a.page_map[i] = c > 0 && i < n ? (int32_t)i : -1;
-      a.new_refs[i] = i < n ? c : 0;
-    }
-    int total;
-    int at = found + block_scan(cnt, &total, scan);
+  for (int e = 0; e < 8; ++e) k += c[e] > 0 && i + e < n;
+  return k;
+}
+__device__ __forceinline__ void read_counts(const CompactArgs& a, int64_t i, int (&c)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if ((ok >> e) & 1) a.list[at++] = (int32_t)(base + 8 * tid + e);
-    found += total;
-  }
-  __syncthreads();
-  const int m = found / 2;
-  if (tid == 0) {
-    a.counts[0] = n;
-    a.counts[1] = m;
-  }
-  for (int i = tid; i < m; i += 1024) {
+  for (int e = 0; e < 8; ++e) c[e] = i + e < a.pages ? a.refs[i + e] : 0;
+}
+
+// entries of pairs i0, i0 + step, ... of m: where a page went, its count there
+__device__ __forceinline__ void move_pages(const CompactArgs& a, int m, int i0, int step) {
+  for (int i = i0; i < m; i += step) {
     const int to = a.list[i], from = a.list[m + i];
     a.page_map[from] = to;
     a.new_refs[to] = a.refs[from];
   }
-  __syncthreads();
-  for (int64_t i = tid; i < a.entries; i += 1024) {
-    const int64_t p = a.table[i];
-    a.new_table[i] = p >= 0 && p < a.pages ? a.page_map[p] : -1;
+}
+
+// Table entries renamed, i0, i0 + step, ..., eight of them on their way together
+__device__ __forceinline__ void rename_entries(const CompactArgs& a, int64_t i0, int64_t step) {
+  for (int64_t i = i0; i < a.entries; i += 8 * step) {
+    int p[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) p[u] = i + u * step < a.entries ? a.table[i + u * step] : -1;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) p[u] = p[u] >= 0 && p[u] < a.pages ? a.page_map[p[u]] : -1;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i + u * step < a.entries) a.new_table[i + u * step] = p[u];
   }
+}
+
+// up to 8192 pages: all by one workgroup
+__global__ __launch_bounds__(1024) void compact_small_kernel(CompactArgs a) {
+  __shared__ int scan[16];
+  const int tid = threadIdx.x;
+  const int64_t i = 8 * tid;
+  int c[8], n, below;
+  read_counts(a, i, c);
+  int live = block_scan(live_below(c, i, INT32_MAX), &n, scan);
+  block_scan(live_below(c, i, n), &below, scan);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (i + e < a.pages) place_page(a, i + e, c[e], n, live, below);
+    live += c[e] > 0;
+  }
+  if (tid == 0) {
+    a.counts[0] = n;
+    a.counts[1] = n - below;
+  }
+  __syncthreads();
+  move_pages(a, n - below, tid, 1024);
+  __syncthreads();
+  rename_entries(a, tid, 1024);
+}
+
+// Larger pools: 8192 pages a workgroup, four launches.
+__global__ __launch_bounds__(1024) void compact_count_kernel(CompactArgs a) {
+  __shared__ int scan[16];
+  const int64_t i = blockIdx.x * 8192ll + 8 * threadIdx.x;
+  int c[8], n;
+  read_counts(a, i, c);
+  block_scan(live_below(c, i, INT32_MAX), &n, scan);
+  if (threadIdx.x == 0) a.live[blockIdx.x] = n;
+}
+
+__global__ __launch_bounds__(1024) void compact_place_kernel(CompactArgs a) {
+  __shared__ int scan[16];
+  const int tid = threadIdx.x;
+  const int64_t i = blockIdx.x * 8192ll + 8 * tid;
+  int c[8], v, n, before, below, part;
+  read_counts(a, i, c);
+  v = 0;
+  for (int k = tid; k < (int)gridDim.x; k += 1024) v += a.live[k];
+  block_scan(v, &n, scan);
+  v = 0;
+  for (int k = tid; k < (int)blockIdx.x; k += 1024) v += a.live[k];
+  block_scan(v, &before, scan);
+  const int cut = n / 8192;  // the workgroup that page n is in (there may be none)
+  v = 0;
+  for (int k = tid; k < cut; k += 1024) v += a.live[k];
+  int at[8];
+  read_counts(a, cut * 8192ll + 8 * tid, at);
+  v += live_below(at, cut * 8192ll + 8 * tid, n);
+  block_scan(v, &below, scan);
+  int live = before + block_scan(live_below(c, i, INT32_MAX), &part, scan);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (i + e < a.pages) place_page(a, i + e, c[e], n, live, below);
+    live += c[e] > 0;
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    a.counts[0] = n;
+    a.counts[1] = n - below;
+  }
+}
+
+__global__ __launch_bounds__(256) void compact_move_kernel(CompactArgs a) {
+  move_pages(a, a.counts[1], (int)(blockIdx.x * 256 + threadIdx.x), (int)(gridDim.x * 256));
+}
+
+__global__ __launch_bounds__(256) void compact_rename_kernel(CompactArgs a) {
+  rename_entries(a, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
 }
 
 }  // namespace
@@ -485,7 +594,10 @@ int mk_fork_kv_sequences(void* const* tensors, const int64_t* page_bytes, int64_
     fork_init_kernel<<<(unsigned)(init < 1024 ? init : 1024), 256, 0, st>>>(a);
     const int64_t drop = (B * max_blocks + 255) / 256;
     if (n + drop > 0) fork_rows_kernel<<<(unsigned)(n + (drop < 1024 ? drop : 1024)), 256, 0, st>>>(a);
-    if (reserve > 0 && n > 0) fork_allot_kernel<<<1, 1024, 0, st>>>(a);
+    if (reserve > 0 && n > 0) {
+      if (n > kPairRows) fork_pairs_kernel<<<(unsigned)n, 256, 0, st>>>(a);
+      fork_allot_kernel<<<1, 1024, 0, st>>>(a, n > kPairRows);
+    }
   }
   MK_CHECK_LAUNCH();
   if (reserve == 0 || n == 0) return MK_OK;
@@ -497,13 +609,26 @@ int mk_compact_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t
                         int32_t* new_ref_counts, int32_t* page_map, int32_t* counts, int32_t* workspace,
                         int64_t workspace_ints, int64_t entries, int64_t num_pages, void* stream) {
   MK_REQUIRE(entries >= 0 && num_pages > 0 && num_pages < (1LL << 31) && ref_counts && new_ref_counts && page_map);
-  MK_REQUIRE(counts && workspace && workspace_ints >= num_pages && (entries == 0 || (block_table && new_table)));
+  const int64_t chunks = (num_pages + 8191) / 8192;
+  MK_REQUIRE(counts && workspace && workspace_ints >= num_pages + chunks);
+  MK_REQUIRE(entries == 0 || (block_table && new_table));
   MK_REQUIRE(num_tensors >= 0 && (num_tensors == 0 || (tensors && page_bytes)));
   for (int64_t i = 0; i < num_tensors; ++i) MK_REQUIRE(tensors[i] && page_bytes[i] >= 0);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const CompactArgs a = {block_table, ref_counts, new_table, new_ref_counts, page_map, counts, workspace, entries,
-                         num_pages};
-  compact_kernel<<<1, 1024, 0, st>>>(a);
+  const CompactArgs a = {block_table, ref_counts, new_table, new_ref_counts, page_map, counts, workspace,
+                         workspace + num_pages, entries, num_pages};
+  // One launch of one workgroup, or four over all CUs, us a call: 8000 pages and
+  // 16384 entries 20 / 32; 40000 pages and 32768 entries 69 / 32; 300000 pages
+  // 470 / 33.
+  if (num_pages <= 8192 && entries <= 16384) {
+    compact_small_kernel<<<1, 1024, 0, st>>>(a);
+  } else {
+    const int64_t moves = (num_pages / 2 + 255) / 256, names = (entries + 2047) / 2048;
+    compact_count_kernel<<<(unsigned)chunks, 1024, 0, st>>>(a);
+    compact_place_kernel<<<(unsigned)chunks, 1024, 0, st>>>(a);
+    compact_move_kernel<<<(unsigned)(moves < 1024 ? moves : 1024), 256, 0, st>>>(a);
+    if (names > 0) compact_rename_kernel<<<(unsigned)(names < 1024 ? names : 1024), 256, 0, st>>>(a);
+  }
   MK_CHECK_LAUNCH();
   // no more pages move than are free, and than are live
   return num_pages > 1 ? copy_pages(tensors, page_bytes, num_tensors, nullptr, workspace, counts + 1, num_pages / 2,

@@ -300,10 +300,11 @@ def compact_kv_pages(pages, block_table, ref_counts, *, backend: str = "auto"):
     table, refs = narrow_i32(block_table, dev), narrow_i32(ref_counts, dev)
     new_table = torch.empty_like(table)
     new_refs, page_map = torch.empty_like(refs), torch.empty_like(refs)
-    buf = torch.empty(2 + num_pages, dtype=torch.int32, device=dev)  # live and moved pages, then the workspace
+    ints = num_pages + -(-num_pages // 8192)
+    buf = torch.empty(2 + ints, dtype=torch.int32, device=dev)  # live and moved pages, then the workspace
     at, sizes = _addresses(pages, num_pages)
     base = buf.data_ptr()
     _lib.launch("mk_compact_kv_pages", dev, at.buffer_info()[0], sizes.buffer_info()[0], len(pages),
                 table.data_ptr() or None, refs.data_ptr(), new_table.data_ptr() or None, new_refs.data_ptr(),
-                page_map.data_ptr(), base, base + 8, num_pages, table.numel(), num_pages)
+                page_map.data_ptr(), base, base + 8, ints, table.numel(), num_pages)
     return new_table, new_refs, page_map, buf[:1]

@@ -68,6 +68,47 @@ def test_compact(dev, seed):
     assert all(torch.equal(bits(a), bits(b)) for a, b in zip(pages, moved(before, want[4])))
 
 
+@pytest.mark.parametrize("NP,held,entries", [(16384, 8192, 60), (16384, 16384, 0), (24576, 0, 9), (16385, 1, 20000),
+                                             (70000, 40001, 300000), (50, 30, 16385), (8193, 8192, 5),
+                                             (8192, 8191, 16384)])
+def test_compact_large(dev, NP, held, entries):
+    """Live counts at and beside the edges of a workgroup's pages, in any order; tables of more entries than pages."""
+    rng = np.random.default_rng(NP + held)
+    refs = np.zeros(NP, np.int64)
+    refs[rng.permutation(NP)[:held]] = rng.integers(1, 5, size=held)
+    table = rng.integers(-1, NP, size=(1, entries)) if entries else np.full((1, 1), -1)
+    counts = np.bincount(table[table >= 0], minlength=NP)
+    refs = np.where(refs > 0, refs + counts, 0)
+    table = np.where((table >= 0) & (refs[table] > 0), table, -1)
+    pages = [t.to(dev) for t in pool(rng, NP, 1, [((3,), torch.float16)])]
+    before = [t.clone() for t in pages]
+    got = kp.compact_kv_pages(pages, t32(table, dev), t32(refs, dev))
+    want = sv.compact(table, refs)
+    assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip(got[:3], want[:3])) and got[3].tolist() == [want[3]]
+    src, dst = (torch.tensor([m[k] for m in want[4]], dtype=torch.long, device=dev) for k in (0, 1))
+    before[0][dst] = before[0][src]
+    assert torch.equal(bits(pages[0]), bits(before[0]))
+
+
+@pytest.mark.parametrize("n", [256, 257, 700])
+def test_fork_shared_last_pages(dev, n):
+    """Many rows on few last pages of different fill, the free pages behind thousands that are held."""
+    rng = np.random.default_rng(n)
+    P, blocks, NP, B = 8, 4, 30000, 24
+    table = rng.permutation(20000)[:B * blocks].reshape(B, blocks)
+    table[B // 2:] = table[:B // 2]  # pairs of rows that share all of their pages, up to different positions
+    lengths = rng.integers(2 * P + 1, 3 * P, size=B)
+    table[:, 3] = -1
+    refs = np.bincount(table[table >= 0], minlength=NP)
+    refs[rng.random(NP) < 0.5] += 1
+    refs[:26000] = np.maximum(refs[:26000], 1)
+    parents = rng.integers(-1, B, size=n)
+    pages = [t.to(dev) for t in pool(rng, NP, P, [((2,), torch.float16)])]
+    before = [t.clone() for t in pages]
+    got = kp.fork_kv_sequences(pages, *(t32(a, dev) for a in (table, lengths, refs, parents)), reserve=9)
+    assert check_fork(got, pages, before, table, lengths, refs, parents, P, 9)
+
+
 @pytest.mark.parametrize("spec", SPECS)
 def test_copy(dev, spec):
     rng = np.random.default_rng(3)
