@@ -2,7 +2,8 @@
 quant_ops / mlp_block_ops / paged_kv_ops / paged_quantized_kv_ops modules of
 manishklach/mlx-metal-kernels over torch tensors.
 
-Modules mirror the reference's ``ops/`` files one-to-one; the kernels live in
+Modules mirror the reference's ``ops/`` files one-to-one (``kv_page_ops`` and
+``lora_ops``, for servers, have no counterpart there); the kernels live in
 ``libmk_hip.so`` (C ABI declared in include/mk_hip.h) and are loaded lazily
 by ``mk._lib``.
 """
@@ -15,8 +16,10 @@ __all__ = [
     "fused_ops",
     "gqa_ops",
     "kv_cache_ops",
+    "kv_page_ops",
     "llama_layer_ops",
     "llama_stack_ops",
+    "lora_ops",
     "mlp_block_ops",
     "norm_ops",
     "paged_kv_ops",
