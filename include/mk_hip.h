@@ -333,7 +333,7 @@ int mk_qk_norm_rope_paged_update(const void* qkv, int64_t row_stride, const void
  * together.  page_bytes and addresses that are multiples of 16 take 16-byte
  * accesses.
  *
- * mk_copy_kv_pages: page src[i] onto dst[i] (device int32), i < n; entries
+ * mk_copy_kv_pages: page src[i] onto dst[i] (device int32), i < n < 2^30; entries
  * outside [0, num_pages) are skipped.  No page may be the destination of two
  * pairs, or the source of one and the destination of another. */
 int mk_copy_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors, const int32_t* src,

@@ -558,7 +558,7 @@ extern "C" {
 
 int mk_copy_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors, const int32_t* src,
                      const int32_t* dst, int64_t n, int64_t num_pages, void* stream) {
-  MK_REQUIRE(num_tensors >= 0 && n >= 0 && n < (1LL << 31) && num_pages >= 0 && num_pages < (1LL << 31));
+  MK_REQUIRE(num_tensors >= 0 && n >= 0 && n < (1LL << 30) && num_pages >= 0 && num_pages < (1LL << 31));
   MK_REQUIRE(num_tensors == 0 || (tensors && page_bytes));
   MK_REQUIRE(n == 0 || (src && dst));
   for (int64_t i = 0; i < num_tensors; ++i) MK_REQUIRE(tensors[i] && page_bytes[i] >= 0);
