@@ -47,18 +47,49 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// 8 values p[at .. at + 8), zeros from `end` on
-template <typename T, bool VEC>
-__device__ __forceinline__ typename Frag<T>::v8 load_frag(const T* p, int64_t at, int64_t end) {
+// 16 and 8 bytes from and to any address of a value
+__device__ __forceinline__ u32x4 load16(const void* p) {
+  u32x4 v;
+  __builtin_memcpy(&v, (const uint16_t*)p, 16);
+  return v;
+}
+typedef u32x2 __attribute__((aligned(2))) u32x2_any;
+__device__ __forceinline__ u32x2 load8(const void* p) {
+  u32x2 v;
+  __builtin_memcpy(&v, (const uint16_t*)p, 8);
+  return v;
+}
+
+// Rows along which a fragment of 8 values is read: of whole fragments; with a
+// rest; of fewer than 8 values.
+enum Len { kFew, kRest, kWhole };
+inline Len len_of(int64_t n) { return n < 8 ? kFew : n % 8 ? kRest : kWhole; }
+
+// 8 values p[at .. at + 8) of a row that ends at `end`, zeros behind it and
+// where `ok` is false.  No branch but with under 8 values in all, so that loads
+// stay in flight beside it: a fragment with the end in it is read from 8 before
+// the end and moved down.
+template <typename T, Len LEN>
+__device__ __forceinline__ typename Frag<T>::v8 load_frag(const T* p, int64_t at, int64_t end, bool ok = true) {
   typename Frag<T>::v8 v;
-  if constexpr (VEC) {  // whole 16-byte chunks; no branch, so that loads stay in flight beside it
-    u32x4 w = ldg128(p + (at < end ? at : 0));
+  if constexpr (LEN == kWhole) {
+    ok = ok && at < end;
+    u32x4 w = load16(p + (at < end ? at : 0));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = at < end ? w[e] : 0u;
+    for (int e = 0; e < 4; ++e) w[e] = ok ? w[e] : 0u;
     v = bitcast<typename Frag<T>::v8>(w);
+  } else if constexpr (LEN == kRest) {
+    const int64_t from = at < end - 8 ? at : end - 8;
+    const u32x4 w = load16(p + from);
+    const int s = at - from < 8 ? 16 * (int)(at - from) : 128;  // bits
+    const uint64_t lo = w[0] | (uint64_t)w[1] << 32, hi = w[2] | (uint64_t)w[3] << 32;
+    uint64_t x = s < 64 ? lo >> s | (hi << 1) << (63 - s) : hi >> (s & 63), y = s < 64 ? hi >> s : 0;
+    x = ok && s < 128 ? x : 0;
+    y = ok ? y : 0;
+    v = bitcast<typename Frag<T>::v8>(u32x4{(uint32_t)x, (uint32_t)(x >> 32), (uint32_t)y, (uint32_t)(y >> 32)});
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = at + e < end ? p[at + e] : from_f32<T>(0.0f);
+    for (int e = 0; e < 8; ++e) v[e] = ok && at + e < end ? p[at + e] : from_f32<T>(0.0f);
   }
   return v;
 }
@@ -194,11 +225,11 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(const int32_t* __restr
 constexpr int kShrinkWaves = 8;
 
 // put(i, row, r, s): ranks r .. r + 3 of the group's row number i
-template <typename T, int RT, int MT, bool VEC, typename Put>
+template <typename T, int RT, int MT, Len LEN, typename Put>
 __device__ __forceinline__ void shrink_rows(const T* x, int64_t x_stride, const T* ai, int64_t K, int R, int64_t k0,
                                             int64_t k1, int rowlist, f32x4 (&part)[kShrinkWaves][RT][64], Put put) {
-  constexpr int UN = !VEC || RT * MT > 8 ? 1 : RT * MT > 2 ? 2 : 4;  // turns whose loads are in flight together
-  constexpr bool AHEAD = VEC && RT * MT <= 16;  // (more would not fit the registers)
+  constexpr int UN = LEN == kFew || RT * MT > 8 ? 1 : RT * MT > 2 ? 2 : 4;  // turns whose loads are in flight together
+  constexpr bool AHEAD = LEN != kFew && RT * MT <= 16;  // (more would not fit the registers)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, grp = lane >> 4;
   const int any = __builtin_amdgcn_readfirstlane(rowlist);
@@ -223,11 +254,11 @@ __device__ __forceinline__ void shrink_rows(const T* x, int64_t x_stride, const 
     for (int u = 0; u < UN; ++u) {
       const int64_t k = kb + 32 * u + 8 * grp;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) f.x[u][i] = load_frag<T, VEC>(xr[i], k, k1);
+      for (int i = 0; i < MT; ++i) f.x[u][i] = load_frag<T, LEN>(xr[i], k, k1);
 #pragma unroll
       for (int q = 0; q < RT; ++q) {
         const int r = 16 * q + col;
-        f.a[u][q] = load_frag<T, VEC>(ai + (int64_t)(r < R ? r : 0) * K, k, r < R ? k1 : 0);
+        f.a[u][q] = load_frag<T, LEN>(ai + (int64_t)(r < R ? r : 0) * K, k, k1, r < R);
       }
     }
     return f;
@@ -270,26 +301,26 @@ __device__ __forceinline__ void shrink_rows(const T* x, int64_t x_stride, const 
   }
 }
 
-template <typename T, int RT, bool VEC, typename Put>
+template <typename T, int RT, Len LEN, typename Put>
 __device__ __forceinline__ void shrink_group(const T* x, int64_t x_stride, const T* ai, int64_t K, int R, int64_t k0,
                                              int64_t k1, int n, int rowlist, f32x4 (&part)[kShrinkWaves][RT][64],
                                              Put put) {
-  if constexpr (VEC) {
-    if (n <= 16) shrink_rows<T, RT, 1, VEC>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
-    else if (n <= 32) shrink_rows<T, RT, 2, VEC>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
-    else shrink_rows<T, RT, 4, VEC>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
+  if constexpr (LEN != kFew) {
+    if (n <= 16) shrink_rows<T, RT, 1, LEN>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
+    else if (n <= 32) shrink_rows<T, RT, 2, LEN>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
+    else shrink_rows<T, RT, 4, LEN>(x, x_stride, ai, K, R, k0, k1, rowlist, part, put);
   } else {  // values one by one: 16 rows at a time leave the registers for them
     for (int i = 0; i < n; i += 16) {
       const int at = ((int)threadIdx.x & 63) + i;
       const int row = __shfl(rowlist, at & 63, MK_WAVE);
       if (i) __syncthreads();  // the last rows' sums are read
-      shrink_rows<T, RT, 1, VEC>(x, x_stride, ai, K, R, k0, k1, at < 64 ? row : -1, part,
+      shrink_rows<T, RT, 1, LEN>(x, x_stride, ai, K, R, k0, k1, at < 64 ? row : -1, part,
                                  [&](int j, int m, int r, const f32x4& s) { put(i + j, m, r, s); });
     }
   }
 }
 
-template <typename T, int RT, bool VEC>
+template <typename T, int RT, Len LEN>
 __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(Groups gs, const T* __restrict__ x,
                                                                         int64_t x_stride, const T* __restrict__ a,
                                                                         float* __restrict__ t, int64_t K, int R,
@@ -308,7 +339,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(Groups g
   const int64_t k1 = k0 + k_slice < K ? k0 + k_slice : K;
   const T* ai = a + (int64_t)adapter * R * K;
   t += (int64_t)blockIdx.y * gs.M * (16 * RT);
-  shrink_group<T, RT, VEC>(x, x_stride, ai, K, R, k0, k1, n, rowlist, part,
+  shrink_group<T, RT, LEN>(x, x_stride, ai, K, R, k0, k1, n, rowlist, part,
                            [&](int, int m, int r, f32x4 s) {
 #pragma unroll
                              for (int e = 0; e < 4; ++e) s[e] = r + e < R ? s[e] : 0.0f;  // (0 x infinity behind R)
@@ -366,7 +397,7 @@ struct ExpandRows {
 };
 
 // B's fragments of 64 outputs from n0 on
-template <typename T, int RT, bool VEC>
+template <typename T, int RT, Len LEN>
 __device__ __forceinline__ void load_b(const T* bi, int64_t n0, int64_t N, int R,
                                        typename Frag<T>::v8 (&bf)[4][ExpandRows<T, RT>::KS]) {
   const int col = threadIdx.x & 15, grp = (threadIdx.x & 63) >> 4;
@@ -375,23 +406,36 @@ __device__ __forceinline__ void load_b(const T* bi, int64_t n0, int64_t N, int R
     const int64_t r = n0 + 4 * col + j;
 #pragma unroll
     for (int s = 0; s < ExpandRows<T, RT>::KS; ++s)
-      bf[j][s] = load_frag<T, VEC>(bi + (r < N ? r : N - 1) * R, RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp, R);
+      bf[j][s] = load_frag<T, LEN>(bi + (r < N ? r : N - 1) * R, RT == 1 ? 8 * (grp & 1) : 32 * s + 8 * grp, R);
   }
 }
 
-// rows without an adapter: outputs c0 .. c1 of them copied
+// Rows without an adapter: outputs c0 .. c1 of them copied, by a workgroup, 4
+// side by side a thread and those of 4 places of the rows on their way together
+// (a row at a time is 64 trips to memory one after another).
 template <typename T>
 __device__ __forceinline__ void copy_rows(const T* base, int64_t base_stride, T* out, int64_t out_stride, int64_t c0,
-                                          int64_t c1, int n, int rowlist, bool wide) {
-  for (int i = 0; i < n; ++i) {
-    const int64_t m = __builtin_amdgcn_readlane(rowlist, i);
-    const T* br = base + m * base_stride;
-    T* orow = out + m * out_stride;
-    if (wide) {
-      for (int64_t c = c0 + 4 * (int)threadIdx.x; c < c1; c += 4 * (int)blockDim.x)
-        *reinterpret_cast<u32x2*>(orow + c) = ldg64(br + c);
-    } else {
-      for (int64_t c = c0 + (int)threadIdx.x; c < c1; c += (int)blockDim.x) orow[c] = br[c];
+                                          int64_t c1, int n, int rowlist) {
+  constexpr int UN = 4;
+  const int width = (int)(c1 - c0), chunks = (width + 3) / 4, all = n * chunks;
+  for (int at0 = 0; at0 < all; at0 += UN * (int)blockDim.x) {
+    u32x2 w[UN];
+    const T* br[UN];
+    T* orow[UN];
+    int left[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int at = at0 + u * (int)blockDim.x + (int)threadIdx.x, i = at / chunks, c = at - i * chunks;
+      const int64_t m = __shfl(rowlist, i & 63, MK_WAVE);  // (every lane: the source has to be active)
+      br[u] = base + m * base_stride + c0 + 4 * c;
+      orow[u] = out + m * out_stride + c0 + 4 * c;
+      left[u] = at < all ? width - 4 * c : 0;
+      if (left[u] >= 4) w[u] = load8(br[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (left[u] >= 4) *reinterpret_cast<u32x2_any*>(orow[u]) = w[u];
+      else for (int e = 0; e < left[u]; ++e) orow[u][e] = br[u][e];
     }
   }
 }
@@ -399,8 +443,7 @@ __device__ __forceinline__ void copy_rows(const T* base, int64_t base_stride, T*
 // 64 outputs from n0 on of a group's n rows, by a wave
 template <typename T, int RT>
 __device__ __forceinline__ void expand_rows(const ExpandRows<T, RT>& l, const T* base, T* out, int64_t N, int64_t n0,
-                                            int n, bool wide,
-                                            const typename Frag<T>::v8 (&bf)[4][ExpandRows<T, RT>::KS]) {
+                                            int n, const typename Frag<T>::v8 (&bf)[4][ExpandRows<T, RT>::KS]) {
   typedef ExpandRows<T, RT> L;
   typedef typename L::v8 v8;
   const int col = threadIdx.x & 15, grp = (threadIdx.x & 63) >> 4;
@@ -427,40 +470,44 @@ __device__ __forceinline__ void expand_rows(const ExpandRows<T, RT>& l, const T*
   };
   const T* bn = base + nn;
   T* on = out + nn;
+  // outputs 4 side by side: the sums of row i of 4 on base's values
+  auto join = [&](const f32x4 (&acc)[4], float back, int i, u32x2 w) {
+    u32x2 o;
+#pragma unroll
+    for (int j = 0; j < 4; j += 2)
+      o[j >> 1] = pack2<T>(fmaf(acc[j][i], back, to_f32(bitcast<T>((uint16_t)w[j >> 1]))),
+                           fmaf(acc[j + 1][i], back, to_f32(bitcast<T>((uint16_t)(w[j >> 1] >> 16)))));
+    return o;
+  };
   int rt = 0;
-  if (wide && n0 + 64 <= N && n >= 16) {
+  if (n0 + 64 <= N && n >= 16) {
     // whole tiles, without a branch: base of the next 16 rows is on its way while these are computed
     const int whole = n / 16;
     u32x2 w[4], next[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = ldg64(bn + l.at_base[4 * grp + i]);
+    for (int i = 0; i < 4; ++i) w[i] = load8(bn + l.at_base[4 * grp + i]);
     for (; rt < whole; ++rt) {
       const int then = 16 * (rt + 1 < whole ? rt + 1 : rt) + 4 * grp;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) next[i] = ldg64(bn + l.at_base[then + i]);
+      for (int i = 0; i < 4; ++i) next[i] = load8(bn + l.at_base[then + i]);
       f32x4 acc[4];
       product(rt, acc);
       const f32x4 back = l.backs[4 * rt + grp];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u32x2 o;
-#pragma unroll
-        for (int j = 0; j < 4; j += 2)
-          o[j >> 1] = pack2<T>(fmaf(acc[j][i], back[i], to_f32(bitcast<T>((uint16_t)w[i][j >> 1]))),
-                               fmaf(acc[j + 1][i], back[i], to_f32(bitcast<T>((uint16_t)(w[i][j >> 1] >> 16)))));
-        // (streamed: 4093 rows x 14336 in 88.8 us, 90.6 by way of the L2)
-        __builtin_nontemporal_store(o, reinterpret_cast<u32x2*>(on + l.at_out[16 * rt + 4 * grp + i]));
-      }
+      for (int i = 0; i < 4; ++i)  // (streamed: 4093 rows x 14336 in 88.8 us, 90.6 by way of the L2)
+        __builtin_nontemporal_store(join(acc, back[i], i, w[i]),
+                                    reinterpret_cast<u32x2_any*>(on + l.at_out[16 * rt + 4 * grp + i]));
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = next[i];
     }
   }
+  const bool four = nn + 4 <= N;
   for (; 16 * rt < n; ++rt) {
-    u32x2 w[4];
+    u32x2 w[4] = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 16 * rt + 4 * grp + i;
-      if (wide) w[i] = ldg64(base + l.at_base[r < n ? r : 0] + (nn < N ? nn : 0));
+      if (four) w[i] = load8(bn + l.at_base[r < n ? r : 0]);
     }
     f32x4 acc[4];
     product(rt, acc);
@@ -469,31 +516,22 @@ __device__ __forceinline__ void expand_rows(const ExpandRows<T, RT>& l, const T*
     for (int i = 0; i < 4; ++i) {
       const int r = 16 * rt + 4 * grp + i;
       if (r >= n) continue;
-      T* orow = on + l.at_out[r];
-      if (wide) {  // whole 8-byte chunks
-        if (nn >= N) continue;
-        u32x2 o;
-#pragma unroll
-        for (int j = 0; j < 4; j += 2)
-          o[j >> 1] = pack2<T>(fmaf(acc[j][i], back[i], to_f32(bitcast<T>((uint16_t)w[i][j >> 1]))),
-                               fmaf(acc[j + 1][i], back[i], to_f32(bitcast<T>((uint16_t)(w[i][j >> 1] >> 16)))));
-        *reinterpret_cast<u32x2*>(orow) = o;
+      if (four) {
+        *reinterpret_cast<u32x2_any*>(on + l.at_out[r]) = join(acc, back[i], i, w[i]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const T* br = bn + l.at_base[r];
-          if (nn + j < N) orow[j] = from_f32<T>(fmaf(acc[j][i], back[i], to_f32(br[j])));
-        }
+        for (int j = 0; j < 4; ++j)
+          if (nn + j < N) on[l.at_out[r] + j] = from_f32<T>(fmaf(acc[j][i], back[i], to_f32(bn[l.at_base[r] + j])));
       }
     }
   }
 }
 
-template <typename T, int RT, bool VEC>
+template <typename T, int RT, Len LEN>
 __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* base, int64_t base_stride,
                                                           const T* __restrict__ b, const float* __restrict__ scales,
                                                           const float* __restrict__ t, T* out, int64_t out_stride,
-                                                          int64_t N, int R, int slices, int blocks, bool wide) {
+                                                          int64_t N, int R, int slices, int blocks) {
   typedef ExpandRows<T, RT> L;
   __shared__ L l;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -502,7 +540,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
   if (n == 0 || (adapter < 0 && base == out)) return;
   if (adapter < 0) {
     const int64_t c0 = (int64_t)blockIdx.x * blocks * 256;
-    copy_rows(base, base_stride, out, out_stride, c0, c0 + 256 * blocks < N ? c0 + 256 * blocks : N, n, rowlist, wide);
+    copy_rows(base, base_stride, out, out_stride, c0, c0 + 256 * blocks < N ? c0 + 256 * blocks : N, n, rowlist);
     return;
   }
   if (wave == 0) {
@@ -512,7 +550,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
   const T* bi = b + (int64_t)adapter * N * R;
   typename L::v8 bf[4][L::KS];
   int64_t n0 = ((int64_t)blockIdx.x * blocks * 4 + wave) * 64;
-  load_b<T, RT, VEC>(bi, n0, N, R, bf);  // on the way while t is joined
+  load_b<T, RT, LEN>(bi, n0, N, R, bf);  // on the way while t is joined
   const float scale = scales ? scales[adapter] : 1.0f;
   const int chunks = ((n + 15) & ~15) * L::CH;
   for (int at0 = 0; at0 < chunks; at0 += 256) {
@@ -536,8 +574,8 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
   lds_barrier();  // (the loads of B stay in flight)
   for (int blk = 0; blk < blocks; ++blk, n0 += 256) {
     if (n0 >= N) return;
-    if (blk) load_b<T, RT, VEC>(bi, n0, N, R, bf);
-    expand_rows<T, RT>(l, base, out, N, n0, n, wide, bf);
+    if (blk) load_b<T, RT, LEN>(bi, n0, N, R, bf);
+    expand_rows<T, RT>(l, base, out, N, n0, n, bf);
   }
 }
 
@@ -555,12 +593,12 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
 
 constexpr int kOneWaves = 8;
 
-template <typename T, int RT, bool VEC>
+template <typename T, int RT, Len LA, Len LB>
 __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(const int32_t* __restrict__ ids, int adapters,
                                                                   const T* __restrict__ x, const T* base,
                                                                   const T* __restrict__ a, const T* __restrict__ b,
                                                                   const float* __restrict__ scales, T* out, int64_t N,
-                                                                  int64_t K, int R, bool wide) {
+                                                                  int64_t K, int R) {
   typedef ExpandRows<T, RT> L;
   constexpr int RW = L::RP / kOneWaves;  // ranks of a wave
   constexpr int UN = RT == 1 ? 4 : 2;    // kilobytes of each row in flight
@@ -570,13 +608,13 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(const int32_t*
   const int adapter = ids[0];
   if (adapter < 0 || adapter >= adapters) {
     const int64_t c0 = (int64_t)blockIdx.x * 64 * kOneWaves;
-    if (base != out) copy_rows(base, 0, out, 0, c0, c0 + 64 * kOneWaves < N ? c0 + 64 * kOneWaves : N, 1, 0, wide);
+    if (base != out) copy_rows(base, 0, out, 0, c0, c0 + 64 * kOneWaves < N ? c0 + 64 * kOneWaves : N, 1, 0);
     return;
   }
   if (wave == 0) l.at_base[lane] = l.at_out[lane] = 0;
   const int64_t n0 = ((int64_t)blockIdx.x * kOneWaves + wave) * 64;
   typename L::v8 bf[4][L::KS];
-  load_b<T, RT, VEC>(b + (int64_t)adapter * N * R, n0, N, R, bf);  // on the way while t is formed
+  load_b<T, RT, LB>(b + (int64_t)adapter * N * R, n0, N, R, bf);  // on the way while t is formed
   const T* ar[RW];
   float acc[RW];
 #pragma unroll
@@ -590,8 +628,8 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(const int32_t*
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
 #pragma unroll
-      for (int q = 0; q < RW; ++q) av[u][q] = load_frag<T, VEC>(ar[q], k0 + 512 * u, K);
-      xv[u] = load_frag<T, VEC>(x, k0 + 512 * u, K);
+      for (int q = 0; q < RW; ++q) av[u][q] = load_frag<T, LA>(ar[q], k0 + 512 * u, K);
+      xv[u] = load_frag<T, LA>(x, k0 + 512 * u, K);
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u)
@@ -617,7 +655,7 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(const int32_t*
     l.put(i & 15, c, v, scales ? scales[adapter] : 1.0f, i < 16);
   }
   lds_barrier();
-  if (n0 < N) expand_rows<T, RT>(l, base, out, N, n0, 1, wide, bf);
+  if (n0 < N) expand_rows<T, RT>(l, base, out, N, n0, 1, bf);
 }
 
 struct LoraPlan {
@@ -630,7 +668,7 @@ inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t ad
   LoraPlan p;
   p.rank_tiles = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
   const int64_t kinds = adapters + 1 < M ? adapters + 1 : M;  // adapters that rows can name, and none
-  p.one = M == 1 && R <= 32 && K * p.rank_tiles <= 16384;
+  p.one = M == 1 && R <= 32 && K >= 8 && K * p.rank_tiles <= 16384;
   p.groups = M <= kGroupRows ? kinds : M / kGroupRows + kinds;
   p.order_ints = M <= kGroupRows ? 0 : (p.groups * (kGroupRows + 1) + 1 + 3) / 4 * 4;
   // Half a group is more workgroups and reads A twice as often; K 4096, N 4096,
@@ -684,49 +722,51 @@ int mk_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_
   const LoraPlan p = lora_plan(M, N, K, R, adapters);
   int32_t* order = reinterpret_cast<int32_t*>(workspace);
   float* t = reinterpret_cast<float*>(workspace) + p.order_ints;
-  const bool vec_a = K % 8 == 0 && x_stride % 8 == 0 && mk_aligned(x, 16) && mk_aligned(a, 16);
-  const bool vec_b = R % 8 == 0 && mk_aligned(b, 16);
-  const bool wide = N % 4 == 0 && base_stride % 4 == 0 && out_stride % 4 == 0 && mk_aligned(base, 8) &&
-                    mk_aligned(out, 8);
+  const Len len_a = len_of(K), len_b = len_of(R);
   Groups gs = {adapter_ids, nullptr, nullptr, M, (int)adapters};
   if (M > kGroupRows) {
     gs.rows = order;
     gs.adapters = order + p.groups * kGroupRows;
     lora_group_kernel<<<1, 1024, 0, st>>>(adapter_ids, order, order + p.groups * kGroupRows, M, (int)adapters);
   }
-#define MK_ONE(T, RT, V)                                                                                             \
-  lora_one_kernel<T, RT, V><<<(unsigned)((N + 64 * kOneWaves - 1) / (64 * kOneWaves)), 64 * kOneWaves, 0, st>>>( \
-      adapter_ids, (int)adapters, (const T*)x, (const T*)base, (const T*)a, (const T*)b, scales, (T*)out, N, K,  \
-      (int)R, wide)
-#define MK_ONE_VEC(T, RT)                     \
-  do {                                        \
-    if (vec_a && vec_b) MK_ONE(T, RT, true);  \
-    else MK_ONE(T, RT, false);                \
+#define MK_ONE(T, RT, LA, LB)                                                                                        \
+  lora_one_kernel<T, RT, LA, LB><<<(unsigned)((N + 64 * kOneWaves - 1) / (64 * kOneWaves)), 64 * kOneWaves, 0, st>>>( \
+      adapter_ids, (int)adapters, (const T*)x, (const T*)base, (const T*)a, (const T*)b, scales, (T*)out, N, K, (int)R)
+#define MK_ONE_LEN(T, RT)                                                 \
+  do {                                                                    \
+    if (len_b == kFew && len_a == kRest) MK_ONE(T, RT, kRest, kFew);      \
+    else if (len_b == kFew) MK_ONE(T, RT, kWhole, kFew);                  \
+    else if (len_b == kRest && len_a == kRest) MK_ONE(T, RT, kRest, kRest); \
+    else if (len_b == kRest) MK_ONE(T, RT, kWhole, kRest);                \
+    else if (len_a == kRest) MK_ONE(T, RT, kRest, kWhole);                \
+    else MK_ONE(T, RT, kWhole, kWhole);                                   \
   } while (0)
   if (p.one) {
-    if (dtype == MK_DT_F16 && p.rank_tiles == 1) MK_ONE_VEC(f16, 1);
-    else if (dtype == MK_DT_F16) MK_ONE_VEC(f16, 2);
-    else if (p.rank_tiles == 1) MK_ONE_VEC(bf16, 1);
-    else MK_ONE_VEC(bf16, 2);
+    if (dtype == MK_DT_F16 && p.rank_tiles == 1) MK_ONE_LEN(f16, 1);
+    else if (dtype == MK_DT_F16) MK_ONE_LEN(f16, 2);
+    else if (p.rank_tiles == 1) MK_ONE_LEN(bf16, 1);
+    else MK_ONE_LEN(bf16, 2);
     MK_CHECK_LAUNCH();
     return MK_OK;
   }
-#undef MK_ONE_VEC
+#undef MK_ONE_LEN
 #undef MK_ONE
   const dim3 shrink((unsigned)(p.groups * (kGroupRows / p.rows)), (unsigned)p.slices);
   const dim3 expand((unsigned)((N + 256 * p.blocks - 1) / (256 * p.blocks)), (unsigned)p.groups);
-#define MK_SHRINK(T, RT, V)                                                                                         \
-  lora_shrink_kernel<T, RT, V><<<shrink, 64 * kShrinkWaves, 0, st>>>(gs, (const T*)x, x_stride, (const T*)a, t, K, \
+#define MK_SHRINK(T, RT, L)                                                                                         \
+  lora_shrink_kernel<T, RT, L><<<shrink, 64 * kShrinkWaves, 0, st>>>(gs, (const T*)x, x_stride, (const T*)a, t, K, \
                                                                      (int)R, p.k_slice, p.rows)
-#define MK_EXPAND(T, RT, V)                                                                                      \
-  lora_expand_kernel<T, RT, V><<<expand, 256, 0, st>>>(gs, (const T*)base, base_stride, (const T*)b, scales, t, \
-                                                       (T*)out, out_stride, N, (int)R, p.slices, p.blocks, wide)
-#define MK_LORA(T, RT)                  \
-  do {                                  \
-    if (vec_a) MK_SHRINK(T, RT, true);  \
-    else MK_SHRINK(T, RT, false);       \
-    if (vec_b) MK_EXPAND(T, RT, true);  \
-    else MK_EXPAND(T, RT, false);       \
+#define MK_EXPAND(T, RT, L)                                                                                      \
+  lora_expand_kernel<T, RT, L><<<expand, 256, 0, st>>>(gs, (const T*)base, base_stride, (const T*)b, scales, t, \
+                                                       (T*)out, out_stride, N, (int)R, p.slices, p.blocks)
+#define MK_LORA(T, RT)                                  \
+  do {                                                  \
+    if (len_a == kWhole) MK_SHRINK(T, RT, kWhole);      \
+    else if (len_a == kRest) MK_SHRINK(T, RT, kRest);   \
+    else MK_SHRINK(T, RT, kFew);                        \
+    if (len_b == kWhole) MK_EXPAND(T, RT, kWhole);      \
+    else if (RT > 1 || len_b == kRest) MK_EXPAND(T, RT, kRest); \
+    else MK_EXPAND(T, 1, kFew);                         \
   } while (0)
 #define MK_LORA_RANK(T)                         \
   do {                                          \

@@ -185,3 +185,25 @@ def test_infinity_beside_large_sums(dev, M):
     a[0, 2, 7], b[0, 32:, 2] = float("inf"), 2.0 ** -5
     got = lo.lora_add(*on(dev, x, base, a, b, torch.zeros(M, dtype=torch.int32))).cpu()
     assert (got == float("inf")).all()
+
+
+@pytest.mark.parametrize("M,N", [(1, 517), (1, 2), (40, 3), (64, 255), (64, 1030), (200, 93), (700, 1026)])
+def test_rows_without_an_adapter(dev, M, N):
+    """Most rows have none: copied bit by bit, from and to strided rows at any address, in place left alone."""
+    g = torch.Generator().manual_seed(M + N)
+    x, base = torch.randn(M, 24, generator=g).half().to(dev), torch.randn(M, N + 3, generator=g).half().to(dev)[:, 1:N + 1]
+    base[0, 0] = float("nan")
+    a, b = torch.randn(2, 4, 24, generator=g).half().to(dev), torch.randn(2, N, 4, generator=g).half().to(dev)
+    ids = torch.where(torch.rand(M, generator=g) < 0.9, -1, torch.randint(0, 2, (M,), generator=g)).to(torch.int32)
+    ids[0] = -1
+    out = torch.full((M, N + 2), 7.0, device=dev).half()
+    got = lo.lora_add(x, base, a, b, ids.to(dev), out=out[:, :N])
+    none = (ids < 0).to(dev)
+    bits = lambda t: t.contiguous().view(torch.int16)  # noqa: E731
+    assert torch.equal(bits(got[none]), bits(base[none])) and (out[:, N:] == 7).all()
+    if (~none).any():
+        keep = [t[~none].cpu() for t in (x, base)]
+        check_lora(got[~none], *keep, a.cpu(), b.cpu(), ids[ids >= 0], None)
+    before = base.clone()
+    assert lo.lora_add(x, base, a, b, ids.to(dev), out=base) is base
+    assert torch.equal(bits(base[none]), bits(before[none]))
