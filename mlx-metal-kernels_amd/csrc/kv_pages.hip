@@ -65,19 +65,30 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(PageTensors t, int tens
   }
 }
 
+// lanes of a page (their logarithm), 16 bytes each
+inline int page_lanes(int64_t bytes) {
+  int l = 4;
+  while (l < 8 && (16 << l) < bytes) ++l;
+  return l;
+}
+
 // the moves of all arrays, those of pages of one size class in a launch (at
 // most kMaxTensors of them); n: the most pairs that there can be
 int copy_pages(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors, const int32_t* src,
                const int32_t* dst, const int32_t* count, int64_t n, int64_t num_pages, hipStream_t st) {
-  for (int lgl = 4; lgl <= 8; ++lgl) {
+  // Few pages move all in one launch, with the lanes of the largest: 4 to 44
+  // pages of 46 arrays of codes and 46 of scales in 35.8 us a call, 39.5 in two
+  // (509 pages of the scales alone take 13 us more with a workgroup a page).
+  const bool few = n * num_tensors <= 4096;
+  int64_t largest = 0;
+  for (int64_t i = 0; i < num_tensors; ++i) largest = page_bytes[i] > largest ? page_bytes[i] : largest;
+  for (int lgl = few ? page_lanes(largest) : 4; lgl <= 8; ++lgl) {
     int64_t at = 0;
     while (at < num_tensors) {
       PageTensors t = {};
       int k = 0;
       for (; at < num_tensors && k < kMaxTensors; ++at) {
-        int l = 4;
-        while (l < 8 && (16 << l) < page_bytes[at]) ++l;
-        if (l != lgl || page_bytes[at] == 0) continue;
+        if ((!few && page_lanes(page_bytes[at]) != lgl) || page_bytes[at] == 0) continue;
         t.base[k] = reinterpret_cast<uint8_t*>(tensors[at]);
         t.bytes[k++] = page_bytes[at];
       }
@@ -91,6 +102,7 @@ int copy_pages(void* const* tensors, const int64_t* page_bytes, int64_t num_tens
                                                                              num_pages);
       MK_CHECK_LAUNCH();
     }
+    if (few) break;
   }
   return MK_OK;
 }

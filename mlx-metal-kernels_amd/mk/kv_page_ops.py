@@ -18,7 +18,6 @@ equal inputs give equal tables.
 from __future__ import annotations
 
 from array import array
-from operator import attrgetter
 
 import torch
 
@@ -27,7 +26,7 @@ from ._common import ci_safe_mode_enabled, narrow_i32
 from .kv_cache_ops import host_checks_enabled
 
 MAX_ROWS = 4096  # rows of a forked table
-_SHAPE, _NBYTES = attrgetter("shape"), attrgetter("nbytes")
+_SHAPE, _NBYTES = torch.Tensor.shape.__get__, torch.Tensor.nbytes.__get__  # (as functions of a tensor)
 
 
 def _backend(backend: str) -> bool:
