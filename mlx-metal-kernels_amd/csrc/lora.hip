@@ -560,13 +560,24 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (m >= 0) {
       const float* tr = t + (int64_t)m * L::RP + 8 * c;
-      for (int z = 0; z < slices; ++z, tr += gs.M * L::RP) {
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(tr), hi = *reinterpret_cast<const f32x4*>(tr + 4);
+      const int64_t step = gs.M * L::RP;
+      for (int z = 0; z < slices; z += 4) {  // four slices on their way together
+        f32x4 lo[4], hi[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] += lo[e];
-          v[4 + e] += hi[e];
+        for (int u = 0; u < 4; ++u) {
+          lo[u] = hi[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (z + u < slices) {
+            lo[u] = *reinterpret_cast<const f32x4*>(tr + (z + u) * step);
+            hi[u] = *reinterpret_cast<const f32x4*>(tr + (z + u) * step + 4);
+          }
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] += lo[u][e];
+            v[4 + e] += hi[u][e];
+          }
       }
     }
     l.put(i, c, v, scale, at < chunks);
