@@ -596,9 +596,9 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(Groups gs, const T* ba
 // has every 8th rank, and reads a kilobyte of a row at a time.  That costs the
 // workgroup K ranks x 2 bytes from the L2, and saves a launch and the way
 // through memory.  One launch against two, us a call in a graph (the host's time
-// falls from 18 to 14 us): K 4096, rank 16: 5.3 / 7.2; K 4096, rank 32: 6.6 /
-// 8.4; K 14336, rank 16: 8.8 / 8.9; K 8192, rank 32: 9.0 / 9.5; K 14336, rank
-// 32: 14.4 / 11.0.  (Two rows at K 4096, rank 16 would take 10.2 / 7.6: the
+// falls from 18 to 14 us): K 4096, rank 16: 5.2 / 6.9; K 4096, rank 32: 6.6 /
+// 7.4; K 14336, rank 16: 8.8 / 8.3; K 8192, rank 32: 9.0 / 8.3; K 14336, rank
+// 32: 14.3 / 9.3.  (Two rows at K 4096, rank 16 would take 10.2 / 7.6: the
 // matrix cores are the better way for more.)
 // ---------------------------------------------------------------------------
 
@@ -687,9 +687,14 @@ inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t ad
   // 17.5 / 19.5, of rank 128 31.4 / 35.1; 2000 rows 24.0 / 24.9, 41.9 / 42.8;
   // 4093 rows 36.2 / 34.1, 70.6 / 61.0.
   p.rows = M > kGroupRows && M <= 2048 ? 32 : kGroupRows;
-  // K in slices of four turns of a workgroup where there are few of them
+  // K in slices where there are few workgroups: of four turns, or of two while
+  // there are no more than 8 of them.  Two / four / eight turns, us a call: 32
+  // rows of K 4096, rank 64: 10.0 / 11.4 / 15.8, of rank 16: 8.0 / 8.2 / 9.6; 8
+  // rows of K 14336, rank 16 (28, 14 and 7 slices to join): 9.5 / 8.8 / 9.1.
   const int64_t turn = 32 * kShrinkWaves;
   int64_t s = (K + 4 * turn - 1) / (4 * turn);
+  const int64_t two = (K + 2 * turn - 1) / (2 * turn);
+  if (s < 8) s = two < 8 ? two : 8;
   const int64_t full = (M + kGroupRows - 1) / kGroupRows;
   const int64_t fill = 256 / ((M + p.rows - 1) / p.rows + kinds);  // one round of a workgroup for each CU
   if (s > fill) s = fill > 1 ? fill : 1;
