@@ -5,8 +5,9 @@
 // No counterpart in the reference.  The rows of one adapter, up to 64 of them,
 // are a group.  One launch sums t = A_i x[m] of a group's rows in fp32 (in
 // slices of K, kept in the workspace), the next joins the slices, multiplies
-// by B_i and adds base, with one rounding.  Up to 64 rows a wave finds its
-// group by itself; beyond, a launch before them lists the groups.  So every
+// by B_i and adds base, with one rounding.  Up to 64 rows, or 256 of few
+// adapters, a wave finds its group by itself; beyond, a launch before them
+// lists the groups.  So every
 // adapter's matrices are read once for 64 rows, whatever the rows' order.
 //
 // Both products run on 16x16x32 matrix instructions with the rows as columns:
@@ -99,26 +100,84 @@ __device__ __forceinline__ typename Frag<T>::v8 load_frag(const T* p, int64_t at
 // ---------------------------------------------------------------------------
 
 constexpr int kGroupRows = 64;
+// What a wave groups by itself beyond 64 rows.  Against a launch that lists the
+// groups, K and N 4096, rank 16, us a call: 100 rows of 5 adapters 11.2 / 14.0,
+// of 8 11.3 / 13.9, of 15 16.4 / 14.1; 256 rows 13.0 / 15.5, 14.1 / 15.6, 19.2
+// / 15.7.
+constexpr int kWaveRows = 256, kWaveAdapters = 8;
 constexpr int kMaxAdapters = 4096;
 
 struct Groups {
   const int32_t* ids;
-  const int32_t* rows;      // [groups, 64], -1 behind a group's rows; NULL: up to 64 rows in all
+  const int32_t* rows;      // [groups, 64], -1 behind a group's rows; NULL: the waves look for them
   const int32_t* adapters;  // [groups + 1]: the adapter of each (-1: none), in front of them their number
   int64_t M;
   int count;  // of adapters
 };
 
+// Group g of 65 to 256 rows, by a wave: adapters in the order of their first
+// rows, the rows of each in order.
+__device__ __forceinline__ int sort_out(const Groups& gs, int g, int* adapter, int* row) {
+  constexpr int J = kWaveRows / 64;
+  const int lane = threadIdx.x & 63;
+  const uint64_t below = (1ull << lane) - 1;
+  int id[J];
+  uint64_t rest[J], have[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) id[j] = lane + 64 * j < gs.M ? gs.ids[lane + 64 * j] : -1;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    if (id[j] < 0 || id[j] >= gs.count) id[j] = -1;
+    rest[j] = __ballot(lane + 64 * j < gs.M);
+  }
+  for (;;) {
+    bool any = false;
+    int n = 0;
+#pragma unroll
+    for (int j = J - 1; j >= 0; --j)
+      if (rest[j]) {
+        *adapter = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(rest[j]));
+        any = true;
+      }
+    if (!any) return 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      have[j] = __ballot(id[j] == *adapter) & rest[j];
+      rest[j] &= ~have[j];
+      n += __builtin_popcountll(have[j]);
+    }
+    const int groups = (n + kGroupRows - 1) / kGroupRows;
+    if (g < groups) break;
+    g -= groups;
+  }
+  // the rows from 64 g on of those, the i-th to lane i; every lane sends, the others to the lanes that take nothing
+  int before = -kGroupRows * g;
+  *row = -1;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int rank = before + __builtin_popcountll(have[j] & below);
+    const bool in = (have[j] >> lane) & 1 && rank >= 0 && rank < kGroupRows;
+    const uint64_t members = __ballot(in);
+    const int first = before > 0 ? before : 0, k = __builtin_popcountll(members);
+    const int to = in ? rank : (first + k + __builtin_popcountll(~members & below)) & 63;
+    const int got = __builtin_amdgcn_ds_permute(4 * to, lane + 64 * j);
+    if (lane >= first && lane < first + k) *row = got;
+    before += __builtin_popcountll(have[j]);
+  }
+  return before < kGroupRows ? before : kGroupRows;
+}
+
 // Group g: its adapter (-1: rows without one), its rows (row i in lane i, -1
 // behind them), their number (0: there is no such group).  Uniform but `row`.
 __device__ __forceinline__ int find_group(const Groups& gs, int g, int* adapter, int* row) {
-  const int lane = threadIdx.x & 63;
   if (gs.rows) {
     if (g >= gs.adapters[0]) return 0;
     *adapter = gs.adapters[1 + g];
-    *row = gs.rows[(int64_t)g * kGroupRows + lane];
+    *row = gs.rows[(int64_t)g * kGroupRows + (threadIdx.x & 63)];
     return __builtin_popcountll(__ballot(*row >= 0));
   }
+  if (gs.M > kGroupRows) return sort_out(gs, g, adapter, row);
+  const int lane = threadIdx.x & 63;
   int id = lane < gs.M ? gs.ids[lane] : -1;
   if (id < 0 || id >= gs.count) id = -1;
   uint64_t rest = __ballot(lane < gs.M), have = 0;
@@ -137,7 +196,7 @@ __device__ __forceinline__ int find_group(const Groups& gs, int g, int* adapter,
   return n;
 }
 
-// The groups of more than 64 rows, by one workgroup.  Rows of an adapter take
+// The groups of more rows, by one workgroup.  Rows of an adapter take
 // places in the order in which the threads get there: which rows share a group
 // changes no result.
 __global__ __launch_bounds__(1024) void lora_group_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ rows,
@@ -672,7 +731,8 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(const int32_t*
 struct LoraPlan {
   int64_t groups, k_slice, order_ints;  // most groups that there can be
   int slices, rank_tiles, blocks, rows;  // rows of a workgroup of the first product
-  bool one;  // one launch, no workspace
+  bool one;   // one launch, no workspace
+  bool list;  // a launch that lists the groups
 };
 
 inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t adapters) {
@@ -680,8 +740,9 @@ inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t ad
   p.rank_tiles = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
   const int64_t kinds = adapters + 1 < M ? adapters + 1 : M;  // adapters that rows can name, and none
   p.one = M == 1 && R <= 32 && K >= 8 && K * p.rank_tiles <= 16384;
+  p.list = M > kWaveRows || (M > kGroupRows && adapters > kWaveAdapters);
   p.groups = M <= kGroupRows ? kinds : M / kGroupRows + kinds;
-  p.order_ints = M <= kGroupRows ? 0 : (p.groups * (kGroupRows + 1) + 1 + 3) / 4 * 4;
+  p.order_ints = !p.list ? 0 : (p.groups * (kGroupRows + 1) + 1 + 3) / 4 * 4;
   // Half a group is more workgroups and reads A twice as often; K 4096, N 4096,
   // 5 adapters, 32 / 64 rows of a workgroup, us a call: 500 rows of rank 16
   // 17.5 / 19.5, of rank 128 31.4 / 35.1; 2000 rows 24.0 / 24.9, 41.9 / 42.8;
@@ -740,7 +801,7 @@ int mk_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_
   float* t = reinterpret_cast<float*>(workspace) + p.order_ints;
   const Len len_a = len_of(K), len_b = len_of(R);
   Groups gs = {adapter_ids, nullptr, nullptr, M, (int)adapters};
-  if (M > kGroupRows) {
+  if (p.list) {
     gs.rows = order;
     gs.adapters = order + p.groups * kGroupRows;
     lora_group_kernel<<<1, 1024, 0, st>>>(adapter_ids, order, order + p.groups * kGroupRows, M, (int)adapters);

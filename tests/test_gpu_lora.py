@@ -207,3 +207,23 @@ def test_rows_without_an_adapter(dev, M, N):
     before = base.clone()
     assert lo.lora_add(x, base, a, b, ids.to(dev), out=base) is base
     assert torch.equal(bits(base[none]), bits(before[none]))
+
+
+@pytest.mark.parametrize("M", [63, 64, 65, 128, 129, 192, 255, 256, 257])
+@pytest.mark.parametrize("adapters", [1, 2, 70, 300])
+def test_groups(dev, M, adapters):
+    """Every number of adapters in a batch, each of one row to all of them, in any order."""
+    g = torch.Generator().manual_seed(M + adapters)
+    x, base, a, b, _, s = lora_case(M, M, 40, 16, 8, adapters, torch.float16)
+    few = torch.randint(-1, adapters, (3,), generator=g)
+    for ids in (torch.randint(-1, adapters, (M,), generator=g), few[torch.randint(0, 3, (M,), generator=g)],
+                torch.full((M,), adapters - 1), torch.full((M,), -1), torch.arange(M) % adapters,
+                torch.where(torch.arange(M) == M - 1, 0, -1), torch.arange(M).flip(0) // 67 % (adapters + 1) - 1):
+        ids = ids.to(torch.int32)
+        check_lora(lo.lora_add(*on(dev, x, base, a, b, ids), scales=s.to(dev)), x, base, a, b, ids, s)
+
+
+def test_many_adapters_of_many_rows(dev):
+    case = lora_case(9, 600, 16, 24, 3, 4096, torch.bfloat16)
+    x, base, a, b, ids, s = on(dev, *case)
+    check_lora(lo.lora_add(x, base, a, b, ids, scales=s), *case)
