@@ -743,11 +743,11 @@ inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t ad
   p.list = M > kWaveRows || (M > kGroupRows && adapters > kWaveAdapters);
   p.groups = M <= kGroupRows ? kinds : M / kGroupRows + kinds;
   p.order_ints = !p.list ? 0 : (p.groups * (kGroupRows + 1) + 1 + 3) / 4 * 4;
-  // Half a group is more workgroups and reads A twice as often; K 4096, N 4096,
-  // 5 adapters, 32 / 64 rows of a workgroup, us a call: 500 rows of rank 16
-  // 17.5 / 19.5, of rank 128 31.4 / 35.1; 2000 rows 24.0 / 24.9, 41.9 / 42.8;
-  // 4093 rows 36.2 / 34.1, 70.6 / 61.0.
-  p.rows = M > kGroupRows && M <= 2048 ? 32 : kGroupRows;
+  // Half a group is more workgroups and reads A twice as often; N 4096, 32 / 64
+  // rows of a workgroup, us a call: K 4096: 500 rows of rank 16 17.5 / 19.5, of
+  // rank 128 31.4 / 35.1; 1000 rows 20.1 / 22.1, 35.4 / 39.1; 2000 rows 24.0 /
+  // 24.9, 41.9 / 42.8; K 8192, 2000 rows of rank 128 43.2 / 37.4.
+  p.rows = M > kGroupRows && M <= 1024 ? 32 : kGroupRows;
   // K in slices where there are few workgroups: of four turns, or of two while
   // there are no more than 8 of them.  Two / four / eight turns, us a call: 32
   // rows of K 4096, rank 64: 10.0 / 11.4 / 15.8, of rank 16: 8.0 / 8.2 / 9.6; 8
@@ -762,13 +762,11 @@ inline LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t R, int64_t ad
   p.k_slice = (K + s - 1) / s;
   p.k_slice = (p.k_slice + turn - 1) / turn * turn;
   p.slices = (int)((K + p.k_slice - 1) / p.k_slice);
-  // Outputs of a workgroup: joining t and finding the group count less over
-  // more of them, and fewer workgroups fill the CUs less.  256 against 512
-  // outputs (us a call): 512 rows x 6144, rank 16 (192 workgroups of 256):
-  // 21.4 / 24.0; 2000 rows x 8192, rank 128 (1024): 74.5 / 62.8; 4093 rows x
-  // 14336, rank 64 (3584): 90.3 / 89.7 (and 90.7 with 1024).
-  const int64_t work = (N + 255) / 256 * full;
-  p.blocks = work >= 1024 ? 2 : 1;
+  // Outputs of a workgroup, 512 against 256: joining t and finding the group
+  // count less, and fewer workgroups fill the CUs less.  us a call: 8192 rows x
+  // 14336, rank 128: 177 / 187; x 4096, rank 128: 120 / 118; 4093 rows x 14336,
+  // rank 16: 70.2 / 67.2; 8192 x 8192, rank 32: 85.4 / 82.5.
+  p.blocks = R > 64 && (N + 255) / 256 * full >= 4096 ? 2 : 1;
   return p;
 }
 

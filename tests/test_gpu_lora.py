@@ -227,3 +227,17 @@ def test_many_adapters_of_many_rows(dev):
     case = lora_case(9, 600, 16, 24, 3, 4096, torch.bfloat16)
     x, base, a, b, ids, s = on(dev, *case)
     check_lora(lo.lora_add(x, base, a, b, ids, scales=s), *case)
+
+
+@pytest.mark.parametrize("M,N,R", [(4100, 16390, 72), (9000, 8191, 128), (5000, 4100, 8)])
+def test_many_rows(dev, M, N, R):
+    """Prompts of thousands of rows: some of them against the oracle, rows without an adapter in between."""
+    g = torch.Generator(device=dev).manual_seed(M)
+    rand = lambda *s: torch.randn(*s, generator=g, device=dev).bfloat16()  # noqa: E731
+    x, base, a, b = rand(M, 40), rand(M, N), rand(3, R, 40), (rand(3, N, R) / 8)
+    ids = torch.arange(M, device=dev) // 700 % 4 - 1
+    got = lo.lora_add(x, base, a, b, ids)
+    some = torch.randperm(M, generator=g, device=dev)[:40]
+    some = torch.cat([some, torch.tensor([0, 1, M - 2, M - 1], device=dev)])
+    check_lora(got[some], *(t.cpu() for t in (x[some], base[some], a, b, ids[some])), None)
+    assert torch.equal(got[ids < 0], base[ids < 0])
