@@ -15,31 +15,42 @@
 namespace {
 
 constexpr int kMaxTensors = 128;  // tensors of one launch: their addresses travel as kernel arguments
+constexpr int kClasses = 5;       // lanes that move a page: 16, 32, .. 256
 
 struct PageTensors {
   uint8_t* base[kMaxTensors];
   int64_t bytes[kMaxTensors];  // of a page
+  int first[kClasses + 1];     // class c has the tensors from first[c] to first[c + 1]
 };
 
 // Pages src[i] -> dst[i], i < m, in every array: m = *count (n where count is
 // NULL), src = dst + m where src is NULL.  Entries outside [0, num_pages) and
-// pages onto themselves are skipped.  1 << lgl lanes move a page, so a
-// workgroup takes 256 >> lgl of an array (509 pages of 256 bytes in 64 arrays:
-// 5.7 us, 19 with a workgroup a page).  Where the device knows their number,
-// workgroups go round until all are done: those of empty entries would cost a
-// trip to memory each (11 pages of 64 arrays in a list of 32: 16 us).
-__global__ __launch_bounds__(256) void copy_pages_kernel(PageTensors t, int tensors, const int32_t* __restrict__ src,
+// pages onto themselves are skipped.  A page is moved by lanes of 16 bytes, at
+// most 256 of them, and a workgroup takes several small pages of an array (509
+// pages of 256 bytes in 64 arrays: 5.7 us, 19 with a workgroup a page); the
+// large pages come first.  Where the device knows their number, workgroups go
+// round until all are done: those of empty entries would cost a trip to memory
+// each (11 pages of 64 arrays in a list of 32: 16 us).
+__global__ __launch_bounds__(256) void copy_pages_kernel(PageTensors t, const int32_t* __restrict__ src,
                                                          const int32_t* __restrict__ dst,
-                                                         const int32_t* __restrict__ count, int n, int lgl,
+                                                         const int32_t* __restrict__ count, int n,
                                                          int64_t num_pages) {
   const int m = count ? min(*count, n) : n;
   if (!src) src = dst + m;
-  const int lane = threadIdx.x & ((1 << lgl) - 1), lanes = 1 << lgl;
-  const int per = 256 >> lgl;
-  const int64_t work = (int64_t)((m + per - 1) / per) * tensors;
-  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
-    const int batch = (int)(w / tensors), k = (int)(w - (int64_t)batch * tensors);
-    const int i = batch * per + ((int)threadIdx.x >> lgl);
+  for (int64_t w = blockIdx.x;; w += gridDim.x) {
+    int c = kClasses - 1, tensors = 0, lgl = 0;
+    int64_t rest = w;
+    for (; c >= 0; --c) {
+      lgl = 4 + c;
+      tensors = t.first[c + 1] - t.first[c];
+      const int64_t work = (int64_t)((m + (256 >> lgl) - 1) >> (8 - lgl)) * tensors;
+      if (rest < work) break;
+      rest -= work;
+    }
+    if (c < 0) return;
+    const int lane = threadIdx.x & ((1 << lgl) - 1), lanes = 1 << lgl;
+    const int batch = (int)(rest / tensors), k = t.first[c] + (int)(rest - (int64_t)batch * tensors);
+    const int i = (batch << (8 - lgl)) + ((int)threadIdx.x >> lgl);
     if (i >= m) continue;
     const int64_t a = src[i], b = dst[i];
     if (a < 0 || a >= num_pages || b < 0 || b >= num_pages || a == b) continue;
@@ -65,44 +76,40 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(PageTensors t, int tens
   }
 }
 
-// lanes of a page (their logarithm), 16 bytes each
-inline int page_lanes(int64_t bytes) {
-  int l = 4;
-  while (l < 8 && (16 << l) < bytes) ++l;
-  return l;
+// class of a page of so many bytes
+inline int page_class(int64_t bytes) {
+  int c = 0;
+  while (c < kClasses - 1 && (256 << c) < bytes) ++c;
+  return c;
 }
 
-// the moves of all arrays, those of pages of one size class in a launch (at
-// most kMaxTensors of them); n: the most pairs that there can be
+// The moves of all arrays, kMaxTensors of them in a launch, whatever their pages'
+// sizes (4 to 44 pages of 46 arrays of codes and 46 of scales: 35.8 us a call,
+// 39.5 with a launch for each size); n: the most pairs that there can be.
 int copy_pages(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors, const int32_t* src,
                const int32_t* dst, const int32_t* count, int64_t n, int64_t num_pages, hipStream_t st) {
-  // Few pages move all in one launch, with the lanes of the largest: 4 to 44
-  // pages of 46 arrays of codes and 46 of scales in 35.8 us a call, 39.5 in two
-  // (509 pages of the scales alone take 13 us more with a workgroup a page).
-  const bool few = n * num_tensors <= 4096;
-  int64_t largest = 0;
-  for (int64_t i = 0; i < num_tensors; ++i) largest = page_bytes[i] > largest ? page_bytes[i] : largest;
-  for (int lgl = few ? page_lanes(largest) : 4; lgl <= 8; ++lgl) {
-    int64_t at = 0;
-    while (at < num_tensors) {
-      PageTensors t = {};
-      int k = 0;
-      for (; at < num_tensors && k < kMaxTensors; ++at) {
-        if ((!few && page_lanes(page_bytes[at]) != lgl) || page_bytes[at] == 0) continue;
-        t.base[k] = reinterpret_cast<uint8_t*>(tensors[at]);
-        t.bytes[k++] = page_bytes[at];
+  for (int64_t at = 0; at < num_tensors; at += kMaxTensors) {
+    const int64_t end = at + kMaxTensors < num_tensors ? at + kMaxTensors : num_tensors;
+    PageTensors t = {};
+    int k = 0;
+    int64_t work = 0;
+    for (int c = 0; c < kClasses; ++c) {
+      t.first[c] = k;
+      for (int64_t i = at; i < end; ++i) {
+        if (page_bytes[i] == 0 || page_class(page_bytes[i]) != c) continue;
+        t.base[k] = reinterpret_cast<uint8_t*>(tensors[i]);
+        t.bytes[k++] = page_bytes[i];
       }
-      if (k == 0) break;
-      const int64_t work = (n + (256 >> lgl) - 1) / (256 >> lgl) * k;
-      // a workgroup for each piece of a known number of pages (64 x 509 pages of
-      // 16 KB: 202 us, 225 with 2048 workgroups going round), else as many as
-      // the CUs hold at a time
-      const int64_t most = count ? 2048 : 1 << 20;
-      copy_pages_kernel<<<(unsigned)(work < most ? work : most), 256, 0, st>>>(t, k, src, dst, count, (int)n, lgl,
-                                                                             num_pages);
-      MK_CHECK_LAUNCH();
+      work += ((n + (16 >> c) - 1) / (16 >> c)) * (k - t.first[c]);
     }
-    if (few) break;
+    t.first[kClasses] = k;
+    if (k == 0) continue;
+    // a workgroup for each piece of a known number of pages (64 x 509 pages of
+    // 16 KB: 202 us, 225 with 2048 workgroups going round), else as many as
+    // the CUs hold at a time
+    const int64_t most = count ? 2048 : 1 << 20;
+    copy_pages_kernel<<<(unsigned)(work < most ? work : most), 256, 0, st>>>(t, src, dst, count, (int)n, num_pages);
+    MK_CHECK_LAUNCH();
   }
   return MK_OK;
 }
