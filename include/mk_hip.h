@@ -220,9 +220,10 @@ int mk_q8_rmsnorm_qkv_rope_paged(const void* x, const void* norm_w, float eps, c
  * for i = adapter_ids[m], base[m] where i is outside [0, adapters).  x [M,K],
  * base and out [M,N] at strides in values (out may be base); a [adapters,R,K],
  * b [adapters,N,R], all in dtype (fp16 / bf16); scales fp32 [adapters] (NULL:
- * 1); 1 <= R <= 128, 1 <= adapters <= 4096.  Sums in fp32, one rounding.  The workspace (16-byte
- * aligned, any content) has mk_lora_workspace_bytes(M, N, K, R, adapters)
- * bytes (0: none needed); calls that may run concurrently need distinct ones. */
+ * 1); M < 2^20, N < 2^24, 1 <= R <= 128, 1 <= adapters <= 4096.  Sums in fp32,
+ * one rounding.  The workspace (16-byte aligned, any content) has
+ * mk_lora_workspace_bytes(M, N, K, R, adapters) bytes (0: none needed); calls
+ * that may run concurrently need distinct ones. */
 size_t mk_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t adapters);
 int mk_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_stride, const void* a, const void* b,
                 const int32_t* adapter_ids, const float* scales, void* out, int64_t out_stride, int64_t M, int64_t N,

@@ -7,8 +7,13 @@
 // slices of K, kept in the workspace), the next joins the slices, multiplies
 // by B_i and adds base, with one rounding.  Up to 64 rows, or 256 of few
 // adapters, a wave finds its group by itself; beyond, a launch before them
-// lists the groups.  So every
-// adapter's matrices are read once for 64 rows, whatever the rows' order.
+// lists the groups.  So every adapter's matrices are read once for 64 rows,
+// whatever the rows' order.  A single row of few ranks takes one launch.
+//
+// Few rows are bound by trips to memory one after another (32 rows, K 4096, N
+// 6144, rank 16: 4.2 and 5.1 us for 3.7 MB), many by the streams of x, base and
+// out: 4093 rows, K 4096, N 14336, rank 64: 7, 18 and 60 us for 280 MB, which a
+// copy moves in 52.
 //
 // Both products run on 16x16x32 matrix instructions with the rows as columns:
 // a row's values touch no other row (an infinity or NaN stays where it is),
