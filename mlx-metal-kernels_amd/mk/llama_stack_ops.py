@@ -21,6 +21,7 @@ from typing import Any
 import torch
 
 from . import _lib
+from ._common import narrow_i32
 from .llama_layer_ops import (
     LlamaLayerKernelWeights,
     LlamaLikeConfig,
@@ -178,6 +179,8 @@ def llama_stack_decode_step(x, stack_weights: LlamaStackWeights, stack_cache: Ll
         if lengths is None:
             raise ValueError("verify_width needs per-row positions as a device tensor")
         lengths = lengths[verify_width - 1::verify_width].contiguous()  # per sequence: the last row's + 1
+    if isinstance(adapter_ids, torch.Tensor):
+        adapter_ids = narrow_i32(adapter_ids, x.device)  # once for all layers
     for li, lw in enumerate(stack_weights.layers):
         if reference:
             hidden, cache = reference_llama_layer_decode_step(hidden, lw, stack_cache.layer_caches[li], cos, sin,
@@ -217,12 +220,14 @@ def llama_stack_decode_step(x, stack_weights: LlamaStackWeights, stack_cache: Ll
 
 def llama_stack_decode_loop(inputs, stack_weights: LlamaStackWeights, stack_cache: LlamaStackCache, cos, sin,
                             config: LlamaLikeConfig, *, backend_preset: str = "fused_experimental",
-                            cache_layout: str = "contiguous", T: int | None = None, return_logits: bool = True):
+                            cache_layout: str = "contiguous", T: int | None = None, return_logits: bool = True,
+                            adapter_ids=None):
     """ops/llama_stack_ops.py:439-495: decode inputs [B, T, hidden] (or
     [B, T, 1, hidden]) one step at a time, step t at position t of every
     sequence.  Returns (logits [B, T, vocab] -- or the final hidden states
     when ``return_logits`` is False or there is no head -- and the final
-    cache).  Preset "reference" runs the torch reference path."""
+    cache).  Preset "reference" runs the torch reference path.  ``adapter_ids``
+    as in llama_stack_decode_step."""
     if inputs.ndim == 4:
         if inputs.shape[2] != 1:
             raise ValueError(f"inputs with rank 4 must have shape [B,T,1,H], got {tuple(inputs.shape)}")
@@ -241,7 +246,7 @@ def llama_stack_decode_loop(inputs, stack_weights: LlamaStackWeights, stack_cach
     running = stack_cache
     for t in range(T):
         result = llama_stack_decode_step(inputs[:, t:t + 1, :], stack_weights, running, cos, sin, t, config,
-                                         reference=backend_preset == "reference")
+                                         reference=backend_preset == "reference", adapter_ids=adapter_ids)
         if stack_weights.lm_head is None:
             out_t, running = result
         else:
@@ -254,10 +259,11 @@ def llama_stack_decode_loop(inputs, stack_weights: LlamaStackWeights, stack_cach
 
 def reference_llama_stack_decode_loop(inputs, stack_weights: LlamaStackWeights, stack_cache: LlamaStackCache, cos,
                                       sin, config: LlamaLikeConfig, *, cache_layout: str = "contiguous",
-                                      T: int | None = None, return_logits: bool = True):
+                                      T: int | None = None, return_logits: bool = True, adapter_ids=None):
     """ops/llama_stack_ops.py:413-436."""
     return llama_stack_decode_loop(inputs, stack_weights, stack_cache, cos, sin, config, backend_preset="reference",
-                                   cache_layout=cache_layout, T=T, return_logits=return_logits)
+                                   cache_layout=cache_layout, T=T, return_logits=return_logits,
+                                   adapter_ids=adapter_ids)
 
 
 def _random_linear(out_dim, in_dim, bits, group_size, gen, device, dtype):

@@ -231,6 +231,17 @@ def rmsnorm_qkv_rope_paged_update(x2d, norm_weight, qkv_w, qkv_scales, qkv_zeros
     return q_out, pos
 
 
+def _verify_rows(q, K_pages, V_pages, block_table, lengths, scale, W):
+    """Attention of B * W draft rows over the B sequences' own table rows; ``lengths`` per sequence."""
+    from .speculative_verify_ops import _hip_verify_attention
+
+    rows, _, H, D = q.shape
+    if lengths is None or rows % W:
+        raise ValueError("verify_width needs B * W rows and per-sequence lengths")
+    return _hip_verify_attention(q.reshape(-1, W, H, D), K_pages, V_pages, block_table[::W].contiguous(), lengths,
+                                 scale).reshape(rows, 1, H, D)
+
+
 def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_pages, V_pages, block_table, cos, sin,
                                  position, *, qkv_zeros=None, out_zeros=None, bits=4, group_size=32, H=None,
                                  num_key_value_heads=None, head_dim=None, D=None, scale=None,
@@ -283,14 +294,7 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
             eps=eps)
         sc = 1.0 / math.sqrt(D) if scale is None else scale
         if verify_width > 1:
-            from .speculative_verify_ops import _hip_verify_attention
-
-            W = verify_width
-            if lengths is None or q.shape[0] % W:
-                raise ValueError("verify_width needs B * W rows and per-sequence lengths")
-            bt_seq = block_table[::W].contiguous()
-            attn_out = _hip_verify_attention(q.reshape(-1, W, H, D), K_pages, V_pages, bt_seq, lengths,
-                                             sc).reshape(q.shape[0], 1, H, D)
+            attn_out = _verify_rows(q, K_pages, V_pages, block_table, lengths, sc, verify_width)
         else:
             attn_out = _hip_paged_attention(q[:, 0], K_pages, V_pages, _i32(block_table, q.device),
                                             pos + 1 if lengths is None else lengths, sc).unsqueeze(1)
@@ -317,9 +321,13 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
             qkv, K_pages, V_pages, block_table, cos, sin, position, num_attention_heads=H,
             num_key_value_heads=kv_heads, head_dim=D, q_weight=q_norm_weight, k_weight=k_norm_weight, eps=eps,
             layout=rope_layout, rotary_dim=rotary_dim, backend=plain)
-        if lengths is None or verify_width > 1:  # verify rows here: one sequence each
-            lengths = (position if isinstance(position, int) else torch.as_tensor(position)) + 1
-        attn_out = paged_gqa_decode_attention(q, K_pages, V_pages, block_table, lengths, scale, backend=plain)
+        if verify_width > 1 and plain == "auto":
+            attn_out = _verify_rows(q, K_pages, V_pages, block_table, lengths,
+                                    1.0 / math.sqrt(D) if scale is None else scale, verify_width)
+        else:
+            if lengths is None or verify_width > 1:  # verify rows here: one sequence each
+                lengths = (position if isinstance(position, int) else torch.as_tensor(position)) + 1
+            attn_out = paged_gqa_decode_attention(q, K_pages, V_pages, block_table, lengths, scale, backend=plain)
     elif block_fn is not None:
         attn_out, K_pages, V_pages = block_fn(qkv, K_pages, V_pages, block_table, cos, sin, position,
                                               num_attention_heads=H, num_key_value_heads=kv_heads, head_dim=D,

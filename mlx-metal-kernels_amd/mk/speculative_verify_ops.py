@@ -326,14 +326,15 @@ def _rows_cache(stack_cache: LlamaStackCache, B: int, W: int) -> LlamaStackCache
 
 
 def llama_stack_verify_step(x, stack_weights: LlamaStackWeights, stack_cache: LlamaStackCache, cos, sin, position,
-                            config: LlamaLikeConfig, *, float_logits: bool = True):
+                            config: LlamaLikeConfig, *, float_logits: bool = True, adapter_ids=None):
     """W draft rows per sequence through the whole stack in one pass: x
     [B, W, hidden], ``position`` [B] (int or tensor) the first draft's
     position.  Each layer writes the W rows' K/V at position + w (into the
     cache's own pages, in place) and attends with row w seeing up to its own
     position.  Returns (logits [B, W, vocab] or None without a head,
     final_hidden [B, W, hidden], stack_cache) -- what W staged
-    llama_stack_decode_step calls give, row by row."""
+    llama_stack_decode_step calls give, row by row.  ``adapter_ids``
+    (extension) int32 [B]: each sequence's low-rank adapter."""
     config = config.validate()
     if x.ndim != 3 or x.shape[2] != config.hidden_size:
         raise ValueError(f"x must have shape [B,W,{config.hidden_size}], got {tuple(x.shape)}")
@@ -341,8 +342,14 @@ def llama_stack_verify_step(x, stack_weights: LlamaStackWeights, stack_cache: Ll
     dev = _lib.require_device(x)
     p0 = normalize_positions(position, B, stack_cache.max_seq_len - W + 1, device=dev).to(torch.int32)
     pos_rows = (p0[:, None] + torch.arange(W, dtype=torch.int32, device=dev)[None, :]).reshape(B * W)
+    if adapter_ids is not None:
+        adapter_ids = torch.as_tensor(adapter_ids, device=dev)
+        if tuple(adapter_ids.shape) != (B,):
+            raise ValueError(f"adapter_ids must have shape [B]={(B,)}, got {tuple(adapter_ids.shape)}")
+        adapter_ids = adapter_ids[:, None].expand(B, W).reshape(B * W)
     res = llama_stack_decode_step(x.reshape(B * W, 1, H), stack_weights, _rows_cache(stack_cache, B, W), cos, sin,
-                                  pos_rows, config, float_logits=float_logits, verify_width=W)
+                                  pos_rows, config, float_logits=float_logits, verify_width=W,
+                                  adapter_ids=adapter_ids)
     if stack_weights.lm_head is None:
         fh, _ = res
         return None, fh.reshape(B, W, H), stack_cache
@@ -357,14 +364,15 @@ def _clone_cache(stack_cache: LlamaStackCache) -> LlamaStackCache:
 
 def parallel_verify_tokens(*, context_token_ids: list[int], proposed_token_ids: list[int], pipeline=None,
                            model_config=None, stack_weights=None, stack_cache=None, embedding=None, lm_head=None,
-                           cos=None, sin=None, position=None, verification_config=None
+                           cos=None, sin=None, position=None, verification_config=None, adapter_id=None
                            ) -> ParallelVerificationPassResult:
     """ops/speculative_verify_ops.py:161-296 for one sequence: the K drafts
     go through llama_stack_verify_step on a staged copy of the cache; the
     greedy targets, accept mask, accepted prefix and replacement token follow
     the reference's rules.  ``pipeline`` (an object with llama_config,
     stack_weights, model.embedding / model.lm_head and an optional _state)
-    is accepted as in the reference."""
+    is accepted as in the reference.  ``adapter_id`` (extension): the
+    sequence's low-rank adapter."""
     if pipeline is not None:
         model_config = pipeline.llama_config
         stack_weights = pipeline.stack_weights
@@ -392,7 +400,8 @@ def parallel_verify_tokens(*, context_token_ids: list[int], proposed_token_ids: 
     staged = _clone_cache(stack_cache)
     x = embed_proposed_tokens(proposed_token_ids, embedding, B=1)
     p = int(position)
-    logits, _, staged = llama_stack_verify_step(x, stack_weights, staged, cos, sin, p, model_config)
+    logits, _, staged = llama_stack_verify_step(x, stack_weights, staged, cos, sin, p, model_config,
+                                                adapter_ids=None if adapter_id is None else [int(adapter_id)])
     logits_list = [logits[0, i] for i in range(K)]
     targets = greedy_sample(logits[0]).cpu().tolist()  # first maximum per row, as np.argmax
     mask = compute_accept_mask(list(proposed_token_ids), targets, require_exact_match=True)

@@ -204,3 +204,67 @@ def test_numbers_past_32_bits(dev, monkeypatch):
     a, b = torch.ones(1, 2, 4, device=dev).half(), torch.ones(1, 8, 2, device=dev).half()
     out = lora_ops.lora_add(torch.ones(2, 4, device=dev).half(), base, a, b, ids(far, 0))
     assert torch.equal(out[0], base[0]) and (out[1] != base[1]).all()
+
+
+@pytest.mark.parametrize("W", [2, 5])
+@pytest.mark.parametrize("layout", ["paged", "contiguous"])
+def test_verify_step_with_adapters(dev, W, layout):
+    """One pass over W draft rows of three sequences, each with its adapter, against W staged steps; the bound of the
+    plain stack's own test."""
+    from mk.speculative_verify_ops import llama_stack_verify_step, parallel_verify_tokens
+
+    torch.manual_seed(W)
+    w, (cos, sin) = _weights(dev), _tables(dev)
+    B, S = 3, 64
+    first = [ll.init_llama_layer_cache(CFG, B, S, cache_layout=layout, device=dev) for _ in range(CFG.num_hidden_layers)]
+    for c in first:
+        for t in c[:2]:
+            t.copy_(torch.randn(t.shape, device=dev))
+    caches = [ls.LlamaStackCache([tuple(t.clone() for t in c) for c in first], layout, S, 16) for _ in range(2)]
+    x = torch.randn(B, W, CFG.hidden_size, device=dev).half()
+    pos = torch.tensor([0, 30, S - W], dtype=torch.int32, device=dev)
+    ids = torch.tensor([2, -1, 0], device=dev)
+    logits, _, caches[0] = llama_stack_verify_step(x, w, caches[0], cos, sin, pos, CFG, adapter_ids=ids)
+    staged = []
+    for i in range(W):
+        lg, _, caches[1] = ls.llama_stack_decode_step(x[:, i:i + 1], w, caches[1], cos, sin, pos + i, CFG, adapter_ids=ids)
+        staged.append(lg[:, 0])
+    staged = torch.stack(staged, 1).float()
+    rms = float(staged.square().mean().sqrt())
+    assert_close(logits.float().cpu().numpy() / rms, staged.cpu().numpy() / rms, atol=8 * 2.0 ** -11, what="verify")
+    # k and v are sums over 256 activations, and the passes' matvec kernels (for 3 and for 3 W rows) may round each to
+    # a neighbour, 2^-10 of it: a sum moves by up to 2^-10 sum |w a| = 2^-10 (2 / pi) sqrt(256) of its rms (products
+    # of normal values); a norm weight multiplies that, 1.8 at most.  (1e-3 flat, as for values of a single rounding,
+    # was below that: 4e-3 came.)
+    moves = 2.0 ** -10 * (2 / np.pi) * 16 * 1.8
+    for a, b in zip(caches[0].layer_caches, caches[1].layer_caches):
+        for s, t in zip(a[:2], b[:2]):
+            t = t.float().cpu().numpy()
+            assert_close(s, t, rtol=0, atol=moves * float(np.sqrt((t ** 2).mean())), what="cache")
+    with pytest.raises(ValueError, match="adapter_ids must have shape"):
+        llama_stack_verify_step(x, w, caches[0], cos, sin, pos, CFG, adapter_ids=ids[:2])
+    one = ls.LlamaStackCache([tuple(t[:1] for t in c) if layout == "contiguous" else (*c[:2], c[2][:1]) for c in first],
+                             layout, S, 16)
+    kw = dict(context_token_ids=[1], proposed_token_ids=[3] * W, model_config=CFG, stack_weights=w, stack_cache=one,
+              cos=cos, sin=sin, position=9)
+    with_a, without = (parallel_verify_tokens(**kw, adapter_id=i).logits[0] for i in (1, None))
+    assert not torch.equal(with_a, without)
+
+
+def test_decode_loop_with_adapters(dev):
+    w, (cos, sin) = _weights(dev), _tables(dev)
+    x = torch.randn(2, 3, CFG.hidden_size, device=dev).half()
+    ids = torch.tensor([1, -1], dtype=torch.int32, device=dev)
+
+    def cache():
+        return ls.LlamaStackCache([ll.init_llama_layer_cache(CFG, 2, 16, cache_layout="contiguous", device=dev)
+                                   for _ in range(CFG.num_hidden_layers)], "contiguous", 16, 16)
+
+    got, _ = ls.llama_stack_decode_loop(x, w, cache(), cos, sin, CFG, adapter_ids=ids)
+    plain, _ = ls.llama_stack_decode_loop(x, w, cache(), cos, sin, CFG)
+    assert not torch.equal(got[0], plain[0]) and torch.equal(got[1], plain[1])
+    want, run = [], cache()
+    for t in range(3):
+        lg, _, run = ls.llama_stack_decode_step(x[:, t:t + 1], w, run, cos, sin, t, CFG, adapter_ids=ids)
+        want.append(lg)
+    assert torch.equal(got, torch.cat(want, 1))
