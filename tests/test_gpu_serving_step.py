@@ -268,3 +268,69 @@ def test_decode_loop_with_adapters(dev):
         lg, _, run = ls.llama_stack_decode_step(x[:, t:t + 1], w, run, cos, sin, t, CFG, adapter_ids=ids)
         want.append(lg)
     assert torch.equal(got, torch.cat(want, 1))
+
+
+def test_two_streams_at_once(dev):
+    """Calls of two streams that run side by side share no workspace: each gives what it gives alone."""
+    g = torch.Generator(device=dev).manual_seed(5)
+    rand = lambda *s: torch.randn(*s, generator=g, device=dev).half()  # noqa: E731
+    work = []
+    for k in range(2):
+        x, base, a, b = rand(300, 512), rand(300, 1024), rand(20, 16, 512), rand(20, 1024, 16)
+        ids = torch.randint(-1, 20, (300,), generator=g, device=dev, dtype=torch.int32)
+        table = torch.randperm(9000, generator=g, device=dev)[:1200].reshape(300, 4).int()
+        lengths = torch.randint(1, 13, (300,), generator=g, device=dev, dtype=torch.int32)
+        parents = torch.randint(-1, 300, (300,), generator=g, device=dev, dtype=torch.int32)
+        refs = kv_page_ops.count_page_refs(table, 10000)
+        pages = [rand(10000, 4, 8)]
+        work.append((x, base, a, b, ids, table, lengths, parents, refs, pages))
+
+    def run(x, base, a, b, ids, table, lengths, parents, refs, pages):
+        pool = [t.clone() for t in pages]
+        out = lora_ops.lora_add(x, base, a, b, ids)
+        new = kv_page_ops.fork_kv_sequences(pool, table, lengths, refs, parents)
+        packed = kv_page_ops.compact_kv_pages(pool, new[0], new[2])
+        return [out, *new, *packed, *pool]
+
+    want = [run(*w) for w in work]
+    streams = [torch.cuda.Stream(dev) for _ in work]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(run(*work[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for one in got[k]:
+            assert all(torch.equal(p, q) for p, q in zip(one, want[k]))
+
+
+def test_two_graphs_of_one_pool(dev):
+    """Two captured steps that share a memory pool, replayed in turn, several times, with eager work between."""
+    g = torch.Generator(device=dev).manual_seed(6)
+    rand = lambda *s: torch.randn(*s, generator=g, device=dev).half()  # noqa: E731
+    x, base, a, b = rand(300, 256), rand(300, 512), rand(9, 16, 256), rand(9, 512, 16)
+    ids = torch.randint(-1, 9, (300,), generator=g, device=dev, dtype=torch.int32)
+    few = torch.randint(-1, 9, (40,), generator=g, device=dev, dtype=torch.int32)
+    side, pool = torch.cuda.Stream(dev), torch.cuda.graph_pool_handle()
+    side.wait_stream(torch.cuda.current_stream(dev))
+    calls = [lambda: lora_ops.lora_add(x, base, a, b, ids), lambda: lora_ops.lora_add(x[:40], base[:40], a, b, few)]
+    with torch.cuda.stream(side):
+        for call in calls:
+            call()
+    side.synchronize()
+    graphs, outs = [], []
+    for call in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool, stream=side):
+            outs.append(call())
+        graphs.append(graph)
+    for i in range(4):
+        x.copy_(rand(300, 256))
+        want = [call() for call in calls]
+        torch.cuda.synchronize()
+        for graph, out, w in zip(graphs, outs, want):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, w), i
