@@ -283,7 +283,8 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(const int32_t* __restr
 // t = A x: a workgroup of 8 waves has a group, or half of one, and a slice of
 // K; its waves take turns of 32 values of K and are summed through LDS.  The
 // product is A (ranks down) times x (rows across): a lane ends with 4 ranks of
-// a row.
+// a row.  The order in which a row's values are added depends neither on its
+// place nor on the number of rows beside it.
 // ---------------------------------------------------------------------------
 
 constexpr int kShrinkWaves = 8;
@@ -292,7 +293,6 @@ constexpr int kShrinkWaves = 8;
 template <typename T, int RT, int MT, Len LEN, typename Put>
 __device__ __forceinline__ void shrink_rows(const T* x, int64_t x_stride, const T* ai, int64_t K, int R, int64_t k0,
                                             int64_t k1, int rowlist, f32x4 (&part)[kShrinkWaves][RT][64], Put put) {
-  constexpr int UN = LEN == kFew || RT * MT > 8 ? 1 : RT * MT > 2 ? 2 : 4;  // turns whose loads are in flight together
   constexpr bool AHEAD = LEN != kFew && RT * MT <= 16;  // (more would not fit the registers)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, grp = lane >> 4;
@@ -309,39 +309,34 @@ __device__ __forceinline__ void shrink_rows(const T* x, int64_t x_stride, const 
   for (int q = 0; q < RT; ++q)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[q][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  struct Turns {
-    typename Frag<T>::v8 x[UN][MT], a[UN][RT];
+  struct Turn {
+    typename Frag<T>::v8 x[MT], a[RT];
   };
   auto load = [&](int64_t kb) {
-    Turns f;
+    Turn f;
+    const int64_t k = kb + 8 * grp;
 #pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const int64_t k = kb + 32 * u + 8 * grp;
+    for (int i = 0; i < MT; ++i) f.x[i] = load_frag<T, LEN>(xr[i], k, k1);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) f.x[u][i] = load_frag<T, LEN>(xr[i], k, k1);
-#pragma unroll
-      for (int q = 0; q < RT; ++q) {
-        const int r = 16 * q + col;
-        f.a[u][q] = load_frag<T, LEN>(ai + (int64_t)(r < R ? r : 0) * K, k, k1, r < R);
-      }
+    for (int q = 0; q < RT; ++q) {
+      const int r = 16 * q + col;
+      f.a[q] = load_frag<T, LEN>(ai + (int64_t)(r < R ? r : 0) * K, k, k1, r < R);
     }
     return f;
   };
-  auto multiply = [&](const Turns& f) {
+  auto multiply = [&](const Turn& f) {
 #pragma unroll
-    for (int u = 0; u < UN; ++u)
+    for (int q = 0; q < RT; ++q)
 #pragma unroll
-      for (int q = 0; q < RT; ++q)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[q][i] = Frag<T>::mfma(f.a[u][q], f.x[u][i], acc[q][i]);
+      for (int i = 0; i < MT; ++i) acc[q][i] = Frag<T>::mfma(f.a[q], f.x[i], acc[q][i]);
   };
-  constexpr int64_t step = 32 * kShrinkWaves * UN;
-  int64_t kb = k0 + 32 * UN * wave;
+  constexpr int64_t step = 32 * kShrinkWaves;
+  int64_t kb = k0 + 32 * wave;
   if constexpr (AHEAD) {  // the next turn is on its way while one is multiplied
     if (kb < k1) {
-      Turns cur = load(kb);
+      Turn cur = load(kb);
       for (kb += step; kb < k1; kb += step) {
-        const Turns next = load(kb);
+        const Turn next = load(kb);
         multiply(cur);
         cur = next;
       }

@@ -241,3 +241,16 @@ def test_many_rows(dev, M, N, R):
     some = torch.cat([some, torch.tensor([0, 1, M - 2, M - 1], device=dev)])
     check_lora(got[some], *(t.cpu() for t in (x[some], base[some], a, b, ids[some])), None)
     assert torch.equal(got[ids < 0], base[ids < 0])
+
+
+@pytest.mark.parametrize("M,K,R,adapters", [(20, 2048, 16, 2), (64, 1500, 40, 3), (200, 2048, 16, 4), (333, 2048, 16, 5),
+                                            (1500, 1024, 64, 7), (3000, 4096, 8, 40), (700, 515, 128, 3)])
+def test_results_do_not_depend_on_places(dev, M, K, R, adapters):
+    """The same call again, and its rows in another order, bit by bit: groups of every number of rows."""
+    x, base, a, b, ids = on(dev, *lora_case(M + R, M, 96, K, R, adapters, torch.bfloat16)[:5])
+    base = base.zero_()  # (what a row adds is not rounded away)
+    want = lo.lora_add(x, base, a, b, ids)
+    for k in range(6):
+        assert torch.equal(lo.lora_add(x, base, a, b, ids), want)
+        p = torch.randperm(M, generator=torch.Generator().manual_seed(k)).to(dev)
+        assert torch.equal(lo.lora_add(x[p], base, a, b, ids[p]), want[p])
