@@ -108,12 +108,18 @@ def _rows(t, width):
 
 
 def _apart(a, b):
-    """Whether the memory that two tensors span does not overlap."""
+    """Whether two tensors (of one dtype) share no memory: their spans do not overlap, or they are different columns."""
     def span(t):
         n = sum((s - 1) * k for s, k in zip(t.shape, t.stride()))
         return t.data_ptr(), t.data_ptr() + (n + 1) * t.element_size()
     (a0, a1), (b0, b1) = span(a), span(b)
-    return a1 <= b0 or b1 <= a0
+    if a1 <= b0 or b1 <= a0:
+        return True
+    if a.ndim != 2 or b.ndim != 2 or a.stride() != b.stride() or a.stride(1) != 1:
+        return False
+    # columns of the same rows
+    row, off = a.stride(0) * a.element_size(), b0 - a0
+    return off % row >= a.shape[1] * a.element_size() and off % row + b.shape[1] * b.element_size() <= row
 
 
 def lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None, out=None, backend: str = "auto"):

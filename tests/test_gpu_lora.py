@@ -254,3 +254,27 @@ def test_results_do_not_depend_on_places(dev, M, K, R, adapters):
         assert torch.equal(lo.lora_add(x, base, a, b, ids), want)
         p = torch.randperm(M, generator=torch.Generator().manual_seed(k)).to(dev)
         assert torch.equal(lo.lora_add(x[p], base, a, b, ids[p]), want[p])
+
+
+def test_far_adapters_and_rows(dev):
+    """Adapters and rows past 2^31 values of their arrays."""
+    N, R, K, M, NA = 8192, 128, 256, 66000, 2100
+    g = torch.Generator().manual_seed(1)
+    a, b = torch.zeros(NA, R, K, dtype=torch.float16, device=dev), torch.zeros(NA, N, R, dtype=torch.float16, device=dev)
+    a[-1], b[-1] = torch.randn(R, K, generator=g).half().to(dev), torch.randn(N, R, generator=g).half().to(dev)
+    wide = torch.zeros(M, 33000, dtype=torch.float16, device=dev)
+    x, base = wide[:, :K], wide[:, 1024:1024 + N]
+    rows = torch.tensor([0, 1, M - 2, M - 1], device=dev)
+    x[rows] = torch.randn(4, K, generator=g).half().to(dev)
+    base[rows] = torch.randn(4, N, generator=g).half().to(dev)
+    ids = torch.full((M,), -1, dtype=torch.int32, device=dev)
+    ids[rows] = NA - 1
+    own = [x[rows].cpu(), base[rows].cpu(), a[-1:].cpu(), b[-1:].cpu(), torch.zeros(4, dtype=torch.int32), None]
+    for take in (slice(None), slice(M - 2, M)):  # listed groups; two rows
+        got = lo.lora_add(x[take], base[take], a, b, ids[take])
+        which = rows if take == slice(None) else torch.tensor([0, 1], device=dev)
+        want = own if take == slice(None) else [own[0][2:], own[1][2:], *own[2:4], own[4][2:], None]
+        check_lora(got[which], *want)
+    assert lo.lora_add(x, base, a, b, ids, out=base) is base
+    check_lora(base[rows], *own)
+    assert not base[2:M - 2].any()

@@ -334,3 +334,29 @@ def test_two_graphs_of_one_pool(dev):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, w), i
+
+
+def test_far_pages(dev):
+    """Pages past 2^31 values of an array: written, copied, forked and compacted."""
+    NP, P, Hkv, D = 140000, 16, 8, 128
+    K, V = (torch.zeros(NP, P, Hkv, D, dtype=torch.float16, device=dev) for _ in range(2))
+    cos, sin = build_scaled_rope_tables(64, D, device=dev)
+    table = torch.tensor([[NP - 1, NP - 2]], dtype=torch.int32, device=dev)
+    qkv = torch.randn(1, 32 * D, device=dev).half()
+    kw = dict(num_attention_heads=16, num_key_value_heads=Hkv, head_dim=D)
+    gqa_ops.paged_qk_norm_rope_update(qkv, K, V, table, cos, sin, torch.tensor([5], device=dev), **kw)
+    small = [torch.zeros(2, P, Hkv, D, dtype=torch.float16, device=dev) for _ in range(2)]
+    gqa_ops.paged_qk_norm_rope_update(qkv, *small, torch.tensor([[0, 1]], dtype=torch.int32, device=dev), cos, sin,
+                                      torch.tensor([5], device=dev), **kw)
+    assert torch.equal(K[NP - 1], small[0][0]) and torch.equal(V[NP - 1], small[1][0]) and V[NP - 1, 5].any()
+    kv_page_ops.copy_kv_pages([K, V], [NP - 1, NP - 1], [3, NP - 5])
+    assert torch.equal(K[3], small[0][0]) and torch.equal(V[NP - 5], small[1][0])
+    refs = torch.ones(NP, dtype=torch.int32, device=dev)
+    refs[NP - 7] = 0
+    new, _, refs, ready = kv_page_ops.fork_kv_sequences([K, V], table, [6], refs, [0, 0])
+    assert new[:, 0].tolist() == [NP - 1, NP - 7] and all(ready.tolist()) and torch.equal(K[NP - 7], small[0][0])
+    refs.zero_()
+    refs[new[:, 0].long()] = 1
+    new, refs, _, live = kv_page_ops.compact_kv_pages([K, V], new, refs)
+    assert new[:, 0].tolist() == [1, 0] and int(live) == 2 and int(refs.sum()) == 2
+    assert all(torch.equal(t[i], s[0]) for t, s in ((K, small[0]), (V, small[1])) for i in range(2))

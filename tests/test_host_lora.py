@@ -109,3 +109,16 @@ def test_limits():
     for M, N in ((lo.MAX_ROWS + 1, 1), (1, lo.MAX_OUTPUTS + 1)):
         with pytest.raises(ValueError, match="at most"):
             lo.lora_add(z(M, 1), z(M, N), z(1, 1, 1), z(1, N, 1), torch.zeros(M, dtype=torch.int32))
+
+
+def test_apart():
+    wide = torch.zeros(6, 20)
+    part = lambda r0, r1, c0, c1: wide[r0:r1, c0:c1]  # noqa: E731
+    apart = [(part(0, 6, 0, 5), part(0, 6, 5, 20)), (part(0, 6, 10, 20), part(0, 6, 0, 10)),
+             (part(0, 2, 0, 20), part(2, 6, 0, 20)), (part(1, 6, 3, 6), part(0, 5, 7, 19)),
+             (part(0, 6, 0, 5), torch.zeros(6, 20))]
+    over = [(part(0, 6, 0, 6), part(0, 6, 5, 20)), (part(0, 6, 10, 20), part(1, 5, 8, 11)), (wide, wide),
+            (part(0, 6, 0, 20), part(0, 6, 3, 4)), (wide.view(3, 40)[:, :5], part(0, 6, 7, 9)),
+            (wide.view(-1)[18:].as_strided((5, 4), (20, 1)), part(0, 6, 0, 3))]
+    assert all(lo._apart(a, b) and lo._apart(b, a) for a, b in apart)
+    assert not any(lo._apart(a, b) or lo._apart(b, a) for a, b in over)
