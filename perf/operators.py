@@ -394,7 +394,7 @@ def _plain_fork(s, c):
     pages = refs.shape[0]
     ids = torch.zeros(pages + 1, dtype=torch.int64, device=DEV)
     ids = ids.scatter(0, torch.where(free, rank - 1, pages), torch.arange(pages, device=DEV))
-    ready = ~live | (fits & ((need == 0) | (off + need <= rank[-1])))
+    ready = ~live | (fits & (off + need <= rank[-1]))
     k = j - nb[:, None] + copy[:, None].long()
     take = (k >= 0) & (k < need[:, None]) & ready[:, None]
     got = ids[(off[:, None] + k).clamp(0, pages)]
