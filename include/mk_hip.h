@@ -352,7 +352,8 @@ int mk_copy_kv_pages(void* const* tensors, const int64_t* page_bytes, int64_t nu
  * suffice or the table has no room: such a row gets none of them, shares its
  * last page and must not be appended to.  Pages that only dropped rows held
  * are free, and may be given away by the same call.  n <= 4096 rows; workspace
- * int32, at least 2 n + 1 + min(num_pages, n (1 + ceil(reserve / page_size))). */
+ * int32, at least 2 n + 1 + min(num_pages, n (1 + ceil(reserve / page_size))),
+ * and NULL where n or reserve is 0. */
 int mk_fork_kv_sequences(void* const* tensors, const int64_t* page_bytes, int64_t num_tensors,
                          const int32_t* block_table, const int32_t* lengths, const int32_t* ref_counts,
                          const int32_t* parents, int32_t* new_table, int32_t* new_lengths, int32_t* new_ref_counts,

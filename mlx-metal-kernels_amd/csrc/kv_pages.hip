@@ -597,9 +597,10 @@ int mk_fork_kv_sequences(void* const* tensors, const int64_t* page_bytes, int64_
   MK_REQUIRE(B * max_blocks < (1LL << 40));
   MK_REQUIRE(ref_counts && new_ref_counts && (B == 0 || (block_table && lengths)));
   MK_REQUIRE(n == 0 || (parents && new_table && new_lengths && ready));
+  if (n == 0) reserve = 0;  // no row takes pages: nothing below may touch the workspace, which may be NULL
   const int64_t most = n * (1 + (reserve + page_size - 1) / page_size);  // pages that the rows can need
   const int64_t max_new = reserve == 0 ? 0 : (most < num_pages ? most : num_pages);
-  MK_REQUIRE(reserve == 0 || n == 0 || (workspace && workspace_ints >= 2 * n + 1 + max_new));
+  MK_REQUIRE(reserve == 0 || (workspace && workspace_ints >= 2 * n + 1 + max_new));
   MK_REQUIRE(num_tensors >= 0 && (num_tensors == 0 || (tensors && page_bytes)));
   for (int64_t i = 0; i < num_tensors; ++i) MK_REQUIRE(tensors[i] && page_bytes[i] >= 0);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -613,13 +614,13 @@ int mk_fork_kv_sequences(void* const* tensors, const int64_t* page_bytes, int64_
     fork_init_kernel<<<(unsigned)(init < 1024 ? init : 1024), 256, 0, st>>>(a);
     const int64_t drop = (B * max_blocks + 255) / 256;
     if (n + drop > 0) fork_rows_kernel<<<(unsigned)(n + (drop < 1024 ? drop : 1024)), 256, 0, st>>>(a);
-    if (reserve > 0 && n > 0) {
+    if (reserve > 0) {
       if (n > kPairRows) fork_pairs_kernel<<<(unsigned)n, 256, 0, st>>>(a);
       fork_allot_kernel<<<1, 1024, 0, st>>>(a, n > kPairRows);
     }
   }
   MK_CHECK_LAUNCH();
-  if (reserve == 0 || n == 0) return MK_OK;
+  if (reserve == 0) return MK_OK;
   return copy_pages(tensors, page_bytes, num_tensors, workspace, workspace + n, workspace + 2 * n, n, num_pages, st);
 }
 

@@ -194,3 +194,26 @@ def test_stream_and_graph(dev):
         assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip(new[:3], want[:3]))
         after = moved(moved(before, moves), want[4])
         assert all(torch.equal(bits(a), bits(b)) for a, b in zip(pages, after))
+
+
+@pytest.mark.parametrize("NP", [40, 9000])
+def test_all_rows_end_without_a_workspace(dev, NP):
+    """The C entry point with no new rows: the old rows' pages are freed, and no workspace is needed or touched."""
+    from mk import _lib
+
+    table = torch.tensor([[3, 7, -1], [3, 9, 2]], dtype=torch.int32, device=dev)
+    lengths = torch.tensor([6, 11], dtype=torch.int32, device=dev)
+    refs = kp.count_page_refs(table, NP)
+    refs[5] = 2
+    page = torch.arange(NP * 4, device=dev).half().reshape(NP, 4)
+    before = page.clone()
+    for ints in (0, 3):  # none; one that is left alone
+        new_refs, guard = torch.full_like(refs, -7), torch.full((3,), -7, dtype=torch.int32, device=dev)
+        at, size = kp._addresses([page], NP)
+        _lib.launch("mk_fork_kv_sequences", dev, at.buffer_info()[0], size.buffer_info()[0], 1, table.data_ptr(),
+                    lengths.data_ptr(), refs.data_ptr(), None, None, None, new_refs.data_ptr(), None,
+                    guard.data_ptr() if ints else None, ints, 2, 0, 3, 4, NP, 5)
+        torch.cuda.synchronize()
+        want = torch.zeros_like(refs)
+        want[5] = 2
+        assert torch.equal(new_refs, want) and (guard == -7).all() and torch.equal(page, before)
