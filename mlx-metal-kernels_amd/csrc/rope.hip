@@ -225,12 +225,13 @@ __device__ __forceinline__ void norm_weights16(const void* w, int wdt, const Pie
   else unpack16<bf16>(a, b, v);
 }
 
-// cache row (page * page_size + offset) of token t, -1 where it has none
+// cache row (page * page_size + offset) of token t, -1 where it has none: an
+// empty row (no position in the tables, no sequence) has none either
 __device__ __forceinline__ int64_t token_slot(const int32_t* pos, const int32_t* seq, const int32_t* bt,
                                               const QkDims& d, int t) {
   const int64_t p = pos[t];
   const int64_t b = seq ? seq[t] : t;
-  if (p < 0 || b < 0 || b >= d.B) return -1;
+  if (p < 0 || p >= d.rows || b < 0 || b >= d.B) return -1;
   const int64_t blk = p / d.page_size;
   if (blk >= d.max_blocks) return -1;
   const int64_t page = bt[b * d.max_blocks + blk];

@@ -255,3 +255,30 @@ def test_rope_long(dev, B, S, H):
         live = sum(int((row != 0).any(-1).any(-1).sum()) for part in got.split(2 ** 26, 1) for row in part)
         assert live == 10 * B
         del got, pos
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_qk_rows_past_the_tables(dev, layout, monkeypatch):
+    """Tables shorter than the block table's reach: a row past them is empty, and keeps no earlier row of the slot that it
+    would have had from writing; among the live rows of a slot the later one still wins."""
+    monkeypatch.setenv("MK_SKIP_DEVICE_RANGE_CHECKS", "1")
+    T, P = 300, 4
+    qkv, K, V, bt, cos, sin, pos, c = qk_case(31, T, T, 2, 1, 32, 32, P, 3, torch.float16)
+    cos, sin = cos[:9], sin[:9]  # positions 9, 10 and 11 of the table's twelve are past them
+    pos[2::3] = 8 + pos[2::3] % 4
+    bt[7, 2] = bt[100, 2] = bt[7, 1]  # page of positions 4 .. 7 and 8 .. 11 of row 7, and of row 100
+    bt[299, 1] = bt[40, 0]
+    pos[7], pos[100] = 5, 9  # row 100 would write slot 1 of the page, row 7 does
+    pos[40], pos[299] = 2, 6  # both live: row 299's
+    bt[200, 2], bt[201, 2], bt[202, 0] = bt[199, 0], bt[199, 0], bt[199, 0]
+    pos[199], pos[200], pos[201], pos[202] = 1, 9, 9, -1  # empty rows of two kinds behind a live one
+    case = qkv, K, V, bt, cos, sin, pos, c
+    d = lambda t: t.to(dev) if isinstance(t, torch.Tensor) else t  # noqa: E731
+    got = gqa.paged_qk_norm_rope_update(d(qkv), d(K), d(V), d(bt), d(cos), d(sin), d(pos), layout=layout,
+                                        **{k: d(v) for k, v in c.items()})
+    check_qk(got, case, torch.float16, layout)
+    want = gqa.reference_paged_qk_norm_rope_update(d(qkv), d(K), d(V), d(bt), d(cos), d(sin), d(pos), layout=layout,
+                                                   **{k: d(v) for k, v in c.items()})
+    assert torch.equal(got[2], want[2])  # v is copied
+    for t in (7, 199):
+        assert torch.equal(got[2][bt[t, pos[t] // P].long(), pos[t] % P].cpu(), qkv[t].reshape(-1, 32)[3:])
