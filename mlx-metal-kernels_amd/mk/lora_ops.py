@@ -19,6 +19,7 @@ from . import _lib
 from ._common import ACT_DTYPES, as_dense, ci_safe_mode_enabled, narrow_i32, values_only
 from .kv_cache_ops import host_checks_enabled
 from .mlp_block_ops import quantized_linear
+from .quant_ops import _MATVEC_BACKENDS_MSG
 
 MAX_RANK, MAX_ADAPTERS = 128, 4096
 MAX_ROWS, MAX_OUTPUTS = 2 ** 20 - 1, 2 ** 24 - 1
@@ -182,8 +183,17 @@ def lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None, out=None, bac
 def quantized_lora_linear(x, w, scales, zeros, lora_a, lora_b, adapter_ids, *, lora_scales=None, bits=4, group_size=32,
                           backend: str = "auto"):
     """``quantized_linear`` with every row's adapter added to its result, in place:
-    the shared product in the activation dtype, then ``lora_add``."""
+    the shared product in the activation dtype, then ``lora_add``.  Where x, scales
+    or zeros need more than their values (a gradient, a function transform,
+    tracing) the shared product takes the tensor ops too, so that a gradient has
+    both parts; where only the adapters do, it stays on its kernel."""
+    if backend.lower() not in ("reference", "metal", "metal_parallel", "metal_tiled", "auto"):
+        raise ValueError(_MATVEC_BACKENDS_MSG)
+    if not values_only(*(t for t in (x, scales, zeros) if t is not None)):
+        backend = "reference"
     y = quantized_linear(x, w, scales, zeros, bits=bits, group_size=group_size, backend=backend)
     reference = backend.lower() == "reference"
-    return lora_add(x, y, lora_a, lora_b, adapter_ids, scales=lora_scales, out=None if reference else y,
+    adapters = (lora_a, lora_b) if lora_scales is None else (lora_a, lora_b, lora_scales)
+    return lora_add(x, y, lora_a, lora_b, adapter_ids, scales=lora_scales,
+                    out=None if reference or not values_only(*adapters) else y,
                     backend="reference" if reference else "auto")

@@ -7,7 +7,7 @@ import torch
 import mk.lora_ops as lo
 from mk.mlp_block_ops import quantized_linear
 from tests._data import quant_weight, to_dev
-from tests.test_host_lora import check_lora, lora_case
+from tests.test_host_lora import check_linear_gradients, check_lora, lora_case, quantized_case
 
 import numpy as np
 
@@ -278,3 +278,22 @@ def test_far_adapters_and_rows(dev):
     assert lo.lora_add(x, base, a, b, ids, out=base) is base
     check_lora(base[rows], *own)
     assert not base[2:M - 2].any()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_quantized_lora_linear_gradients(dev, bits):
+    """x's gradient has both parts; where only the adapters record one, the shared product stays on its kernel and the
+    adapters' gradients are those of the same formula."""
+    *tensors, W = quantized_case(10 + bits, 40, 64, 128, 8, 3, bits, 32, dev)
+    x, w, sc, z, a, b, ids, s = tensors
+    g = torch.randn(40, 64, generator=torch.Generator().manual_seed(bits)).half().to(dev)
+    kw = dict(lora_scales=s, bits=bits, group_size=32)
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+    lo.quantized_lora_linear(leaves[0], w, sc, z, *leaves[1:], ids, **kw).backward(g)
+    check_linear_gradients([t.grad for t in leaves], x, a, b, ids, s, W, g)
+    own = [t.clone().requires_grad_() for t in (a, b)]
+    y = lo.quantized_lora_linear(x, w, sc, z, *own, ids, **kw)
+    y.backward(g)
+    assert all(torch.equal(p.grad, q.grad) for p, q in zip(own, leaves[1:]))
+    shared = quantized_linear(x, w, sc, z, bits=bits, group_size=32)
+    assert torch.equal(y, lo.lora_add(x, shared, a, b, ids, scales=s, backend="reference"))

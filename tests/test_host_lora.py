@@ -122,3 +122,72 @@ def test_apart():
             (wide.view(-1)[18:].as_strided((5, 4), (20, 1)), part(0, 6, 0, 3))]
     assert all(lo._apart(a, b) and lo._apart(b, a) for a, b in apart)
     assert not any(lo._apart(a, b) or lo._apart(b, a) for a, b in over)
+
+
+def quantized_case(seed, M, N, K, R, NA, bits, group, device="cpu"):
+    """(x, packed w, scales, zeros, adapters, ids, lora scales, W as the product takes it)"""
+    from mk.quant_ops import reference_dequant_q4, reference_dequant_q8
+
+    g = torch.Generator().manual_seed(seed)
+    x, _, a, b, ids, s = lora_case(seed, M, N, K, R, NA, torch.float16)
+    ids[M // 2] = -1
+    w = torch.randint(0, 256, (N, K // 2 if bits == 4 else K), generator=g, dtype=torch.uint8)
+    sc = (0.02 * (0.5 + torch.rand(N, K // group, generator=g))).half()
+    z = torch.randint(3, 12, (N, K // group), generator=g).half()
+    W = (reference_dequant_q4 if bits == 4 else reference_dequant_q8)(w, sc, z, group_size=group, out_dtype=torch.float16)
+    return [t.to(device) for t in (x, w, sc, z, a, b, ids, s, W)]
+
+
+def check_linear_gradients(got, x, a, b, ids, s, W, g):
+    """Gradients (x, a, b) of <g, x W^T + s_i B_i A_i x>: fp32 sums, each part rounded to fp16 on its way into x's."""
+    x, a, b, s, W, g = (t.double().cpu() for t in (x, a, b, s, W, g))
+    dx, size = g @ W, g.abs() @ W.abs()
+    for m, i in enumerate(ids.tolist()):
+        if i < 0:
+            continue
+        dx[m] += s[i] * (g[m] @ b[i]) @ a[i]
+        size[m] += s[i] * (g[m].abs() @ b[i].abs()) @ a[i].abs()
+    assert ((got[0].double().cpu() - dx).abs() <= 4 * 2.0 ** -11 * size).all()
+    assert (got[0][ids < 0] != 0).any()  # a row without an adapter has the shared product's part
+    for i in range(len(a)):
+        rows = (ids == i).cpu()
+        da, db = s[i] * (b[i].t() @ g[rows].t()) @ x[rows], s[i] * g[rows].t() @ (x[rows] @ a[i].t())
+        sa, sb = (s[i] * (b[i].abs().t() @ g[rows].abs().t()) @ x[rows].abs(),
+                  s[i] * g[rows].abs().t() @ (x[rows].abs() @ a[i].abs().t()))
+        for t, want, mag in ((got[1][i], da, sa), (got[2][i], db, sb)):
+            assert ((t.double().cpu() - want).abs() <= 2 * 2.0 ** -11 * mag + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("backend", ["auto", "reference"])
+def test_quantized_lora_linear_gradients(bits, backend):
+    """The gradient of x has the shared product's part as well as the adapters', on every backend."""
+    x, w, sc, z, a, b, ids, s, W = quantized_case(bits, 9, 12, 16, 3, 2, bits, 8)
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+    g = torch.randn(9, 12, generator=torch.Generator().manual_seed(1)).half()
+    kw = dict(lora_scales=s, bits=bits, group_size=8, backend=backend)
+    y = lo.quantized_lora_linear(leaves[0], w, sc, z, *leaves[1:], ids, **kw)
+    y.backward(g)
+    check_linear_gradients([t.grad for t in leaves], x, a, b, ids, s, W, g)
+    with torch.no_grad():
+        assert torch.equal(y, lo.quantized_lora_linear(x, w, sc, z, a, b, ids, **{**kw, "backend": "reference"}))
+    # against differences: linear in x, so exact but for the roundings of both results and of the gradient
+    step = torch.randn(9, 16, generator=torch.Generator().manual_seed(2)).half()
+    y0, y1 = (lo.quantized_lora_linear(t, w, sc, z, a, b, ids, **{**kw, "backend": "reference"}).double()
+              for t in (x, x + step))
+    moved = (x + step).double() - x.double()
+    slope = (leaves[0].grad.double() * moved).sum()
+    size = (leaves[0].grad.double().abs() * moved.abs()).sum() + (g.double().abs() * (y0.abs() + y1.abs())).sum()
+    assert abs(((y1 - y0) * g.double()).sum() - slope) <= 4 * 2.0 ** -11 * size
+    # a gradient of the quantization's scales, and a forward-mode tangent
+    sc_leaf = sc.clone().requires_grad_()
+    lo.quantized_lora_linear(x, w, sc_leaf, z, a, b, ids, **kw).sum().backward()
+    assert sc_leaf.grad.abs().sum() > 0
+    _, tangent = torch.func.jvp(lambda t: lo.quantized_lora_linear(t, w, sc, z, a, b, ids, **kw).float(), (x,), (step,))
+    want = step.double() @ W.double().t()
+    for m, i in enumerate(ids.tolist()):
+        if i >= 0:
+            want[m] += s[i].double() * (step[m].double() @ a[i].double().t()) @ b[i].double().t()
+    assert (tangent.double() - want).abs().max() <= 8 * 2.0 ** -11 * want.abs().max()
+    with pytest.raises(ValueError, match="backend must be one of"):
+        lo.quantized_lora_linear(leaves[0], w, sc, z, a, b, ids, **{**kw, "backend": "x"})
