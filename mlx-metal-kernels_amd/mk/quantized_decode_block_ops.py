@@ -242,6 +242,17 @@ def _verify_rows(q, K_pages, V_pages, block_table, lengths, scale, W):
                                  scale).reshape(rows, 1, H, D)
 
 
+def _tensors_of(lora):
+    return () if lora is None else (lora.a, lora.b, lora.scales)
+
+
+def _refuse_gradient(*tensors):
+    """Beside launches that leave no graph ``lora_add`` would give a result whose gradient is the adapters' part alone."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the decode block's kernels record no gradient; with adapters, call it under torch.no_grad() "
+                           "or with both backends 'reference'")
+
+
 def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_pages, V_pages, block_table, cos, sin,
                                  position, *, qkv_zeros=None, out_zeros=None, bits=4, group_size=32, H=None,
                                  num_key_value_heads=None, head_dim=None, D=None, scale=None,
@@ -270,7 +281,9 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
     each head (``rope_layout``, ``rotary_dim``) take ``paged_qk_norm_rope_update``
     between the projection and the attention.  ``qkv_lora``, ``out_lora``
     (``LoraAdapters``) with ``adapter_ids`` [rows] add every row's adapter to
-    the two projections (``lora_add``; to the output one behind the residual)."""
+    the two projections (``lora_add``; to the output one behind the residual).
+    With adapters an input that records a gradient is refused, but on the
+    reference backends, which are tensor ops throughout."""
     x2d, _, _ = normalize_hidden_input(x)
     H, kv_heads, D = _block_dims(qkv_w, H, num_key_value_heads, head_dim, D, bits)
     validate_quantized_weight_shapes(x2d, qkv_w, qkv_scales, qkv_zeros, bits=bits, group_size=group_size,
@@ -279,8 +292,11 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
     validate_quantized_weight_shapes(x2d.new_empty((x2d.shape[0], H * D)), out_w, out_scales, out_zeros, bits=bits,
                                      group_size=group_size, expected_in_dim=H * D, name="output_projection")
     reference = matvec_backend.lower() == "reference"
-    if (qkv_lora is not None or out_lora is not None) and adapter_ids is None:
-        raise ValueError("qkv_lora and out_lora need adapter_ids")
+    if qkv_lora is not None or out_lora is not None:
+        if adapter_ids is None:
+            raise ValueError("qkv_lora and out_lora need adapter_ids")
+        if not (reference and block_backend.lower() == "reference"):
+            _refuse_gradient(x, residual, norm_weight, *_tensors_of(qkv_lora), *_tensors_of(out_lora))
     other_rope = (q_norm_weight is not None or k_norm_weight is not None or rope_layout != "interleaved"
                   or rotary_dim not in (None, D))
     fuse_front = (norm_weight is not None and not other_rope and qkv_lora is None and not reference and

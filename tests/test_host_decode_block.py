@@ -129,3 +129,39 @@ def test_contiguous_gqa_block_validation_messages():
         gqa.gqa_decode_block_from_qkv(qkv, K, K[:1], cos, sin, 0, **kw)
     with pytest.raises(ValueError, match="cache batch/head/head_dim"):
         gqa.gqa_decode_block_from_qkv(qkv[:1], K, K, cos, sin, 0, **kw)
+
+
+def test_adapters_refuse_gradients_beside_kernels():
+    """With adapters the kernels' backends take no input that records a gradient: the result would have the adapters'
+    part of it alone.  The reference backends are tensor ops throughout and give all of it."""
+    from mk.lora_ops import LoraAdapters
+    from mk.quantized_decode_block_ops import paged_quantized_decode_block
+
+    g = torch.Generator().manual_seed(3)
+    B, H, Hkv, D, K, P = 2, 2, 1, 16, 32, 4
+    N = (H + 2 * Hkv) * D
+    w = lambda n, k: torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)  # noqa: E731
+    sc = lambda n, k: (0.02 * torch.rand(n, k // 32, generator=g)).half()  # noqa: E731
+    rand = lambda *s: torch.randn(*s, generator=g).half()  # noqa: E731
+    cos, sin = (torch.randn(12, D // 2, generator=g) for _ in range(2))
+    lora = lambda n, k: LoraAdapters(rand(1, 4, k) / 4, rand(1, n, 4) / 4, torch.ones(1))  # noqa: E731
+    x, qkv_lora, out_lora = rand(B, 1, K), lora(N, K), lora(K, H * D)
+    args = (w(N, K), sc(N, K), w(K, H * D), sc(K, H * D), rand(6, P, Hkv, D), rand(6, P, Hkv, D),
+            torch.arange(6, dtype=torch.int32).reshape(2, 3), cos, sin, torch.tensor([5, 2]))
+    kw = dict(H=H, num_key_value_heads=Hkv, head_dim=D, qkv_lora=qkv_lora, out_lora=out_lora,
+              adapter_ids=torch.tensor([0, -1], dtype=torch.int32))
+    leaves = [x, qkv_lora.a, qkv_lora.b, qkv_lora.scales, out_lora.a, out_lora.b, out_lora.scales]
+    for leaf in leaves:
+        leaf.requires_grad_()
+        for backends in ({}, dict(matvec_backend="reference"), dict(block_backend="reference")):
+            with pytest.raises(RuntimeError, match="record no gradient"):
+                paged_quantized_decode_block(x, *args, **kw, **backends)
+        with torch.no_grad(), pytest.raises(ValueError, match="ROCm device"):
+            paged_quantized_decode_block(x, *args, **kw)
+        leaf.requires_grad_(False)
+    for leaf in leaves:
+        leaf.requires_grad_()
+    y, _, _ = paged_quantized_decode_block(x, *args, **kw, matvec_backend="reference", block_backend="reference")
+    y.float().sum().backward()
+    assert all(leaf.grad.abs().sum() > 0 for leaf in leaves)
+    assert (x.grad[1] != 0).any()  # the row without an adapter: through the projections and the attention
