@@ -227,3 +227,15 @@ def test_qk_row_limits(T, ragged):
                                       one.expand(1 if ragged else T, 1), torch.ones(1, 1), torch.ones(1, 1),
                                       one.expand(T), sequences=one.expand(T) if ragged else None,
                                       num_attention_heads=1, num_key_value_heads=1, head_dim=2)
+
+
+@pytest.mark.parametrize("name", ["qkv", "K_pages", "V_pages", "cos", "sin", "q_weight", "k_weight"])
+def test_qk_records_no_gradient_of_any_input(name):
+    """Every floating input that records a gradient is refused, not only the rows and the norm weights."""
+    qkv, K, V, bt, cos, sin, pos, c = qk_case(7, 3, 3, 4, 2, 16, 8, 4, 3, torch.float16)
+    ok = dict(qkv=qkv, K_pages=K, V_pages=V, block_table=bt, cos=cos, sin=sin, position=pos, **c)
+    ok[name] = ok[name].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="records no gradient"):
+        gqa.paged_qk_norm_rope_update(**ok)
+    with torch.no_grad(), pytest.raises(ValueError, match="ROCm device"):
+        gqa.paged_qk_norm_rope_update(**ok)
