@@ -47,7 +47,7 @@ def normalize_positions(positions, B: int, MAX_S: int, *, device=None) -> torch.
         if positions.ndim == 0:
             pos = positions.to(device=dev, dtype=torch.int32).reshape(1).expand(B).contiguous()
         elif positions.ndim == 1 and positions.shape[0] == B:
-            pos = positions.to(device=dev, dtype=torch.int32)
+            pos = positions.to(device=dev, dtype=torch.int32).contiguous()  # (the kernels read it as an array)
         else:
             raise ValueError(f"positions must be scalar or shape [B], got {tuple(positions.shape)}")
     else:

@@ -558,3 +558,19 @@ def test_quantized_fused_update_bit_exact(dev, bits, B, Hq, Hkv, D, P, mb, g):
     got = pq.paged_quantized_kv_gqa_decode_attention(q_out, cache, backend=f"metal_q{bits}")
     ref = op.quantized_paged_attention(rq.astype(np.float32), rkq, rvq, rks, rvs, bt, pos + 1, g, bits)
     assert_close(got[:, 0], ref, what="attention after fused write")
+
+
+def test_positions_of_a_wider_table(dev):
+    """Positions that are a column of another tensor, which the kernels read as an array."""
+    B, Hq, Hkv, D, P, mb = 5, 4, 2, 64, 8, 4
+    g = torch.Generator().manual_seed(6)
+    K, V = (torch.randn(B * mb, P, Hkv, D, generator=g).half().to(dev) for _ in range(2))
+    bt = torch.randperm(B * mb, generator=g).reshape(B, mb).to(torch.int32).to(dev)
+    qkv = torch.randn(B, 1, (Hq + 2 * Hkv) * D, generator=g).half().to(dev)
+    cos, sin = (torch.randn(P * mb, D // 2, generator=g).to(dev) for _ in range(2))
+    wide = torch.randint(0, P * mb, (B, 3), generator=g, dtype=torch.int32).to(dev)
+    kw = dict(num_attention_heads=Hq, num_key_value_heads=Hkv, head_dim=D)
+    for pos in (wide[:, 1], wide[2, 2].expand(B)):
+        want = gqa.paged_gqa_decode_block_from_qkv(qkv, K.clone(), V.clone(), bt, cos, sin, pos.contiguous(), **kw)
+        got = gqa.paged_gqa_decode_block_from_qkv(qkv, K.clone(), V.clone(), bt, cos, sin, pos, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

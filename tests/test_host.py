@@ -337,3 +337,14 @@ def test_loader_rejects_another_abi_version(monkeypatch):
     monkeypatch.setattr(_lib, "ABI_VERSION", _lib.ABI_VERSION + 1)
     with pytest.raises(_lib.NativeLibraryError, match="ABI version"):
         _lib.load()
+
+
+def test_positions_are_an_array_for_the_kernels():
+    """Positions that are a column or an expanded value of another tensor: the kernels read them one after another."""
+    from mk.kv_cache_ops import normalize_positions
+
+    both = torch.tensor([[3, 90], [5, 91], [4, 92]], dtype=torch.int32)
+    for pos, want in ((both[:, 0], [3, 5, 4]), (both[1, :1].expand(3), [5, 5, 5]), (both.long()[:, 0], [3, 5, 4]),
+                      (torch.tensor(4), [4, 4, 4]), (both[:, 0].contiguous(), [3, 5, 4])):
+        got = normalize_positions(pos, 3, 10)
+        assert got.tolist() == want and got.is_contiguous() and got.dtype == torch.int32
