@@ -261,6 +261,8 @@ def paged_gqa_decode_block_from_qkv(qkv, K_pages, V_pages, block_table, cos, sin
     MAX_BLOCKS = block_table.shape[1]
     x, c, s, pos, q_out, B = _qkv_rope_update_prep(qkv, block_table, cos, sin, position, Hq, Hkv, D, P,
                                                    K_pages.dtype, dev)
+    if lengths is not None and tuple(lengths.shape) != (B,):
+        raise ValueError(f"lengths must have shape {(B,)}, got {tuple(lengths.shape)}")
     bt = _i32(block_table, dev)
     _lib.launch("mk_qkv_rope_paged_update", dev, _lib.ptr(x), _lib.ptr(c), _lib.ptr(s), _lib.ptr(pos), _lib.ptr(bt),
                 _lib.ptr(K_pages), _lib.ptr(V_pages), _lib.ptr(q_out), B, Hq, Hkv, D, P, MAX_BLOCKS, NUM_PAGES,

@@ -173,7 +173,9 @@ def llama_stack_decode_step(x, stack_weights: LlamaStackWeights, stack_cache: Ll
     hidden = x
     layers_out = []
     new_caches = []
-    # every layer attends over positions 0..position: the lengths are shared
+    if isinstance(position, torch.Tensor) and position.ndim == 0:  # one position for all rows
+        position = position.reshape(1).expand(x.shape[0])
+    # every layer attends over positions 0..position: the lengths are shared, one a row for the attention to read
     lengths = position.to(torch.int32) + 1 if isinstance(position, torch.Tensor) and position.is_cuda else None
     if verify_width > 1:
         if lengths is None:

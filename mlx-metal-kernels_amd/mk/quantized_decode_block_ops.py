@@ -291,6 +291,8 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
                                      name="qkv_projection")
     validate_quantized_weight_shapes(x2d.new_empty((x2d.shape[0], H * D)), out_w, out_scales, out_zeros, bits=bits,
                                      group_size=group_size, expected_in_dim=H * D, name="output_projection")
+    if lengths is not None and tuple(lengths.shape) != (x2d.shape[0] // verify_width,):
+        raise ValueError(f"lengths must have shape {(x2d.shape[0] // verify_width,)}, got {tuple(lengths.shape)}")
     reference = matvec_backend.lower() == "reference"
     if qkv_lora is not None or out_lora is not None:
         if adapter_ids is None:

@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+from mk import gqa_ops
 from mk import llama_layer_ops as ll
 from mk import llama_stack_ops as ls
 from oracle import llama as ol
@@ -224,3 +225,33 @@ def fused_vs_two_step(dev, rng, cfg, w, bits, B, g, P, mb):
     expect = np.zeros_like(changed)
     expect[page, off] = True
     assert np.array_equal(changed, expect)
+
+
+def test_positions_of_every_form(dev):
+    """One position for all rows -- an int, a host or device tensor without dimensions -- and one a row, as a list or a
+    tensor: the same step.  The attention reads a length of every row, so a single one is spread over them."""
+    cfg = _cfg()
+    w = ls.create_random_quantized_llama_stack_weights(cfg, bits=4, seed=3, device=dev)
+    cos, sin = ll.build_rope_tables(cfg, device=dev)
+    B, S, p = 5, 64, 37
+    torch.manual_seed(2)
+    x = torch.randn(B, 1, cfg.hidden_size, device=dev).half()
+    first = [tuple(torch.randn_like(t) if t.is_floating_point() else t
+                   for t in ll.init_llama_layer_cache(cfg, B, S, cache_layout="paged", device=dev))
+             for _ in range(cfg.num_hidden_layers)]
+    outs = []
+    for position in (p, torch.tensor([p] * B, dtype=torch.int32, device=dev), torch.tensor(p, device=dev),
+                     torch.tensor(p, dtype=torch.int32, device=dev), torch.tensor(p), [p] * B, torch.tensor([p] * B)):
+        cache = ls.LlamaStackCache([tuple(t.clone() for t in c) for c in first], "paged", S, 16)
+        logits, hidden, cache = ls.llama_stack_decode_step(x, w, cache, cos, sin, position, cfg)
+        outs.append([logits, hidden, *(t for c in cache.layer_caches for t in c)])
+    for out in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out, outs[0]))
+    ln = torch.tensor(p + 1, dtype=torch.int32, device=dev)
+    for bad in (ln, ln.reshape(1), ln.expand(B + 1)):
+        with pytest.raises(ValueError, match="lengths must have shape"):
+            ll.llama_layer_decode_step(x, w.layers[0], first[0], cos, sin, p, cfg, cache_layout="paged", lengths=bad)
+        with pytest.raises(ValueError, match="lengths must have shape"):
+            gqa_ops.paged_gqa_decode_block_from_qkv(
+                torch.zeros(B, 1, cfg.qkv_output_dim(), device=dev).half(), *first[0], cos, sin, p, lengths=bad,
+                num_attention_heads=4, num_key_value_heads=2, head_dim=64)
