@@ -323,8 +323,10 @@ def _qk_norm_rope_prep(qkv, K_pages, V_pages, block_table, cos, sin, position, H
         position = torch.full((T,), position, dtype=torch.int32, device=dev)
     elif not isinstance(position, torch.Tensor):
         position = torch.as_tensor(position, dtype=torch.int32)
+    if position.ndim == 0:  # one for all rows, as normalize_positions takes it
+        position = position.reshape(1).expand(T)
     if position.dtype not in (torch.int32, torch.int64) or position.shape != (T,):
-        raise ValueError(f"position must be an int or int32 [T]={(T,)}, got {position.dtype} {tuple(position.shape)}")
+        raise ValueError(f"position must be a value or int32 [T]={(T,)}, got {position.dtype} {tuple(position.shape)}")
     if sequences is None:
         if T != B:
             raise ValueError(f"qkv has {T} rows and block_table {B}: without sequences they are one to one")
@@ -398,7 +400,7 @@ def paged_qk_norm_rope_update(qkv, K_pages, V_pages, block_table, cos, sin, posi
 
     qkv [T, (Hq+2Hkv)*D] (also [T,1,...] as the decode blocks take it; rows may
     be strided) in the pages' dtype; cos, sin fp32 [rows, rotary_dim/2];
-    position int or int32 [T].  Without ``sequences`` row t is the new token of
+    position int32 [T], or one value for all rows.  Without ``sequences`` row t is the new token of
     block_table's row t, and the later of two rows of one slot wins.  With
     ``sequences`` int32 [T] the rows are the tokens of prompts, in any order:
     row t is of block_table row sequences[t], and no two rows may have the same

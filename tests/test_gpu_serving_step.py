@@ -360,3 +360,25 @@ def test_far_pages(dev):
     new, refs, _, live = kv_page_ops.compact_kv_pages([K, V], new, refs)
     assert new[:, 0].tolist() == [1, 0] and int(live) == 2 and int(refs.sum()) == 2
     assert all(torch.equal(t[i], s[0]) for t, s in ((K, small[0]), (V, small[1])) for i in range(2))
+
+
+def test_positions_of_every_form(dev):
+    """A stack of layers with head norms takes positions in the forms that plain layers take."""
+    w, (cos, sin) = _weights(dev), _tables(dev)
+    B, S, p = 5, 64, 37
+    torch.manual_seed(2)
+    x = torch.randn(B, 1, CFG.hidden_size, device=dev).half()
+    first = [tuple(torch.randn_like(t) if t.is_floating_point() else t
+                   for t in ll.init_llama_layer_cache(CFG, B, S, cache_layout="paged", device=dev))
+             for _ in range(CFG.num_hidden_layers)]
+    outs = []
+    for position in (p, torch.tensor([p] * B, dtype=torch.int32, device=dev), torch.tensor(p, device=dev),
+                     torch.tensor(p, dtype=torch.int32, device=dev), torch.tensor(p), [p] * B, torch.tensor([p] * B),
+                     torch.full((B, 2), p, dtype=torch.int32, device=dev)[:, 1]):
+        cache = ls.LlamaStackCache([tuple(t.clone() for t in c) for c in first], "paged", S, 16)
+        logits, hidden, cache = ls.llama_stack_decode_step(x, w, cache, cos, sin, position, CFG)
+        step, layer_cache = ll.llama_layer_decode_step(x, w.layers[0], tuple(t.clone() for t in first[0]), cos, sin,
+                                                       position, CFG, cache_layout="paged")
+        outs.append([logits, hidden, *(t for c in cache.layer_caches for t in c), step, *layer_cache])
+    for out in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out, outs[0]))

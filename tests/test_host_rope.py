@@ -239,3 +239,15 @@ def test_qk_records_no_gradient_of_any_input(name):
         gqa.paged_qk_norm_rope_update(**ok)
     with torch.no_grad(), pytest.raises(ValueError, match="ROCm device"):
         gqa.paged_qk_norm_rope_update(**ok)
+
+
+def test_qk_one_position_for_all_rows():
+    """An int, a number of numpy's and a tensor without dimensions are one position for every row."""
+    qkv, K, V, bt, cos, sin, _, c = qk_case(8, 3, 3, 4, 2, 16, 8, 4, 3, torch.float16)
+    outs = [gqa.paged_qk_norm_rope_update(qkv, K, V, bt, cos, sin, position, backend="reference", **c)
+            for position in ([5, 5, 5], 5, np.int64(5), torch.tensor(5), torch.tensor(5, dtype=torch.int32))]
+    for out in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out, outs[0]))
+    for bad in (torch.tensor(12), torch.tensor(-2), torch.tensor(1.0), torch.tensor([5]), [5]):
+        with pytest.raises(ValueError, match="position must be"):
+            gqa.paged_qk_norm_rope_update(qkv, K, V, bt, cos, sin, bad, backend="reference", **c)
