@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _lib
-from ._common import as_u8, scales_for_kernel
+from ._common import ACT_DTYPES, as_u8, scales_for_kernel
 from .gqa_ops import (
     paged_gqa_decode_attention,
     paged_gqa_decode_block_from_qkv,
@@ -331,9 +331,12 @@ def paged_quantized_decode_block(x, qkv_w, qkv_scales, out_w, out_scales, K_page
         qkv = lora_add(x2d[:, None], qkv, qkv_lora.a, qkv_lora.b, adapter_ids, scales=qkv_lora.scales,
                        backend="reference" if reference else "auto")
     block_fn = reference_paged_gqa_decode_block_from_qkv if block_backend.lower() == "reference" else None
+    # draft rows whose projection has adapters: the page write alone, then their sequence's pages read once for all of them
+    adapted_drafts = (verify_width > 1 and qkv_lora is not None and block_fn is None and
+                      K_pages.dtype == V_pages.dtype == qkv.dtype and K_pages.dtype in ACT_DTYPES)
     if fuse_front:
         pass
-    elif other_rope:
+    elif other_rope or adapted_drafts:
         plain = "reference" if block_fn is not None else "auto"
         q, K_pages, V_pages = paged_qk_norm_rope_update(
             qkv, K_pages, V_pages, block_table, cos, sin, position, num_attention_heads=H,

@@ -382,3 +382,122 @@ def test_positions_of_every_form(dev):
         outs.append([logits, hidden, *(t for c in cache.layer_caches for t in c), step, *layer_cache])
     for out in outs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(out, outs[0]))
+
+
+def _plain_weights(dev, adapted, bits=4, dtype=torch.float16):
+    """Layers as an ordinary stack has them -- interleaved rotation of whole heads, no head norms -- with adapters beside
+    qkv and o, or one of them; and their tables."""
+    w = _weights(dev, bits, dtype)
+    for layer in w.layers:
+        layer.q_norm_weight = layer.k_norm_weight = None
+        layer.rope_layout = "interleaved"
+        if "qkv" not in adapted:
+            layer.qkv_lora = None
+        if "o" not in adapted:
+            layer.o_lora = None
+    return w, ll.build_rope_tables(CFG, device=dev)
+
+
+ADAPTED = [("qkv", "o"), ("qkv",), ("o",)]
+
+
+def _filled(dev, B, S, layout="paged", dtype=torch.float16):
+    first = [ll.init_llama_layer_cache(CFG, B, S, cache_layout=layout, dtype=dtype, device=dev)
+             for _ in range(CFG.num_hidden_layers)]
+    for c in first:
+        for t in c[:2]:
+            t.copy_(torch.randn(t.shape, device=dev))
+    return first
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("adapted", ADAPTED)
+def test_plain_layer_with_adapters_against_reference_backend(dev, adapted, bits, dtype):
+    torch.manual_seed(bits)
+    w, (cos, sin) = _plain_weights(dev, adapted, bits, dtype)
+    w, (cache, _) = w.layers[0], _filled(dev, 5, 48, dtype=dtype)
+    x = torch.randn(5, 1, CFG.hidden_size, device=dev).to(dtype)
+    pos = torch.tensor([0, 47, 16, 15, 30], dtype=torch.int32, device=dev)
+    ids = torch.tensor([2, -1, 0, 1, 2], dtype=torch.int32, device=dev)
+    kw = dict(cache_layout="paged", adapter_ids=ids)
+    ref, ref_cache = ll.reference_llama_layer_decode_step(x, w, cache, cos, sin, pos, CFG, **kw)
+    got, got_cache = ll.llama_layer_decode_step(x, w, tuple(t.clone() for t in cache), cos, sin, pos, CFG, **kw)
+    # the bound of the layer's other tests against its reference path; bf16 rounds 8 times as coarsely
+    scale = 1 if dtype == torch.float16 else 8
+    assert_close(got, ref.float().cpu().numpy(), what="layer", rtol=1e-2 * scale, atol=1e-3 * scale)
+    for a, b in zip(got_cache[:2], ref_cache[:2]):
+        assert_close(a, b.float().cpu().numpy(), what="cache", rtol=1e-2 * scale, atol=1e-3 * scale)
+    none, _ = ll.llama_layer_decode_step(x, w, tuple(t.clone() for t in cache), cos, sin, pos, CFG, cache_layout="paged",
+                                         adapter_ids=torch.full_like(ids, -1))
+    assert not torch.equal(got[ids >= 0], none[ids >= 0]) and torch.equal(got[1], none[1])
+
+
+@pytest.mark.parametrize("W", [2, 5])
+@pytest.mark.parametrize("layout", ["paged", "contiguous"])
+@pytest.mark.parametrize("adapted", ADAPTED)
+def test_plain_verify_step_with_adapters(dev, adapted, layout, W, monkeypatch):
+    """W draft rows of an ordinary stack with adapters: one read of a sequence's pages a layer, and what W staged steps
+    give (bounds as in test_verify_step_with_adapters, without its norm weights' 1.8)."""
+    from mk import _lib
+    from mk.speculative_verify_ops import llama_stack_verify_step
+
+    torch.manual_seed(W)
+    w, (cos, sin) = _plain_weights(dev, adapted)
+    B, S = 3, 64
+    first = _filled(dev, B, S, layout)
+    caches = [ls.LlamaStackCache([tuple(t.clone() for t in c) for c in first], layout, S, 16) for _ in range(2)]
+    x = torch.randn(B, W, CFG.hidden_size, device=dev).half()
+    pos = torch.tensor([0, 30, S - W], dtype=torch.int32, device=dev)
+    ids = torch.tensor([2, -1, 0], device=dev)
+    names, launch = [], _lib.launch
+    monkeypatch.setattr(_lib, "launch", lambda name, *a: (names.append(name), launch(name, *a))[1])
+    logits, _, caches[0] = llama_stack_verify_step(x, w, caches[0], cos, sin, pos, CFG, adapter_ids=ids)
+    assert names.count("mk_paged_verify_attention") == CFG.num_hidden_layers
+    assert "mk_paged_decode_attention" not in names
+    monkeypatch.undo()
+    staged = []
+    for i in range(W):
+        lg, _, caches[1] = ls.llama_stack_decode_step(x[:, i:i + 1], w, caches[1], cos, sin, pos + i, CFG, adapter_ids=ids)
+        staged.append(lg[:, 0])
+    staged = torch.stack(staged, 1).float()
+    rms = float(staged.square().mean().sqrt())
+    assert_close(logits.float().cpu().numpy() / rms, staged.cpu().numpy() / rms, atol=8 * 2.0 ** -11, what="verify")
+    moves = 2.0 ** -10 * (2 / np.pi) * 16
+    for a, b in zip(caches[0].layer_caches, caches[1].layer_caches):
+        for s, t in zip(a[:2], b[:2]):
+            t = t.float().cpu().numpy()
+            assert_close(s, t, rtol=0, atol=moves * float(np.sqrt((t ** 2).mean())), what="cache")
+
+
+@pytest.mark.parametrize("adapted", ADAPTED)
+def test_plain_loop_and_graph_with_adapters(dev, adapted):
+    """The loop against its steps, and the captured step, adapters changed between replays, against eager steps."""
+    w, (cos, sin) = _plain_weights(dev, adapted)
+    B, S = 4, 64
+    x = torch.randn(B, 3, CFG.hidden_size, device=dev).half()
+    ids = torch.tensor([0, 1, 2, -1], dtype=torch.int32, device=dev)
+    caches = [ls.LlamaStackCache([ll.init_llama_layer_cache(CFG, B, S, cache_layout="paged", device=dev)
+                                  for _ in range(CFG.num_hidden_layers)], "paged", S, 16) for _ in range(4)]
+    got, _ = ls.llama_stack_decode_loop(x, w, caches[0], cos, sin, CFG, cache_layout="paged", adapter_ids=ids)
+    want, run = [], caches[1]
+    for t in range(3):
+        lg, _, run = ls.llama_stack_decode_step(x[:, t:t + 1], w, run, cos, sin, t, CFG, adapter_ids=ids)
+        want.append(lg)
+    assert torch.equal(got, torch.cat(want, 1))
+    tokens, pos = torch.tensor([3, 5, 7, 11], device=dev), torch.zeros(B, dtype=torch.int32, device=dev)
+    graph = ls.DecodeGraph(w, caches[2], cos, sin, CFG, tokens, pos, adapter_ids=ids)
+    got, order = [graph.first_tokens.clone()], [ids.clone()]
+    for _ in range(6):
+        ids.copy_(torch.roll(ids, 1))
+        order.append(ids.clone())
+        got.append(graph.step().clone())
+    want, run, t, p = [], caches[3], tokens, pos.clone()
+    for step_ids in order:
+        h = ls.embed_token_ids(t, w.embedding)
+        logits, _, run = ls.llama_stack_decode_step(h, w, run, cos, sin, p, CFG, float_logits=False, adapter_ids=step_ids)
+        t, p = ls.greedy_sample(logits), p + 1
+        want.append(t)
+    assert torch.equal(torch.stack(got), torch.stack(want))
+    for a, b in zip(caches[2].layer_caches, run.layer_caches):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
