@@ -207,6 +207,12 @@ def reference_paged_gqa_decode_block_from_qkv(qkv, K_pages, V_pages, block_table
     return out, updated_K, updated_V
 
 
+def _check_rope_tables(cos, sin, D):
+    """The kernels read rows of D/2 angles: narrower tables would be read past their end."""
+    if cos.ndim != 2 or cos.shape != sin.shape or cos.shape[1] != D // 2:
+        raise ValueError(f"cos and sin must be [rows,D/2={D // 2}], got {tuple(cos.shape)}, {tuple(sin.shape)}")
+
+
 def _qkv_rope_update_prep(qkv, block_table, cos, sin, position, Hq, Hkv, D, page_size, dtype, dev):
     """Shape checks and device buffers for the fused qkv split + RoPE + paged
     write launches.  Returns (x [B,(Hq+2Hkv)*D], cos, sin, positions int32,
@@ -256,6 +262,7 @@ def paged_gqa_decode_block_from_qkv(qkv, K_pages, V_pages, block_table, cos, sin
         raise TypeError(f"K_pages/V_pages must share a float16/bfloat16 dtype, got {K_pages.dtype}, {V_pages.dtype}")
     if not (K_pages.is_contiguous() and V_pages.is_contiguous()):
         raise ValueError("K_pages and V_pages must be contiguous for the in-place update")
+    _check_rope_tables(cos, sin, D)
     dev = _lib.require_device(qkv, K_pages, V_pages, block_table)
     NUM_PAGES, P = K_pages.shape[0], K_pages.shape[1]
     MAX_BLOCKS = block_table.shape[1]

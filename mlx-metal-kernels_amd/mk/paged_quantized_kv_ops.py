@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._common import ci_safe_mode_enabled, values_only
-from .gqa_ops import _per_sequence_rope, _qkv_rope_update_prep, validate_gqa_heads
+from .gqa_ops import _check_rope_tables, _per_sequence_rope, _qkv_rope_update_prep, validate_gqa_heads
 from .kv_cache_ops import normalize_positions
 from .paged_kv_ops import _i32
 from .quant_ops import unpack_q4_reference
@@ -541,6 +541,7 @@ def paged_quantized_kv_update_from_qkv(qkv, paged_qkv: PagedQuantizedKVCache, co
     NUM_PAGES = _check_kernel_layout(paged_qkv, Hkv, D)
     P = int(paged_qkv.page_size)
     dtype = qkv.dtype if qkv.dtype in (torch.float16, torch.bfloat16) else torch.float16
+    _check_rope_tables(cos, sin, D)
     dev = _lib.require_device(qkv, paged_qkv.k_pages_q, paged_qkv.v_pages_q, paged_qkv.k_scales, paged_qkv.v_scales)
     MAX_BLOCKS = paged_qkv.block_table.shape[1]
     x, c, s, pos, q_out, B = _qkv_rope_update_prep(qkv, paged_qkv.block_table, cos, sin, position, Hq, Hkv, D, P,

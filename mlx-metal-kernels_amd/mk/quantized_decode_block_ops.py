@@ -21,6 +21,7 @@ import torch
 from . import _lib
 from ._common import ACT_DTYPES, as_u8, scales_for_kernel
 from .gqa_ops import (
+    _check_rope_tables,
     paged_gqa_decode_attention,
     paged_gqa_decode_block_from_qkv,
     paged_qk_norm_rope_update,
@@ -209,6 +210,7 @@ def rmsnorm_qkv_rope_paged_update(x2d, norm_weight, qkv_w, qkv_scales, qkv_zeros
     cols = math.ceil(K / 2) if bits == 4 else K
     if w8.ndim != 2 or tuple(w8.shape) != (N, cols):
         raise ValueError(f"qkv_w must have shape [{N},{cols}], got {tuple(w8.shape)}")
+    _check_rope_tables(cos, sin, D)
     x2d = x2d.contiguous()
     nw = norm_weight.contiguous()
     dev = _lib.require_device(x2d, nw, w8, qkv_scales, qkv_zeros, K_pages, V_pages, block_table)

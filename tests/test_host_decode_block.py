@@ -165,3 +165,30 @@ def test_adapters_refuse_gradients_beside_kernels():
     y.float().sum().backward()
     assert all(leaf.grad.abs().sum() > 0 for leaf in leaves)
     assert (x.grad[1] != 0).any()  # the row without an adapter: through the projections and the attention
+
+
+def test_tables_of_another_width_are_refused():
+    """The page writes' kernels read D/2 angles a row: tables of another width, or of two shapes, never reach them."""
+    import mk.paged_quantized_kv_ops as pq
+    from mk.quantized_decode_block_ops import rmsnorm_qkv_rope_paged_update
+
+    B, Hq, Hkv, D, P, K = 2, 2, 1, 32, 4, 32
+    N = (Hq + 2 * Hkv) * D
+    Kp, Vp = torch.zeros(2, 6, P, Hkv, D).half()
+    bt, pos = torch.arange(6, dtype=torch.int32).reshape(2, 3), torch.tensor([5, 2])
+    kw = dict(num_attention_heads=Hq, num_key_value_heads=Hkv, head_dim=D)
+    cache = pq.quantize_kv_pages(Kp, Vp, bt, torch.tensor([6, 3]), pq.PagedQuantizedKVConfig(page_size=P))
+    w, sc = torch.zeros(N, K // 2, dtype=torch.uint8), torch.ones(N, K // 32).half()
+    qkv = torch.zeros(B, 1, N).half()
+    calls = [lambda c, s: gqa.paged_gqa_decode_block_from_qkv(qkv, Kp, Vp, bt, c, s, pos, **kw),
+             lambda c, s: rmsnorm_qkv_rope_paged_update(torch.zeros(B, K).half(), torch.ones(K).half(), w, sc, None, Kp,
+                                                        Vp, bt, c, s, pos, **kw),
+             lambda c, s: pq.paged_quantized_kv_update_from_qkv(qkv, cache, c, s, pos, **kw)]
+    cos = torch.ones(12, D // 2)
+    for call in calls:
+        for c, s in ((cos[:, :8], cos[:, :8]), (cos, cos[:, :8]), (cos, cos[:5]), (torch.ones(12, D), torch.ones(12, D)),
+                     (cos[0], cos[0])):
+            with pytest.raises(ValueError, match="cos and sin must be"):
+                call(c, s)
+        with pytest.raises(ValueError, match="ROCm device"):
+            call(cos, cos)
