@@ -136,20 +136,25 @@ class LlamaLayerKernelWeights:
     down_zeros: Any | None = None
     bits: int = 4
     group_size: int = 32
-    # beyond the reference: norms of q and k heads [head_dim], the rotary layout ("interleaved" or "half"; the
-    # tables' width says how much of a head turns), adapters (lora_ops.LoraAdapters) beside qkv and o
+    # beyond the reference: norms of q and k heads [head_dim], the rotary layout ("interleaved" or "half"), adapters
+    # (lora_ops.LoraAdapters) beside qkv and o, how many values of a head turn (tables of another width are refused;
+    # None: as many as the tables have where norms or the half layout are given, all of them in an ordinary layer)
     q_norm_weight: Any | None = None
     k_norm_weight: Any | None = None
     rope_layout: str = "interleaved"
     qkv_lora: Any | None = None
     o_lora: Any | None = None
+    rotary_dim: int | None = None
 
     def block_options(self, cos, config: LlamaLikeConfig, adapter_ids=None) -> dict:
         """What the decode block takes for these fields (nothing for a layer without them)."""
         out = {}
-        if self.q_norm_weight is not None or self.k_norm_weight is not None:
+        norms = self.q_norm_weight is not None or self.k_norm_weight is not None
+        if norms:
             out.update(q_norm_weight=self.q_norm_weight, k_norm_weight=self.k_norm_weight)
-        if self.rope_layout != "interleaved" or 2 * cos.shape[1] != config.head_dim:
+        if self.rotary_dim is not None:
+            out.update(rope_layout=self.rope_layout, rotary_dim=self.rotary_dim)
+        elif norms or self.rope_layout != "interleaved":
             out.update(rope_layout=self.rope_layout, rotary_dim=2 * cos.shape[1])
         if adapter_ids is not None:
             out.update(qkv_lora=self.qkv_lora, out_lora=self.o_lora, adapter_ids=adapter_ids)

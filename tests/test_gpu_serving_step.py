@@ -501,3 +501,26 @@ def test_plain_loop_and_graph_with_adapters(dev, adapted):
     assert torch.equal(torch.stack(got), torch.stack(want))
     for a, b in zip(caches[2].layer_caches, run.layer_caches):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_layer_with_part_rotation(dev):
+    """An ordinary layer whose ``rotary_dim`` is part of a head, against its reference backend; without the field,
+    narrower tables are refused before anything is launched."""
+    w, (cos, sin) = _plain_weights(dev, ("qkv", "o"))
+    w, part = w.layers[0], build_scaled_rope_tables(CFG.max_position_embeddings, ROTARY, device=dev)
+    cache = _filled(dev, 5, 48)[0]
+    x = torch.randn(5, 1, CFG.hidden_size, device=dev).half()
+    pos = torch.tensor([0, 47, 16, 15, 30], dtype=torch.int32, device=dev)
+    for ids in (None, torch.tensor([2, -1, 0, 1, 2], dtype=torch.int32, device=dev)):
+        kw = dict(cache_layout="paged", adapter_ids=ids)
+        with pytest.raises(ValueError, match="cos and sin must be"):
+            ll.llama_layer_decode_step(x, w, cache, *part, pos, CFG, **kw)
+        w.rotary_dim = ROTARY
+        with pytest.raises(ValueError, match="cos and sin must be"):
+            ll.llama_layer_decode_step(x, w, cache, cos, sin, pos, CFG, **kw)
+        ref, ref_cache = ll.reference_llama_layer_decode_step(x, w, cache, *part, pos, CFG, **kw)
+        got, got_cache = ll.llama_layer_decode_step(x, w, tuple(t.clone() for t in cache), *part, pos, CFG, **kw)
+        assert_close(got, ref.float().cpu().numpy(), what="layer")
+        for a, b in zip(got_cache[:2], ref_cache[:2]):
+            assert_close(a, b.float().cpu().numpy(), what="cache")
+        w.rotary_dim = None

@@ -192,3 +192,50 @@ def test_tables_of_another_width_are_refused():
                 call(c, s)
         with pytest.raises(ValueError, match="ROCm device"):
             call(cos, cos)
+
+
+def test_layer_tables_say_no_more_than_its_weights():
+    """An ordinary layer takes tables of whole heads only; part of a head turns where ``rotary_dim`` says so, or where
+    head norms or the half layout leave it to the tables."""
+    from mk import llama_layer_ops as ll
+
+    cfg = ll.LlamaLikeConfig(hidden_size=64, intermediate_size=128, num_attention_heads=2, num_key_value_heads=1,
+                             head_dim=32, num_hidden_layers=1, max_position_embeddings=16, vocab_size=64).validate()
+    g = torch.Generator().manual_seed(1)
+    linears = {}
+    for name, n, k in (("qkv", 128, 64), ("o", 64, 64), ("gate", 128, 64), ("up", 128, 64), ("down", 64, 128)):
+        linears[name + "_w"] = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+        linears[name + "_scales"] = (0.02 * (1 + torch.rand(n, k // 32, generator=g))).half()
+        linears[name + "_zeros"] = torch.full((n, k // 32), 8.0).half()
+    w = ll.LlamaLayerKernelWeights(input_layernorm_weight=torch.ones(64).half(),
+                                   post_attention_layernorm_weight=torch.ones(64).half(), **linears)
+    cos, sin = ll.build_rope_tables(cfg)
+    part = cos[:, :8].contiguous(), sin[:, :8].contiguous()
+    cache = ll.init_llama_layer_cache(cfg, 2, 16, cache_layout="contiguous", device="cpu")
+    x = torch.randn(2, 1, 64, generator=torch.Generator().manual_seed(0)).half()
+    ends = torch.ones(16, 8), torch.zeros(16, 8)  # angles of pairs 8 .. 15: they stay
+
+    def step(tables):
+        return ll.reference_llama_layer_decode_step(x, w, cache, *tables, 3, cfg, cache_layout="contiguous")
+
+    whole, _ = step((cos, sin))
+    for c, s in (part, (torch.cat([cos, cos], 1), torch.cat([sin, sin], 1))):
+        with pytest.raises(ValueError):
+            step((c, s))
+        with pytest.raises(ValueError):
+            ll.llama_layer_decode_step(x, w, cache, c, s, 3, cfg, cache_layout="contiguous")
+    w.rotary_dim = 16
+    got, (K, _) = step(part)
+    with pytest.raises(ValueError, match="cos and sin must be"):
+        step((cos, sin))
+    w.rotary_dim = 32
+    assert torch.equal(step((cos, sin))[0], whole)
+    with pytest.raises(ValueError):
+        step(part)
+    w.rotary_dim = None
+    want, (Kw, _) = step((torch.cat([part[0], ends[0]], 1), torch.cat([part[1], ends[1]], 1)))
+    assert torch.equal(got, want) and torch.equal(K, Kw) and not torch.equal(got, whole)
+    w.rope_layout = "half"
+    half, _ = step(part)
+    w.rotary_dim = 16
+    assert torch.equal(step(part)[0], half)
