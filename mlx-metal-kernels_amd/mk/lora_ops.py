@@ -35,7 +35,13 @@ class LoraAdapters:
     scales: Any | None = None
 
 
-def _validate(x, base, lora_a, lora_b, adapter_ids, scales, out):
+def _check_out(out, base):
+    if out is not None and (out.shape != base.shape or out.dtype != base.dtype or out.device != base.device):
+        raise ValueError(f"out must match base {tuple(base.shape)} {base.dtype} on {base.device}, got "
+                         f"{tuple(out.shape)} {out.dtype} on {out.device}")
+
+
+def _validate(x, base, lora_a, lora_b, adapter_ids, scales):
     """(M, N, K, R, adapters, ids [M])"""
     *rows, K = x.shape or (0,)
     *same, N = base.shape or (0,)
@@ -61,9 +67,6 @@ def _validate(x, base, lora_a, lora_b, adapter_ids, scales, out):
                         f"{lora_b.dtype}")
     if scales is not None and scales.shape != (adapters,):
         raise ValueError(f"scales must have shape {(adapters,)}, got {tuple(scales.shape)}")
-    if out is not None and (out.shape != base.shape or out.dtype != base.dtype or out.device != base.device):
-        raise ValueError(f"out must match base {tuple(base.shape)} {base.dtype} on {base.device}, got "
-                         f"{tuple(out.shape)} {out.dtype} on {out.device}")
     M = math.prod(rows)
     if not isinstance(adapter_ids, torch.Tensor):
         adapter_ids = torch.as_tensor(adapter_ids, dtype=torch.int32)
@@ -89,7 +92,7 @@ def _validate(x, base, lora_a, lora_b, adapter_ids, scales, out):
 
 def reference_lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None):
     """``lora_add`` with tensor ops, an adapter at a time."""
-    M, N, K, R, adapters, ids = _validate(x, base, lora_a, lora_b, adapter_ids, scales, None)
+    M, N, K, R, adapters, ids = _validate(x, base, lora_a, lora_b, adapter_ids, scales)
     x2, out = x.reshape(M, K).float(), base.reshape(M, N).float()
     for i in range(adapters):
         d = (x2 @ lora_a[i].float().t()) @ lora_b[i].float().t()
@@ -140,11 +143,12 @@ def lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None, out=None, bac
     backend_name = backend.lower()
     if backend_name not in ("auto", "reference", "metal"):
         raise ValueError("backend must be one of 'reference', 'metal', 'auto'")
+    _check_out(out, base)
     tensors = (x, base, lora_a, lora_b) if scales is None else (x, base, lora_a, lora_b, scales)
     if backend_name == "reference" or ci_safe_mode_enabled() or not values_only(*tensors):
         y = reference_lora_add(x, base, lora_a, lora_b, adapter_ids, scales=scales)
         return y if out is None else out.copy_(y)
-    M, N, K, R, adapters, ids = _validate(x, base, lora_a, lora_b, adapter_ids, scales, out)
+    M, N, K, R, adapters, ids = _validate(x, base, lora_a, lora_b, adapter_ids, scales)
     if M > MAX_ROWS or N > MAX_OUTPUTS:
         raise ValueError(f"at most {MAX_ROWS} rows and {MAX_OUTPUTS} outputs, got {M}, {N}")
     dev = _lib.require_device(x, base, lora_a, lora_b, scales)

@@ -191,3 +191,18 @@ def test_quantized_lora_linear_gradients(bits, backend):
     assert (tangent.double() - want).abs().max() <= 8 * 2.0 ** -11 * want.abs().max()
     with pytest.raises(ValueError, match="backend must be one of"):
         lo.quantized_lora_linear(leaves[0], w, sc, z, a, b, ids, **{**kw, "backend": "x"})
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_out_of_another_shape_or_type(grad):
+    """The tensor ops take no ``out`` that the kernels would refuse: nothing is broadcast or cast into it."""
+    x, base, a, b, ids, s = lora_case(6, 4, 6, 8, 2, 3, torch.float16)
+    kw = dict(backend="auto") if grad else dict(backend="reference")
+    a.requires_grad_(grad)
+    for out in (torch.zeros(2, 4, 6).half(), torch.zeros(4, 6), torch.zeros(4, 6).bfloat16(), torch.zeros(24).half()):
+        with pytest.raises(ValueError, match="out must match base"):
+            lo.lora_add(x, base, a, b, ids, scales=s, out=out, **kw)
+        assert not out.any()
+    out = torch.zeros(4, 6).half()
+    assert lo.lora_add(x, base, a, b, ids, scales=s, out=out, **kw) is out
+    assert torch.equal(out, lo.lora_add(x, base, a, b, ids, scales=s, backend="reference"))
