@@ -95,10 +95,13 @@ def reference_lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None):
     M, N, K, R, adapters, ids = _validate(x, base, lora_a, lora_b, adapter_ids, scales)
     x2, out = x.reshape(M, K).float(), base.reshape(M, N).float()
     for i in range(adapters):
-        d = (x2 @ lora_a[i].float().t()) @ lora_b[i].float().t()
+        # other rows are zeros in both products: what is not finite in them would reach this adapter's gradients as 0 * inf
+        own = (ids == i)[:, None]
+        t = torch.where(own, torch.where(own, x2, 0.0) @ lora_a[i].float().t(), 0.0)
+        d = t @ lora_b[i].float().t()
         if scales is not None:
             d = d * scales[i].float()
-        out = torch.where((ids == i)[:, None], out + d, out)
+        out = torch.where(own, out + d, out)
     return out.to(base.dtype).reshape(base.shape)
 
 

@@ -206,3 +206,26 @@ def test_out_of_another_shape_or_type(grad):
     out = torch.zeros(4, 6).half()
     assert lo.lora_add(x, base, a, b, ids, scales=s, out=out, **kw) is out
     assert torch.equal(out, lo.lora_add(x, base, a, b, ids, scales=s, backend="reference"))
+
+
+def test_gradients_beside_rows_that_are_not_finite():
+    """What stands in a padding row or in another adapter's rows touches no gradient of an adapter or a finite row."""
+    x, base, a, b, ids, s = lora_case(7, 8, 6, 10, 3, 3, torch.float16)
+    ids = torch.tensor([0, 1, -1, 0, 2, 1, -1, 0], dtype=torch.int32)
+    g = torch.randn(8, 6, generator=torch.Generator().manual_seed(3)).half()
+    clean = [t.clone().requires_grad_() for t in (x, base, a, b, s)]
+    lo.lora_add(*clean[:4], ids, scales=clean[4]).backward(g)
+    x[2], x[6, 3], x[4, 1] = float("nan"), float("inf"), float("-inf")  # two padding rows, the row of adapter 2
+    leaves = [t.clone().requires_grad_() for t in (x, base, a, b, s)]
+    y = lo.lora_add(*leaves[:4], ids, scales=leaves[4])
+    y.backward(g)
+    fine = ids != 2
+    assert torch.equal(y[ids < 0], base[ids < 0])
+    assert torch.equal(leaves[0].grad[fine], clean[0].grad[fine]) and (leaves[0].grad[ids < 0] == 0).all()
+    for k in (2, 3):
+        assert torch.equal(leaves[k].grad[:2], clean[k].grad[:2])
+    assert torch.equal(leaves[4].grad[:2], clean[4].grad[:2])
+    a[2, 1, 4] = float("inf")  # an adapter that no finite row has
+    leaves = [t.clone().requires_grad_() for t in (x, base, a, b, s)]
+    lo.lora_add(*leaves[:4], torch.where(ids == 2, -1, ids), scales=leaves[4]).backward(g)
+    assert all((leaves[k].grad[2] == 0).all() for k in (2, 3, 4)) and leaves[0].grad.isfinite().all()
