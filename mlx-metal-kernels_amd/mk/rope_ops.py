@@ -92,7 +92,8 @@ def _validate_positions(positions, B: int, S: int, rows: int, device):
     if shape != (B,) and shape != (B, S):
         raise ValueError(f"positions must have shape [B]={(B,)} or [B,S]={(B, S)}, got {tuple(positions.shape)}")
     if positions.numel() and host_checks_enabled(positions):
-        lo, hi = int(positions.min()), int(positions.max()) + (S if positions.ndim == 1 else 1)
+        lo, hi = int(positions.min()), int(positions.max())
+        hi += S if positions.ndim == 1 and hi >= 0 else 1  # (a padding sequence has no further rows)
         if lo < -1 or hi > rows:
             raise ValueError(f"positions must be in [-1, {rows}) with S={S}, got {lo} to {hi - 1}")
     return narrow_i32(positions, device)

@@ -251,3 +251,14 @@ def test_qk_one_position_for_all_rows():
     for bad in (torch.tensor(12), torch.tensor(-2), torch.tensor(1.0), torch.tensor([5]), [5]):
         with pytest.raises(ValueError, match="position must be"):
             gqa.paged_qk_norm_rope_update(qkv, K, V, bt, cos, sin, bad, backend="reference", **c)
+
+
+def test_rope_of_padding_alone():
+    """A batch whose sequences are all padding is zeros, also where they are longer than the tables."""
+    cos, sin = rope.build_rope_tables(4, 8)
+    x = torch.ones(2, 9, 1, 8).half()
+    for pos in (torch.tensor([-1, -1]), torch.full((2, 9), -1)):
+        assert not rope.apply_rope(x, cos, sin, positions=pos, backend="reference").any()
+    for pos in (torch.tensor([-1, 0]), torch.tensor([-1, -2]), torch.full((2, 9), 4)):
+        with pytest.raises(ValueError, match="positions must be in"):
+            rope.apply_rope(x, cos, sin, positions=pos, backend="reference")
