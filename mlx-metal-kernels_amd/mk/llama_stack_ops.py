@@ -333,6 +333,12 @@ class DecodeGraph:
                  config: LlamaLikeConfig, token_ids, positions, *, adapter_ids=None):
         if stack_weights.embedding is None or stack_weights.lm_head is None:
             raise ValueError("DecodeGraph needs an embedding and an lm_head")
+        if adapter_ids is not None:  # a host copy cannot be captured, and would not be read anew
+            if not isinstance(adapter_ids, torch.Tensor) or adapter_ids.device != token_ids.device:
+                raise ValueError(f"adapter_ids must be a tensor on the tokens' device {token_ids.device}")
+            if adapter_ids.dtype not in (torch.int32, torch.int64) or adapter_ids.shape != token_ids.shape:
+                raise ValueError(f"adapter_ids must be int32 {tuple(token_ids.shape)}, got {adapter_ids.dtype} "
+                                 f"{tuple(adapter_ids.shape)}")
         self.w, self.cache, self.cos, self.sin, self.config = stack_weights, stack_cache, cos, sin, config
         self.tokens = token_ids.clone()
         self.positions = positions.to(torch.int32).clone()

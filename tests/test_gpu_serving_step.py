@@ -524,3 +524,26 @@ def test_layer_with_part_rotation(dev):
         for a, b in zip(got_cache[:2], ref_cache[:2]):
             assert_close(a, b.float().cpu().numpy(), what="cache")
         w.rotary_dim = None
+
+
+def test_graph_refuses_ids_that_it_cannot_read_anew(dev):
+    """Adapter ids on the host, as a list or of another shape are refused before the capture begins; int64 ones are read
+    anew by every replay."""
+    w, (cos, sin) = _weights(dev), _tables(dev)
+    tokens, pos = torch.tensor([3, 5], device=dev), torch.zeros(2, dtype=torch.int32, device=dev)
+
+    def cache():
+        return ls.LlamaStackCache([ll.init_llama_layer_cache(CFG, 2, 32, cache_layout="paged", device=dev)
+                                   for _ in range(CFG.num_hidden_layers)], "paged", 32, 16)
+
+    for ids in ([0, 1], torch.tensor([0, 1]), torch.tensor([0], device=dev), torch.tensor([0.0, 1.0], device=dev)):
+        with pytest.raises(ValueError, match="adapter_ids must be"):
+            ls.DecodeGraph(w, cache(), cos, sin, CFG, tokens, pos, adapter_ids=ids)
+    runs = []
+    for dtype in (torch.int32, torch.int64):
+        ids = torch.tensor([0, -1], dtype=dtype, device=dev)
+        graph = ls.DecodeGraph(w, cache(), cos, sin, CFG, tokens, pos, adapter_ids=ids)
+        out = [graph.first_tokens.clone(), graph.step().clone()]
+        ids.copy_(torch.tensor([2, 1]))
+        runs.append(torch.stack(out + [graph.step().clone() for _ in range(4)]))
+    assert torch.equal(*runs)
