@@ -262,3 +262,28 @@ def test_rope_of_padding_alone():
     for pos in (torch.tensor([-1, 0]), torch.tensor([-1, -2]), torch.full((2, 9), 4)):
         with pytest.raises(ValueError, match="positions must be in"):
             rope.apply_rope(x, cos, sin, positions=pos, backend="reference")
+
+
+def test_scaled_tables_between_the_ends():
+    """The pairs on the ramps of llama3 and yarn, worked out by hand from their definitions.
+
+    llama3, theta 10000, d 8, factor 8, 1 to 4 turns over 128 positions: pair 1 (0.1 a position) turns 12.8 / 2 pi =
+    2.0371833 times, so 1.0371833 / 3 = 0.34572776 of its frequency stays and the rest is divided by 8: 0.1 (0.34572776 +
+    0.65427224 / 8 = 0.08178403) = 0.042751179.  Pair 0 (20.4 turns) stays, pairs 2 and 3 (0.2 and 0.02) are divided.
+
+    yarn, theta 10000, d 16, factor 4, 4096 positions: the pairs of 32 turns and of one are 16 ln(4096 / 64 pi) / (2 ln
+    10000) = 2.62 and 16 ln(4096 / 2 pi) / (2 ln 10000) = 5.63, outwards 2 and 6; pair i in between keeps 1 - 0.75 (i - 2)
+    / 4 of 10000^(-i / 8), and cos and sin are multiplied by 0.1 ln 4 + 1."""
+    cases = [(8, {"type": "llama3", "factor": 8, "low_freq_factor": 1, "high_freq_factor": 4,
+                  "original_max_position": 128}, [1.0, 0.042751179, 0.00125, 0.000125], 1.0),
+             (16, {"type": "yarn", "factor": 4, "original_max_position": 4096},
+              [1.0, 0.31622777, 0.1, 0.031622777 * 0.8125, 0.01 * 0.625, 0.0031622777 * 0.4375, 0.00025,
+               0.00031622777 / 4], 1.13862944)]
+    for d, scaling, inv, gain in cases:
+        c, s = rope.build_scaled_rope_tables(41, d, 10000.0, scaling=scaling)
+        for p in (1, 7, 40):
+            angles = p * np.array(inv)
+            # eight digits of a frequency, and the table's rounding
+            lim = 40 * 2e-8 * np.maximum(np.array(inv), 1e-3) * gain + 2.0 ** -24 * gain
+            assert (np.abs(c[p].numpy() - gain * np.cos(angles)) <= lim).all(), (scaling, p)
+            assert (np.abs(s[p].numpy() - gain * np.sin(angles)) <= lim).all(), (scaling, p)
