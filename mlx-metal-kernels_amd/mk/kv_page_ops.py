@@ -166,7 +166,10 @@ def fork_kv_sequences(pages, block_table, lengths, ref_counts, parents, *, reser
     are free and may have been given away.  ``ready`` is false for a row whose
     pages did not suffice or whose table row is full: it got none, still shares
     its last page, reads as its parent did, and must not be appended to before
-    another call says it is ready.  n = len(parents) <= 4096.
+    another call says it is ready.  A row that needs no pages is ready also
+    behind one whose pages did not suffice.  An empty row has no pages and may
+    stay in a batch at position 0: a decode step writes and reads nothing for
+    it.  n = len(parents) <= 4096.
 
     ``page_size`` is needed only without page arrays (``pages=[]``: the tables
     alone).  Entries, counts and parents are checked on the host unless that is

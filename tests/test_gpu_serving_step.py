@@ -547,3 +547,52 @@ def test_graph_refuses_ids_that_it_cannot_read_anew(dev):
         ids.copy_(torch.tensor([2, 1]))
         runs.append(torch.stack(out + [graph.step().clone() for _ in range(4)]))
     assert torch.equal(*runs)
+
+
+@pytest.mark.parametrize("kind", ["plain", "norms", "norms at -1"])
+def test_steps_with_ended_rows(dev, kind):
+    """Rows that a fork has ended (parent -1) stay in the batch at position 0, without pages: nothing is written or read
+    for them, their outputs are finite, and the other rows give what they give without them, bit by bit the same whatever
+    the ended rows hold.  Layers with head norms take them at position -1 too; ordinary ones refuse that, as the reference does."""
+    torch.manual_seed(1)
+    w, tables = _plain_weights(dev, ("qkv", "o")) if kind == "plain" else (_weights(dev), _tables(dev))
+    P, blocks, NP, L, D = 8, 4, 30, CFG.num_hidden_layers, CFG.head_dim
+    pages = [torch.randn(NP, P, CFG.num_key_value_heads, D, device=dev).half() for _ in range(2 * L)]
+    table = torch.full((4, blocks), -1, dtype=torch.int32, device=dev)
+    table[:, :3] = torch.randperm(NP, device=dev)[:12].reshape(4, 3).int()
+    lengths = torch.tensor([21, 9, 17, 24], dtype=torch.int32, device=dev)
+    refs = kv_page_ops.count_page_refs(table, NP)
+    parents = torch.tensor([2, -1, 0, 2, -1], dtype=torch.int32, device=dev)
+    table, lengths, refs, ready = kv_page_ops.fork_kv_sequences(pages, table, lengths, refs, parents)
+    live = parents >= 0
+    assert all(ready.tolist()) and (table[~live] == -1).all() and not lengths[~live].any()
+    x = torch.randn(5, 1, CFG.hidden_size, device=dev).half()
+    ids = torch.tensor([0, 1, -1, 2, 0], dtype=torch.int32, device=dev)
+
+    def step(rows, position):
+        pool = [t.clone() for t in pages]
+        cache = ls.LlamaStackCache([(pool[2 * i], pool[2 * i + 1], table[rows].contiguous()) for i in range(L)], "paged",
+                                   blocks * P, P)
+        logits, hidden, _ = ls.llama_stack_decode_step(x[rows], w, cache, *tables, position, CFG, adapter_ids=ids[rows])
+        return logits, hidden, pool
+
+    position = torch.where(live, lengths, -1) if kind == "norms at -1" else lengths
+    all_rows = torch.ones_like(live)
+    logits, hidden, pool = step(all_rows, position)
+    assert logits.isfinite().all()
+    # (a step of fewer rows may take other matvec kernels)
+    want_logits, want_hidden, want_pool = step(live, lengths[live])
+    for got, want in ((logits[live], want_logits), (hidden[live], want_hidden)):
+        assert_close(got.float().cpu().numpy(), want.float().cpu().numpy(), what="live rows")
+    written = torch.zeros(NP, P, dtype=torch.bool, device=dev)
+    for b in live.nonzero().flatten().tolist():
+        written[table[b, int(lengths[b]) // P], int(lengths[b]) % P] = True
+    for a, before, b in zip(pool, pages, want_pool):
+        assert torch.equal(a[~written], before[~written]) and torch.equal(b[~written], before[~written])
+        assert_close(a[written].float().cpu().numpy(), b[written].float().cpu().numpy(), what="new tokens")
+    x[~live] = torch.randn_like(x[~live]) * 3
+    again = step(all_rows, position)
+    assert torch.equal(again[0][live], logits[live]) and all(torch.equal(a, b) for a, b in zip(again[2], pool))
+    if kind == "plain":
+        with pytest.raises(ValueError, match="positions must be in"):
+            step(all_rows, torch.where(live, lengths, -1))
