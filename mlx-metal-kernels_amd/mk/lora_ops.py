@@ -138,6 +138,7 @@ def lora_add(x, base, lora_a, lora_b, adapter_ids, *, scales=None, out=None, bac
     (the rows may be strided; no other overlap).  At most 2^20 - 1 rows and
     2^24 - 1 outputs.  An infinity in lora_b may come back as a NaN of its
     outputs; one in x, base or lora_a is what the formula makes of it.
+    In fp16 a value of A x below 2^-38 of the largest of its row counts as zero.
 
     ids are checked on the host unless that is off (``host_checks_enabled``);
     then one outside [0, ADAPTERS) is a row without an adapter.  Backend
