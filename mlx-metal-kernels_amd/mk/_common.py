@@ -52,6 +52,12 @@ def narrow_i32(t: torch.Tensor, device) -> torch.Tensor:
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
+def has_tangent(*tensors) -> bool:
+    """Whether one of them carries a forward-mode tangent (None: no tensor)."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def values_only(*tensors: torch.Tensor) -> bool:
     """Whether a kernel that reads the tensors' memory does all that tensor ops
     would: no gradient to record, no forward-mode tangent, no function transform

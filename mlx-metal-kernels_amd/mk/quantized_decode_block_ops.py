@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _lib
-from ._common import ACT_DTYPES, as_u8, scales_for_kernel
+from ._common import ACT_DTYPES, as_u8, has_tangent, scales_for_kernel
 from .gqa_ops import (
     _check_rope_tables,
     paged_gqa_decode_attention,
@@ -250,7 +250,7 @@ def _tensors_of(lora):
 
 def _refuse_gradient(*tensors):
     """Beside launches that leave no graph ``lora_add`` would give a result whose gradient is the adapters' part alone."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if has_tangent(*tensors) or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("the decode block's kernels record no gradient; with adapters, call it under torch.no_grad() "
                            "or with both backends 'reference'")
 

@@ -287,3 +287,18 @@ def test_scaled_tables_between_the_ends():
             lim = 40 * 2e-8 * np.maximum(np.array(inv), 1e-3) * gain + 2.0 ** -24 * gain
             assert (np.abs(c[p].numpy() - gain * np.cos(angles)) <= lim).all(), (scaling, p)
             assert (np.abs(s[p].numpy() - gain * np.sin(angles)) <= lim).all(), (scaling, p)
+
+
+def test_qk_refuses_tangents():
+    """A forward-mode tangent would be lost by the kernel as a gradient would."""
+    import torch.autograd.forward_ad as fwad
+
+    qkv, K, V, bt, cos, sin, pos, c = qk_case(7, 3, 3, 4, 2, 16, 8, 4, 3, torch.float16)
+    with fwad.dual_level():
+        for name in ("qkv", "cos", "q_weight"):
+            ok = dict(qkv=qkv, K_pages=K, V_pages=V, block_table=bt, cos=cos, sin=sin, position=pos, **c)
+            ok[name] = fwad.make_dual(ok[name], torch.ones_like(ok[name]))
+            with torch.no_grad(), pytest.raises(RuntimeError, match="records no gradient"):
+                gqa.paged_qk_norm_rope_update(**ok)
+        with pytest.raises(ValueError, match="ROCm device"):
+            gqa.paged_qk_norm_rope_update(qkv, K, V, bt, cos, sin, pos, **c)
