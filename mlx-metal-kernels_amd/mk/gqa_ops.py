@@ -18,6 +18,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _contig, _lib
 from ._common import ACT_DTYPES, ci_safe_mode_enabled, has_tangent, narrow_i32
@@ -433,9 +434,10 @@ def paged_qk_norm_rope_update(qkv, K_pages, V_pages, block_table, cos, sin, posi
                                      k_weight, sequences, layout, rotary_dim)
     if not (K_pages.is_contiguous() and V_pages.is_contiguous()):
         raise ValueError("K_pages and V_pages must be contiguous for the in-place update")
-    if has_tangent(x, K_pages, V_pages, cos, sin, q_weight, k_weight) or torch.is_grad_enabled() and (
+    if (forward_ad._current_level >= 0 and has_tangent(x, K_pages, V_pages, cos, sin, q_weight, k_weight)
+            or torch.is_grad_enabled() and (
             x.requires_grad or K_pages.requires_grad or V_pages.requires_grad or cos.requires_grad or sin.requires_grad
-            or (q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad))):
+            or (q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad)))):
         raise RuntimeError("paged_qk_norm_rope_update records no gradient; call it under torch.no_grad()")
     dev = _lib.require_device(x, K_pages, V_pages, block_table, q_weight, k_weight)
     T, N = x.shape
